@@ -79,7 +79,7 @@ def draw(rng):
                         docs=rng.choice([0, 0, 3, 17]) if tq == tk and tk >= 32 else 0, train=train)
             scores = case["b"] * h * tq * tk
             most = 1.5e8 if dtype == "fp32" else 5e8
-            if 1e4 <= scores * d <= 3.4e10 and scores <= most and case["b"] * tk * g * d <= 1e8:
+            if 1e4 <= scores * d and scores <= most and work(case)["flops"] <= 4.8e11 and work(case)["bytes"] <= 1.3e9:
                 return case
         else:
             case = dict(kind=kind, dtype=dtype, n=_log_uniform(rng, 1, 16384), c=_log_uniform(rng, 2, 200000), top=rng.choice([0, 1, 5, 20]),
