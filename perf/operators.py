@@ -66,7 +66,7 @@ def draw(rng):
         if kind == "norm":
             case = dict(kind=kind, dtype=dtype, b=_log_uniform(rng, 1, 64), t=_log_uniform(rng, 1, 16384), h=h, g=g, d=d,
                         rot=rng.choice([d, d, d // 2]), layout=rng.choice(["half", "interleaved"]), grid=rng.random() < 0.3, train=train)
-            if 500 <= case["b"] * case["t"] * (h + g) * d <= 1.6e8:
+            if case["b"] * case["t"] * (h + g) * d >= 500 and work(case)["bytes"] <= 1.3e9:
                 return case
         elif kind == "attn":
             tk = _log_uniform(rng, 2 if train else 1, 16384)  # (over one key the gradients of q and k are zero)
@@ -85,7 +85,7 @@ def draw(rng):
             case = dict(kind=kind, dtype=dtype, n=_log_uniform(rng, 1, 16384), c=_log_uniform(rng, 2, 200000), top=rng.choice([0, 1, 5, 20]),
                         train=train)
             case["top"] = min(case["top"], case["c"])
-            if 500 <= case["n"] * case["c"] <= 2.6e8:
+            if 500 <= case["n"] * case["c"] <= 1.6e8:
                 return case
 
 
