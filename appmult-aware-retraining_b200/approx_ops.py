@@ -112,6 +112,23 @@ def _load():
     lib.lutgemm_backward_f32lut_scratch_bytes.argtypes = [ci, ci, ci, ci]
     lib.lutgemm_backward_f32lut.restype = ci
     lib.lutgemm_backward_f32lut.argtypes = [vp, vp, vp, vp, vp, vp, vp, ci, ci, ci, ci, vp, sz, vp]
+    lib.lutgemm_norm_rotate.restype = ci
+    lib.lutgemm_norm_rotate.argtypes = [vp, cl, cl, cl] * 2 + [vp] * 4 + [ci] + [vp] * 3 + [ci] * 8 + [cf, vp]
+    lib.lutgemm_norm_rotate_backward_scratch_bytes.restype = sz
+    lib.lutgemm_norm_rotate_backward_scratch_bytes.argtypes = [ci]
+    lib.lutgemm_norm_rotate_backward.restype = ci
+    lib.lutgemm_norm_rotate_backward.argtypes = [vp, cl, cl, cl] * 4 + [vp] * 4 + [ci] + [vp] * 5 + [ci] * 8 + [cf, vp, sz, vp]
+    masks = [cf, cf, vp, ci, vp, vp, cl, vp, cl]
+    lib.lutgemm_attention.restype = ci
+    lib.lutgemm_attention.argtypes = [vp, cl, cl, cl] * 3 + [vp, vp] + [ci] * 7 + masks + [vp]
+    lib.lutgemm_attention_backward.restype = ci
+    lib.lutgemm_attention_backward.argtypes = [vp, cl, cl, cl] * 4 + [vp] * 6 + [ci] * 7 + masks + [vp]
+    lib.lutgemm_token_logprobs_scratch_bytes.restype = sz
+    lib.lutgemm_token_logprobs_scratch_bytes.argtypes = [cl, ci, ci]
+    lib.lutgemm_token_logprobs.restype = ci
+    lib.lutgemm_token_logprobs.argtypes = [vp, ci, cl, cl, ci, vp, ctypes.c_longlong, ci] + [vp] * 6 + [sz, vp]
+    lib.lutgemm_token_logprobs_backward.restype = ci
+    lib.lutgemm_token_logprobs_backward.argtypes = [vp, ci, cl, cl, ci, vp, ctypes.c_longlong] + [vp] * 5
     lib.lutgemm_set_tma.restype = ci
     lib.lutgemm_set_tma.argtypes = [ci]
     lib.lutgemm_set_handover.restype = ci

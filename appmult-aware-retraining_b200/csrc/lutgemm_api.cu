@@ -1,5 +1,6 @@
 // C ABI of liblutgemm_b200.so (declared in include/lutgemm.h): argument validation and dispatch.
 #include <cuda_runtime.h>
+#include <math.h>
 #include <stdio.h>
 #include <stdlib.h>
 #include <string.h>
@@ -8,6 +9,7 @@
 #include <atomic>
 
 #include "lutgemm.h"
+#include "lutgemm_attention.cuh"
 #include "lutgemm_common.cuh"
 #include "lutgemm_kernels.h"
 
@@ -1080,6 +1082,136 @@ int lutgemm_conv2d_layer_pass(const float *x, long x_sb, long x_sc, long x_sh, l
     if (rc != LUTGEMM_OK) return rc;
     return lutgemm_conv2d_forward_layer(codes, wmat, lut, bits, B, C, H, W, Cout, kh, kw, stride, pad, dil, box, sumw_t, taps,
                                         quant, quant + 2, quant + 1, quant + 3, bias, out, scratch, scratch_bytes, stream);
+}
+
+// ---- transformer blocks and classifier outputs ---------------------------------------------------------------------------
+
+static bool dtype_supported(int dtype) { return dtype == LUTGEMM_F32 || dtype == LUTGEMM_BF16 || dtype == LUTGEMM_F16; }
+
+static int norm_rotate_args(lutgemm::NormRotate *n, const void *q, long q_sb, long q_st, long q_sh, const void *k, long k_sb, long k_st,
+                            long k_sh, const float *qw, const float *kw, const float *cos, const float *sin, int table, const int *pos,
+                            void *q_out, void *k_out, int dtype, int B, int T, int H, int G, int D, int rot, int interleaved, float eps) {
+    if (!q || !k || !q_out || !k_out || !dtype_supported(dtype)) return LUTGEMM_E_BADARG;
+    if (B <= 0 || T <= 0 || H <= 0 || G <= 0 || D <= 0 || D % 2 || rot < 0 || rot % 2 || rot > D || table < 0 || !(eps >= 0.f))
+        return LUTGEMM_E_BADARG;
+    if (rot > 0 && (!cos || !sin || (!pos && table < T))) return LUTGEMM_E_BADARG;
+    if (D > 256 || (long)B * T * ((long)H + G) > 0x7fffffffL) return LUTGEMM_E_TOOLARGE;
+    *n = lutgemm::NormRotate{};
+    n->x[0] = {q, q_sb, q_st, q_sh};
+    n->x[1] = {k, k_sb, k_st, k_sh};
+    n->w[0] = qw; n->w[1] = kw;
+    n->y[0] = q_out; n->y[1] = k_out;
+    n->heads[0] = H; n->heads[1] = G;
+    n->cos = cos; n->sin = sin; n->pos = pos; n->table = table;
+    n->B = B; n->T = T; n->D = D; n->rot = rot; n->interleaved = interleaved != 0; n->eps = eps;
+    return LUTGEMM_OK;
+}
+
+int lutgemm_norm_rotate(const void *q, long q_sb, long q_st, long q_sh, const void *k, long k_sb, long k_st, long k_sh, const float *qw,
+                        const float *kw, const float *cos, const float *sin, int table, const int *pos, void *q_out, void *k_out,
+                        int dtype, int B, int T, int H, int G, int D, int rot, int interleaved, float eps, void *stream) {
+    lutgemm::NormRotate n;
+    const int rc = norm_rotate_args(&n, q, q_sb, q_st, q_sh, k, k_sb, k_st, k_sh, qw, kw, cos, sin, table, pos, q_out, k_out, dtype, B, T,
+                                    H, G, D, rot, interleaved, eps);
+    if (rc != LUTGEMM_OK) return rc;
+    const int sms = current_num_sms();
+    if (sms <= 0) return LUTGEMM_E_CUDA;
+    return lutgemm::norm_rotate_forward(n, dtype, sms, static_cast<cudaStream_t>(stream));
+}
+
+size_t lutgemm_norm_rotate_backward_scratch_bytes(int D) {
+    const int sms = current_num_sms();
+    return sms <= 0 || D <= 0 ? 0 : (size_t)(lutgemm::norm_rotate_blocks(sms) + 2) * D * sizeof(float);
+}
+
+int lutgemm_norm_rotate_backward(const void *gq, long gq_sb, long gq_st, long gq_sh, const void *gk, long gk_sb, long gk_st, long gk_sh,
+                                 const void *q, long q_sb, long q_st, long q_sh, const void *k, long k_sb, long k_st, long k_sh,
+                                 const float *qw, const float *kw, const float *cos, const float *sin, int table, const int *pos,
+                                 void *dq, void *dk, float *dqw, float *dkw, int dtype, int B, int T, int H, int G, int D, int rot,
+                                 int interleaved, float eps, void *scratch, size_t scratch_bytes, void *stream) {
+    lutgemm::NormRotate n;
+    const int rc = norm_rotate_args(&n, q, q_sb, q_st, q_sh, k, k_sb, k_st, k_sh, qw, kw, cos, sin, table, pos, dq, dk, dtype, B, T, H, G,
+                                    D, rot, interleaved, eps);
+    if (rc != LUTGEMM_OK) return rc;
+    if (!gq || !gk) return LUTGEMM_E_BADARG;
+    const int sms = current_num_sms();
+    if (sms <= 0) return LUTGEMM_E_CUDA;
+    if (dqw || dkw) {
+        if (scratch_bytes < lutgemm_norm_rotate_backward_scratch_bytes(D)) return LUTGEMM_E_SCRATCH;
+        if (!scratch || (reinterpret_cast<uintptr_t>(scratch) & 3)) return LUTGEMM_E_BADARG;
+    }
+    n.g[0] = {gq, gq_sb, gq_st, gq_sh};
+    n.g[1] = {gk, gk_sb, gk_st, gk_sh};
+    n.gw[0] = dqw; n.gw[1] = dkw;
+    return lutgemm::norm_rotate_backward(n, dtype, static_cast<float *>(scratch), sms, static_cast<cudaStream_t>(stream));
+}
+
+static int attention_args(lutgemm::AttnProblem *p, int dtype, int B, int Tq, int Tk, int H, int G, int D, float scale, float cap,
+                          const float *slopes, int causal, const int *prefix, const int *doc_q, long doc_q_sb, const int *doc_k,
+                          long doc_k_sb) {
+    if (!dtype_supported(dtype) || B <= 0 || Tq <= 0 || Tk <= 0 || H <= 0 || G <= 0 || D <= 0 || H % G || D % 8) return LUTGEMM_E_BADARG;
+    if (!(cap >= 0.f) || !isfinite(cap) || !isfinite(scale) || !doc_q != !doc_k) return LUTGEMM_E_BADARG;
+    if (D > 128 || B > 65535 || G > 65535 || (long)Tq * (H / G) > 0x7fffff00L || Tk > 0x7fffff00) return LUTGEMM_E_TOOLARGE;
+    p->B = B; p->Tq = Tq; p->Tk = Tk; p->H = H; p->G = G; p->R = H / G; p->D = D;
+    p->M = Tq * p->R;
+    p->shift = Tk - Tq;
+    p->scale = scale; p->cap = cap; p->slopes = slopes;
+    p->causal = causal != 0;
+    p->prefix = causal ? prefix : nullptr;
+    p->doc_q = doc_q; p->doc_k = doc_k; p->doc_q_sb = doc_q_sb; p->doc_k_sb = doc_k_sb;
+    return LUTGEMM_OK;
+}
+
+int lutgemm_attention(const void *q, long q_sb, long q_st, long q_sh, const void *k, long k_sb, long k_st, long k_sh, const void *v,
+                      long v_sb, long v_st, long v_sh, void *out, float *lse, int dtype, int B, int Tq, int Tk, int H, int G, int D,
+                      float scale, float cap, const float *slopes, int causal, const int *prefix, const int *doc_q, long doc_q_sb,
+                      const int *doc_k, long doc_k_sb, void *stream) {
+    if (!q || !k || !v || !out || !lse) return LUTGEMM_E_BADARG;
+    lutgemm::AttnProblem p{{q, q_sb, q_st, q_sh}, {k, k_sb, k_st, k_sh}, {v, v_sb, v_st, v_sh}};
+    const int rc = attention_args(&p, dtype, B, Tq, Tk, H, G, D, scale, cap, slopes, causal, prefix, doc_q, doc_q_sb, doc_k, doc_k_sb);
+    if (rc != LUTGEMM_OK) return rc;
+    return lutgemm::attention_f32_forward(p, dtype, out, lse, static_cast<cudaStream_t>(stream));
+}
+
+int lutgemm_attention_backward(const void *go, long go_sb, long go_st, long go_sh, const void *q, long q_sb, long q_st, long q_sh,
+                               const void *k, long k_sb, long k_st, long k_sh, const void *v, long v_sb, long v_st, long v_sh,
+                               const void *out, const float *lse, float *delta, void *dq, void *dk, void *dv, int dtype, int B, int Tq,
+                               int Tk, int H, int G, int D, float scale, float cap, const float *slopes, int causal, const int *prefix,
+                               const int *doc_q, long doc_q_sb, const int *doc_k, long doc_k_sb, void *stream) {
+    if (!go || !q || !k || !v || !out || !lse || !delta || !dq || !dk || !dv) return LUTGEMM_E_BADARG;
+    lutgemm::AttnProblem p{{q, q_sb, q_st, q_sh}, {k, k_sb, k_st, k_sh}, {v, v_sb, v_st, v_sh}};
+    const int rc = attention_args(&p, dtype, B, Tq, Tk, H, G, D, scale, cap, slopes, causal, prefix, doc_q, doc_q_sb, doc_k, doc_k_sb);
+    if (rc != LUTGEMM_OK) return rc;
+    const lutgemm::AttnTensor g{go, go_sb, go_st, go_sh};
+    return lutgemm::attention_f32_backward(p, dtype, g, out, lse, delta, dq, dk, dv, static_cast<cudaStream_t>(stream));
+}
+
+size_t lutgemm_token_logprobs_scratch_bytes(long N, int C, int top) {
+    const int sms = current_num_sms();
+    return sms <= 0 || N <= 0 || C <= 0 || top < 0 ? 0 : lutgemm::logprobs_scratch_bytes(N, C, top, sms);
+}
+
+int lutgemm_token_logprobs(const void *logits, int dtype, long pitch, long N, int C, const long long *target, long long ignore, int top,
+                           float *logp, float *entropy, float *stats, float *top_logp, long long *top_index, void *scratch,
+                           size_t scratch_bytes, void *stream) {
+    if (!logits || !target || !logp || !entropy || !stats || !dtype_supported(dtype)) return LUTGEMM_E_BADARG;
+    if (N <= 0 || C <= 0 || top < 0 || top > C || (top > 0 && (!top_logp || !top_index))) return LUTGEMM_E_BADARG;
+    if (top > 32 || N > 0x7fffffffL) return LUTGEMM_E_TOOLARGE;
+    const int sms = current_num_sms();
+    if (sms <= 0) return LUTGEMM_E_CUDA;
+    const size_t need = lutgemm::logprobs_scratch_bytes(N, C, top, sms);
+    if (scratch_bytes < need) return LUTGEMM_E_SCRATCH;
+    if (need && (!scratch || (reinterpret_cast<uintptr_t>(scratch) & 7))) return LUTGEMM_E_BADARG;
+    return lutgemm::logprobs_forward(logits, dtype, pitch, N, C, target, ignore, top, logp, entropy, stats, top_logp, top_index, scratch,
+                                     sms, static_cast<cudaStream_t>(stream));
+}
+
+int lutgemm_token_logprobs_backward(const void *logits, int dtype, long pitch, long N, int C, const long long *target, long long ignore,
+                                    const float *stats, const float *g_logp, const float *g_entropy, void *grad, void *stream) {
+    if (!logits || !target || !stats || !grad || !dtype_supported(dtype) || N <= 0 || C <= 0) return LUTGEMM_E_BADARG;
+    if (N > 0x7fffffffL) return LUTGEMM_E_TOOLARGE;
+    return lutgemm::logprobs_backward(logits, dtype, pitch, N, C, target, ignore, stats, g_logp, g_entropy, grad,
+                                      static_cast<cudaStream_t>(stream));
 }
 
 }  // extern "C"

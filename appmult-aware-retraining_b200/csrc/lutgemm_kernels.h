@@ -281,4 +281,40 @@ int backward_gw(const float *gc, const uint8_t *a, const uint8_t *w, float *gw, 
                 int M, int K, int N, const ConvGeom &conv, float *scratch, int num_splits, int num_sms,
                 cudaStream_t stream);
 
+// ---- transformer blocks and classifier outputs --------------------------------------------------------------------------
+struct AttnProblem;  // lutgemm_attention.cuh
+struct AttnTensor;
+
+// lutgemm_attention_f32.cu
+int attention_f32_forward(const AttnProblem &p, int dtype, void *out, float *lse, cudaStream_t stream);
+int attention_f32_backward(const AttnProblem &p, int dtype, const AttnTensor &go, const void *out, const float *lse, float *delta, void *gq,
+                           void *gk, void *gv, cudaStream_t stream);
+
+// lutgemm_norm_rotate.cu; index 0: queries, 1: keys
+struct NormOperand {
+    const void *p;
+    long sb, st, sh;
+};
+struct NormRotate {
+    NormOperand x[2], g[2];
+    const float *w[2];
+    void *y[2];
+    float *gw[2];
+    int heads[2];
+    const float *cos, *sin;
+    const int *pos;
+    int table, B, T, D, rot, interleaved;
+    float eps;
+};
+long norm_rotate_blocks(int num_sms);  // most blocks of the backward kernel, each with D sums for the weights
+int norm_rotate_forward(const NormRotate &n, int dtype, int num_sms, cudaStream_t stream);
+int norm_rotate_backward(const NormRotate &n, int dtype, float *scratch, int num_sms, cudaStream_t stream);
+
+// lutgemm_logprobs.cu
+size_t logprobs_scratch_bytes(long N, int C, int top, int num_sms);
+int logprobs_forward(const void *x, int dtype, long pitch, long N, int C, const long long *target, long long ignore, int top, float *logp,
+                     float *entropy, float *stats, float *top_logp, long long *top_at, void *scratch, int num_sms, cudaStream_t stream);
+int logprobs_backward(const void *x, int dtype, long pitch, long N, int C, const long long *target, long long ignore, const float *stats,
+                      const float *g_logp, const float *g_entropy, void *gx, cudaStream_t stream);
+
 }  // namespace lutgemm

@@ -1,0 +1,460 @@
+// Log probability of a given class in each row of logits, the row's entropy and its most probable classes, in one pass over the
+// logits, and the gradient of the first two.
+//
+// With m the row's largest logit, a sum over the others and d_j = m - x_j >= 0:
+//     s = sum_j exp(-d_j),  u = sum_j exp(-d_j) d_j     (one occurrence of m left out of s; it adds nothing to u)
+//     log p_j = -d_j - L,  L = log1p(s);   entropy = L + U,  U = u / (1 + s);   log p_j + entropy = U - d_j
+// No difference of near values occurs, so a row in which one class has nearly all of the probability keeps its entropy and its
+// gradient, which are what is left beside it (with the sum over all classes both are lost from 1 - p = 2^-24 on).
+//     grad_j = g_logp (1[j is given] - p_j) - g_entropy p_j (log p_j + entropy);   1 - p = -expm1(log p) for the given class
+//
+// DRAM bounds both directions: logits once in, in the backward pass once more, and the gradient once out.  A block has a row, or
+// a part of one where there are few rows; every thread keeps (m, s, u) of its own values, and the block joins them.
+// The most probable classes come from the same pass at next to no cost: the k-th largest of the thread groups' largest logits is a
+// bound that at least k values reach, so only threads whose own largest value reaches it look at their values once more (a
+// few dozen of them, from the cache), and the candidates are ranked by counting.  Ties go to the lower class.  Rows with so many
+// ties that the candidates do not fit are gone through once per answer instead.
+#include "lutgemm.h"
+#include "lutgemm_attention.cuh"
+#include "lutgemm_kernels.h"
+
+namespace lutgemm {
+
+namespace {
+
+constexpr int kMaxTop = 32, kCandidates = 512;
+
+// running sums of a set of logits; the empty set has m = -inf, s = -1
+struct RowState {
+    float m, s, u;
+};
+__device__ __forceinline__ RowState empty_state() { return {-INFINITY, -1.f, 0.f}; }
+__device__ __forceinline__ RowState join(const RowState &a, const RowState &b) {
+    const RowState &x = a.m >= b.m ? a : b, &y = a.m >= b.m ? b : a;
+    if (y.m == -INFINITY) return {x.m, x.s + (y.s == -1.f ? 0.f : y.s), x.u};  // (a NaN in y.s stays)
+    const float d = x.m - y.m, e = __expf(-d), n = 1.f + y.s;
+    return {x.m, x.s + e * n, x.u + e * (y.u + d * n)};
+}
+// one more logit; -inf adds nothing, NaN makes s NaN
+__device__ __forceinline__ void add(RowState &a, float x) {
+    if (x > a.m) {
+        const float d = x - a.m, e = __expf(-d), n = 1.f + a.s;
+        if (a.m == -INFINITY) {
+            a.s = a.s == -1.f ? 0.f : a.s;
+        } else {
+            a.u = e * (a.u + d * n);
+            a.s = e * n;
+        }
+        a.m = x;
+    } else if (x != -INFINITY) {
+        const float d = a.m - x, e = __expf(-d);
+        a.s += e;
+        a.u += e * d;
+    }
+}
+
+// order of values by whole numbers: NaN above +inf, -0 as 0 (no key is all ones: that is where the search for ties begins)
+constexpr uint32_t kNanOrder = 0xfffffffeu;
+__device__ __forceinline__ uint32_t order_of(float x) {
+    if (x != x) return kNanOrder;
+    const uint32_t u = __float_as_uint(x + 0.f);
+    return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+__device__ __forceinline__ unsigned long long key_of(float x, long j) {
+    return (unsigned long long)order_of(x) << 32 | (0xffffffffu - (uint32_t)j);
+}
+__device__ __forceinline__ float value_of(unsigned long long key) {
+    const uint32_t o = (uint32_t)(key >> 32);
+    if (o == kNanOrder) return NAN;
+    return __uint_as_float(o & 0x80000000u ? o & 0x7fffffffu : ~o);
+}
+
+struct LogpArgs {
+    const void *x;
+    long pitch;
+    long N;
+    int C, top, parts, part_len;  // part_len: classes of a part
+    const long long *target;
+    long long ignore;
+    float *logp, *entropy, *stats;  // stats [N][3]: m, L, U
+    float *top_logp;
+    long long *top_at;
+    RowState *part_state;           // [N][parts]
+    unsigned long long *part_keys;  // [N][parts][top]
+};
+
+template <typename T>
+struct Wide {
+    static constexpr int n = 16 / sizeof(T);
+    uint4 raw;
+    __device__ __forceinline__ float get(int i) const {
+        const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+        if (sizeof(T) == 4) return __uint_as_float(w[i]);
+        const uint32_t h = i & 1 ? w[i >> 1] >> 16 : w[i >> 1] & 0xffffu;
+        const unsigned short hs = (unsigned short)h;
+        return to_f32<T>(*reinterpret_cast<const T *>(&hs));
+    }
+};
+
+// the values of [first, end) of a row in this thread's order: a scalar head up to the first 16-byte boundary, vectors, a scalar tail
+template <typename T, int THREADS, typename One, typename Many>
+__device__ __forceinline__ void walk(const T *x, int first, int end, One one, Many many) {
+    constexpr int n = Wide<T>::n;
+    const uintptr_t a = reinterpret_cast<uintptr_t>(x + first);
+    const int head = min(end - first, (int)(((16 - (a & 15)) & 15) / sizeof(T)));
+    const int vecs = (end - first - head) / n, tail = first + head + vecs * n;
+    if ((int)threadIdx.x < head) one(first + threadIdx.x, to_f32<T>(x[first + threadIdx.x]));
+    const uint4 *v = reinterpret_cast<const uint4 *>(x + first + head);
+    int i = threadIdx.x;
+    for (; i + 3 * THREADS < vecs; i += 4 * THREADS) {
+        Wide<T> w[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) w[k].raw = v[i + k * THREADS];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) many(first + head + (i + k * THREADS) * n, w[k]);
+    }
+    for (; i < vecs; i += THREADS) {
+        Wide<T> w;
+        w.raw = v[i];
+        many(first + head + i * n, w);
+    }
+    if (tail + (int)threadIdx.x < end) one(tail + threadIdx.x, to_f32<T>(x[tail + threadIdx.x]));
+}
+
+template <int THREADS>
+__device__ __forceinline__ void block_sync() {
+    if (THREADS == 32) __syncwarp(); else __syncthreads();
+}
+
+// the `top` largest of the candidates in order, by counting; every thread of the block
+template <int THREADS, typename Put>
+__device__ __forceinline__ void rank_out(const unsigned long long *cand, int n, int top, Put put) {
+    for (int i = threadIdx.x; i < n; i += THREADS) {
+        const unsigned long long k = cand[i];
+        int rank = 0;
+        for (int j = 0; j < n; ++j) rank += cand[j] > k;
+        if (rank < top) put(rank, k);
+    }
+}
+
+__device__ __forceinline__ void finish_row(const LogpArgs &p, long row, RowState st, float given) {
+    if (st.m == INFINITY) st.s = NAN;
+    const bool none = st.m == -INFINITY && st.s == -1.f;  // no class has any probability
+    const float L = none ? 0.f : log1pf(st.s), U = none ? 0.f : st.u / (1.f + st.s);
+    p.stats[row * 3] = st.m;
+    p.stats[row * 3 + 1] = L;
+    p.stats[row * 3 + 2] = U;
+    p.entropy[row] = L + U;
+    const long long t = p.target[row];
+    float v = 0.f;
+    if (t != p.ignore) v = t < 0 || t >= p.C ? NAN : none ? -INFINITY : (given - st.m) - L;
+    p.logp[row] = v;
+}
+__device__ __forceinline__ float logp_of(float x, float m, float L) { return m == -INFINITY ? -INFINITY : (x - m) - L; }
+
+template <typename T, int THREADS, bool TOP>
+__global__ void __launch_bounds__(THREADS) token_logprobs_kernel(const LogpArgs p) {
+    constexpr int kGroup = THREADS >= 64 ? THREADS / 64 : 1, kGroups = THREADS / kGroup, kWarps = THREADS / 32;
+    __shared__ RowState states[kWarps];
+    __shared__ float group_top[TOP ? kGroups : 1];
+    __shared__ unsigned long long cand[TOP ? kCandidates : 1];
+    __shared__ int count;
+    __shared__ float bound;
+    const long row = blockIdx.x;
+    const int part = blockIdx.y, first = part * p.part_len, end = min(p.C, first + p.part_len);
+    const T *x = static_cast<const T *>(p.x) + row * p.pitch;
+    RowState st = empty_state();
+    walk<T, THREADS>(x, first, end, [&](int, float v) { add(st, v); },
+                     [&](int, const Wide<T> &w) {
+                         float v[Wide<T>::n], top = -INFINITY;
+#pragma unroll
+                         for (int i = 0; i < Wide<T>::n; ++i) { v[i] = w.get(i); top = fmaxf(top, v[i]); }
+                         if (top > st.m || st.m == -INFINITY || st.m == INFINITY) {
+#pragma unroll
+                             for (int i = 0; i < Wide<T>::n; ++i) add(st, v[i]);
+                         } else {
+                             // (-inf: exp gives 0, and 0 * inf must not reach u; a NaN reaches both sums through e)
+#pragma unroll
+                             for (int i = 0; i < Wide<T>::n; ++i) {
+                                 const float t = v[i] - st.m, e = __expf(t);
+                                 st.s += e;
+                                 st.u += e * fminf(-t, 1e30f);
+                             }
+                         }
+                     });
+    const float mine = st.m;
+    RowState all = st;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+        const RowState other{__shfl_xor_sync(0xffffffffu, all.m, d), __shfl_xor_sync(0xffffffffu, all.s, d), __shfl_xor_sync(0xffffffffu, all.u, d)};
+        // (both lanes join in the same order, so that they agree)
+        all = threadIdx.x & d ? join(other, all) : join(all, other);
+    }
+    if (TOP) {
+        float gt = mine;
+#pragma unroll
+        for (int d = 1; d < kGroup; d <<= 1) gt = fmaxf(gt, __shfl_xor_sync(0xffffffffu, gt, d));
+        if (threadIdx.x % kGroup == 0) group_top[threadIdx.x / kGroup] = gt;
+        if (threadIdx.x == 0) { count = 0; bound = -INFINITY; }
+    }
+    if (threadIdx.x % 32 == 0) states[threadIdx.x / 32] = all;
+    block_sync<THREADS>();
+    if (threadIdx.x == 0) {
+        for (int w = 1; w < kWarps; ++w) all = join(all, states[w]);
+        if (p.parts == 1) {
+            const long long t = p.target[row];
+            finish_row(p, row, all, t >= 0 && t < p.C ? to_f32<T>(x[t]) : 0.f);
+        } else {
+            p.part_state[row * p.parts + part] = all;
+        }
+        states[0] = all;
+    }
+    if (!TOP) return;
+    const int top = min(p.top, end - first);
+    if ((int)threadIdx.x < kGroups) {
+        // the top-th largest of the groups' largest values, where there are as many groups
+        const float v = group_top[threadIdx.x];
+        int above = 0, equal = 0;
+        for (int i = 0; i < kGroups; ++i) {
+            above += group_top[i] > v;
+            equal += group_top[i] == v;
+        }
+        if (above < top && above + equal >= top) bound = v;
+    }
+    block_sync<THREADS>();
+    const float least = bound;
+    const bool odd = isnan(states[0].s);  // NaN among the logits: the bound says nothing of them
+    if (mine >= least || odd) {
+        auto offer = [&](int j, float v) {
+            if (v >= least || v != v) {
+                const int at = atomicAdd(&count, 1);
+                if (at < kCandidates) cand[at] = key_of(v, j);
+            }
+        };
+        walk<T, THREADS>(x, first, end, offer, [&](int j, const Wide<T> &w) {
+#pragma unroll
+            for (int i = 0; i < Wide<T>::n; ++i) offer(j + i, w.get(i));
+        });
+    }
+    block_sync<THREADS>();
+    const float m = states[0].m, L = p.parts == 1 ? p.stats[row * 3 + 1] : 0.f;
+    auto put = [&](int rank, unsigned long long key) {
+        if (p.parts > 1) {
+            p.part_keys[(row * p.parts + part) * p.top + rank] = key;
+        } else {
+            p.top_logp[row * p.top + rank] = logp_of(value_of(key), m, L);
+            p.top_at[row * p.top + rank] = 0xffffffffu - (uint32_t)key;
+        }
+    };
+    if (p.parts > 1)  // a part shorter than `top`: keys below every other
+        for (int i = top + threadIdx.x; i < p.top; i += THREADS) p.part_keys[(row * p.parts + part) * p.top + i] = 0;
+    if (count <= kCandidates) {
+        rank_out<THREADS>(cand, count, top, put);
+        return;
+    }
+    // too many ties: the largest key below the last one, `top` times
+    unsigned long long last = ~0ull;
+    for (int r = 0; r < top; ++r) {
+        unsigned long long best = 0;
+        auto look = [&](int j, float v) {
+            const unsigned long long k = key_of(v, j);
+            if (k < last && k > best) best = k;
+        };
+        walk<T, THREADS>(x, first, end, look, [&](int j, const Wide<T> &w) {
+#pragma unroll
+            for (int i = 0; i < Wide<T>::n; ++i) look(j + i, w.get(i));
+        });
+#pragma unroll
+        for (int d = 16; d; d >>= 1) {
+            const unsigned long long o = __shfl_xor_sync(0xffffffffu, best, d);
+            best = o > best ? o : best;
+        }
+        block_sync<THREADS>();
+        if (threadIdx.x % 32 == 0) cand[threadIdx.x / 32] = best;
+        block_sync<THREADS>();
+        for (int w = 0; w < kWarps; ++w) best = cand[w] > best ? cand[w] : best;
+        if (threadIdx.x == 0) put(r, best);
+        last = best;
+    }
+}
+
+// joins the parts of a row
+template <typename T>
+__global__ void __launch_bounds__(256) token_logprobs_join_kernel(const LogpArgs p) {
+    __shared__ unsigned long long cand[kCandidates];
+    __shared__ int count;
+    __shared__ unsigned long long bound;
+    const long row = blockIdx.x;
+    const unsigned long long *keys = p.part_keys + row * p.parts * p.top;
+    RowState all = empty_state();
+    for (int i = 0; i < p.parts; ++i) all = join(all, p.part_state[row * p.parts + i]);
+    if (threadIdx.x == 0) {
+        const long long t = p.target[row];
+        finish_row(p, row, all, t >= 0 && t < p.C ? to_f32<T>(static_cast<const T *>(p.x)[row * p.pitch + t]) : 0.f);
+        count = 0;
+        bound = 0;
+    }
+    if (!p.top) return;
+    __syncthreads();
+    // a key that at least `top` keys reach: the top-th largest of the parts' largest, where there are as many parts
+    for (int i = threadIdx.x; i < p.parts; i += 256) {
+        const unsigned long long k = keys[(long)i * p.top];
+        int above = 0;
+        for (int j = 0; j < p.parts; ++j) above += keys[(long)j * p.top] > k;
+        if (above == p.top - 1) bound = k;
+    }
+    __syncthreads();
+    const unsigned long long least = bound > 1 ? bound : 1;
+    // (at most `top` parts reach it, with `top` keys each)
+    for (int i = threadIdx.x; i < p.parts * p.top; i += 256)
+        if (keys[i] >= least) {
+            const int at = atomicAdd(&count, 1);
+            if (at < kCandidates) cand[at] = keys[i];
+        }
+    __syncthreads();
+    const float L = p.stats[row * 3 + 1];
+    auto put = [&](int rank, unsigned long long key) {
+        p.top_logp[row * p.top + rank] = logp_of(value_of(key), all.m, L);
+        p.top_at[row * p.top + rank] = 0xffffffffu - (uint32_t)key;
+    };
+    if (count <= kCandidates) {
+        rank_out<256>(cand, count, p.top, put);
+        return;
+    }
+    for (int i = threadIdx.x; i < p.parts * p.top; i += 256) {
+        const unsigned long long k = keys[i];
+        if (k < least) continue;
+        int rank = 0;
+        for (int j = 0; j < p.parts * p.top; ++j) rank += keys[j] > k;
+        if (rank < p.top) put(rank, k);
+    }
+}
+
+struct GradArgs {
+    const void *x;
+    long pitch, N;
+    int C;
+    const long long *target;
+    long long ignore;
+    const float *stats, *g_logp, *g_entropy;  // either gradient may be null
+    void *gx;                                 // contiguous [N, C]
+    int span;                                 // classes of a block
+};
+
+template <typename T>
+__global__ void __launch_bounds__(256) token_logprobs_grad_kernel(const GradArgs p) {
+    const long row = blockIdx.x;
+    const int first = blockIdx.y * p.span, end = min(p.C, first + p.span);
+    const T *x = static_cast<const T *>(p.x) + row * p.pitch;
+    T *gx = static_cast<T *>(p.gx) + row * p.C;
+    const float m = p.stats[row * 3], L = p.stats[row * 3 + 1], U = p.stats[row * 3 + 2];
+    const long long t = p.target[row];
+    const bool none = m == -INFINITY && L == 0.f;
+    const float gl = t != p.ignore && p.g_logp ? p.g_logp[row] : 0.f, ge = p.g_entropy ? p.g_entropy[row] : 0.f;
+    const bool bad = t != p.ignore && (t < 0 || t >= p.C);
+    auto grad = [&](int j, float v) {
+        if (none) return 0.f;
+        const float a = v - m, lp = a - L, pr = __expf(lp);
+        float g = j == t ? -gl * expm1f(lp) : -gl * pr;
+        if (pr != 0.f) g -= ge * pr * (a + U);  // (-inf: no probability, no gradient)
+        return bad ? NAN : g;
+    };
+    constexpr int n = Wide<T>::n;
+    const uintptr_t a = reinterpret_cast<uintptr_t>(x + first), b = reinterpret_cast<uintptr_t>(gx + first);
+    if ((a ^ b) & 15) {  // rows that lie differently on 16-byte boundaries
+        for (int j = first + threadIdx.x; j < end; j += 256) gx[j] = from_f32<T>(grad(j, to_f32<T>(x[j])));
+        return;
+    }
+    const int head = min(end - first, (int)(((16 - (a & 15)) & 15) / sizeof(T))), vecs = (end - first - head) / n, tail = first + head + vecs * n;
+    if ((int)threadIdx.x < head) gx[first + threadIdx.x] = from_f32<T>(grad(first + threadIdx.x, to_f32<T>(x[first + threadIdx.x])));
+    if (tail + (int)threadIdx.x < end) gx[tail + threadIdx.x] = from_f32<T>(grad(tail + threadIdx.x, to_f32<T>(x[tail + threadIdx.x])));
+    const uint4 *v = reinterpret_cast<const uint4 *>(x + first + head);
+    uint4 *o = reinterpret_cast<uint4 *>(gx + first + head);
+    for (int i = threadIdx.x; i < vecs; i += 2 * 256) {
+        Wide<T> w[2];
+        w[0].raw = v[i];
+        const bool two = i + 256 < vecs;
+        if (two) w[1].raw = v[i + 256];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            if (k && !two) break;
+            union {
+                uint4 raw;
+                T v[n];
+            } r;
+#pragma unroll
+            for (int e = 0; e < n; ++e) r.v[e] = from_f32<T>(grad(first + head + (i + k * 256) * n + e, w[k].get(e)));
+            o[i + k * 256] = r.raw;
+        }
+    }
+}
+
+template <typename T, int THREADS>
+void launch_forward(const LogpArgs &p, cudaStream_t stream) {
+    if (p.top)
+        token_logprobs_kernel<T, THREADS, true><<<dim3((unsigned)p.N, p.parts), THREADS, 0, stream>>>(p);
+    else
+        token_logprobs_kernel<T, THREADS, false><<<dim3((unsigned)p.N, p.parts), THREADS, 0, stream>>>(p);
+}
+
+template <typename T>
+int forward(LogpArgs &p, cudaStream_t stream) {
+    // a warp for short rows, four for rows of a few thousand classes, sixteen for long ones
+    if (p.part_len <= 512 && p.parts == 1)
+        launch_forward<T, 32>(p, stream);
+    else if (p.part_len <= 4096)
+        launch_forward<T, 128>(p, stream);
+    else
+        launch_forward<T, 512>(p, stream);
+    int rc = launch_status();
+    if (rc == LUTGEMM_OK && p.parts > 1) {
+        token_logprobs_join_kernel<T><<<(unsigned)p.N, 256, 0, stream>>>(p);
+        rc = launch_status();
+    }
+    return rc;
+}
+
+template <typename T>
+int backward(const GradArgs &p, cudaStream_t stream) {
+    token_logprobs_grad_kernel<T><<<dim3((unsigned)p.N, (p.C + p.span - 1) / p.span), 256, 0, stream>>>(p);
+    return launch_status();
+}
+
+}  // namespace
+
+// parts of a row: none where the rows fill the GPU, else parts of at least 2048 classes up to two blocks to an SM
+int logprobs_parts(long N, int C, int sms) {
+    const long want = (2L * sms) / (N > 0 ? N : 1), most = (C + 2047) / 2048;
+    const long parts = want < most ? want : most;
+    return parts < 2 ? 1 : (int)(parts > 64 ? 64 : parts);
+}
+size_t logprobs_scratch_bytes(long N, int C, int top, int sms) {
+    const int parts = logprobs_parts(N, C, sms);
+    return parts == 1 ? 0 : (size_t)N * parts * (16 + sizeof(unsigned long long) * top);
+}
+
+int logprobs_forward(const void *x, int dtype, long pitch, long N, int C, const long long *target, long long ignore, int top, float *logp,
+                     float *entropy, float *stats, float *top_logp, long long *top_at, void *scratch, int sms, cudaStream_t stream) {
+    LogpArgs p{x, pitch, N, C, top, logprobs_parts(N, C, sms), C, target, ignore, logp, entropy, stats, top_logp, top_at, nullptr, nullptr};
+    if (p.parts > 1) {
+        p.part_len = ((C + p.parts - 1) / p.parts + 7) / 8 * 8;
+        p.parts = (C + p.part_len - 1) / p.part_len;
+        p.part_keys = static_cast<unsigned long long *>(scratch);
+        p.part_state = reinterpret_cast<RowState *>(p.part_keys + (size_t)N * p.parts * top);
+    }
+    if (dtype == LUTGEMM_F32) return forward<float>(p, stream);
+    if (dtype == LUTGEMM_BF16) return forward<__nv_bfloat16>(p, stream);
+    return forward<__half>(p, stream);
+}
+
+int logprobs_backward(const void *x, int dtype, long pitch, long N, int C, const long long *target, long long ignore, const float *stats,
+                      const float *g_logp, const float *g_entropy, void *gx, cudaStream_t stream) {
+    GradArgs p{x, pitch, N, C, target, ignore, stats, g_logp, g_entropy, gx, 0};
+    p.span = N * ((C + 8191) / 8192) < 512 ? 2048 : 8192;
+    while ((long)(C + p.span - 1) / p.span > 65535) p.span *= 2;
+    if (dtype == LUTGEMM_F32) return backward<float>(p, stream);
+    if (dtype == LUTGEMM_BF16) return backward<__nv_bfloat16>(p, stream);
+    return backward<__half>(p, stream);
+}
+
+}  // namespace lutgemm

@@ -365,6 +365,69 @@ size_t lutgemm_noalloc_scratch_capacity(void);
 int lutgemm_backward_gw_noalloc(const float *gc, const uint8_t *a, const uint8_t *w, float *gw,
                                 const int16_t *lut_gw, int bits, int M, int K, int N, void *stream);
 
+/* ---- between the approximate projections of a transformer block, and behind its head ---------------------------------
+ *
+ * Exact operators on fp32, bf16 and fp16 operands (`dtype`); sums and statistics are fp32 and every result is rounded once.
+ * Operands [B, T, heads, D] are given by the strides of B, T and heads in elements (s_b, s_t, s_h); D is contiguous and results
+ * are contiguous.  No counterpart in the reference, whose networks are convolutional.
+ */
+#define LUTGEMM_F32 0
+#define LUTGEMM_BF16 1
+#define LUTGEMM_F16 2
+
+/*
+ * Queries and keys of every head divided by sqrt(mean of squares + eps), times `qw` / `kw` (fp32 [D], NULL = 1), and turned by their
+ * positions: pairs (i, i + rot/2), or (2i, 2i + 1) with `interleaved`, of the first `rot` values by the angle whose cosine and
+ * sine stand at [position][i] of `cos` and `sin` (fp32 [table, rot/2]).  `pos` int32 [B, T]; NULL = 0 .. T-1.  A negative
+ * position leaves a token unturned, one from `table` on makes its turned values NaN.  D and rot even, D <= 256.
+ */
+int lutgemm_norm_rotate(const void *q, long q_sb, long q_st, long q_sh, const void *k, long k_sb, long k_st, long k_sh,
+                        const float *qw, const float *kw, const float *cos, const float *sin, int table, const int *pos, void *q_out,
+                        void *k_out, int dtype, int B, int T, int H, int G, int D, int rot, int interleaved, float eps, void *stream);
+/* gq, gk: gradients of the results by strides; dq, dk; dqw, dkw fp32 [D], either NULL where not wanted (with both NULL no scratch is
+ * needed). */
+size_t lutgemm_norm_rotate_backward_scratch_bytes(int D);
+int lutgemm_norm_rotate_backward(const void *gq, long gq_sb, long gq_st, long gq_sh, const void *gk, long gk_sb, long gk_st,
+                                 long gk_sh, const void *q, long q_sb, long q_st, long q_sh, const void *k, long k_sb, long k_st,
+                                 long k_sh, const float *qw, const float *kw, const float *cos, const float *sin, int table,
+                                 const int *pos, void *dq, void *dk, float *dqw, float *dkw, int dtype, int B, int T, int H, int G,
+                                 int D, int rot, int interleaved, float eps, void *scratch, size_t scratch_bytes, void *stream);
+
+/*
+ * out[b,i,h] = sum_j softmax_j(b_ij) v[b,j,g],  g = h / (H/G),  over the keys j that query i sees;
+ * b_ij = s or cap * tanh(s / cap) (cap > 0) with s = scale * q.k, minus slopes[h] * |place_i - j| (slopes fp32 [H] or NULL);
+ * place_i = i + Tk - Tq.  With `causal` a query sees keys up to its place and the first prefix[b] keys (int32 [B] or NULL).
+ * doc_q [B, Tq], doc_k [B, Tk] (int32, rows doc_*_sb apart, NULL = one document): queries see keys of their own id; ids below
+ * zero are padding, which is never read as a value.  A query that sees nothing gives zeros and has no gradient.
+ * `lse` fp32 [B, G, Tq * H/G]: statistics for the backward pass (log 2 of the sum of exponentials, rows ordered query by query).
+ * H a multiple of G, D a multiple of 8 up to 128.
+ * `delta`: fp32 scratch of the size of `lse`.
+ */
+int lutgemm_attention(const void *q, long q_sb, long q_st, long q_sh, const void *k, long k_sb, long k_st, long k_sh, const void *v,
+                      long v_sb, long v_st, long v_sh, void *out, float *lse, int dtype, int B, int Tq, int Tk, int H, int G, int D,
+                      float scale, float cap, const float *slopes, int causal, const int *prefix, const int *doc_q, long doc_q_sb,
+                      const int *doc_k, long doc_k_sb, void *stream);
+int lutgemm_attention_backward(const void *go, long go_sb, long go_st, long go_sh, const void *q, long q_sb, long q_st, long q_sh,
+                               const void *k, long k_sb, long k_st, long k_sh, const void *v, long v_sb, long v_st, long v_sh,
+                               const void *out, const float *lse, float *delta, void *dq, void *dk, void *dv, int dtype, int B, int Tq,
+                               int Tk, int H, int G, int D, float scale, float cap, const float *slopes, int causal,
+                               const int *prefix, const int *doc_q, long doc_q_sb, const int *doc_k, long doc_k_sb, void *stream);
+
+/*
+ * For each of N rows of C logits, `pitch` elements apart: logp[n] = log softmax(logits[n])[target[n]] (0 where the target is `ignore`,
+ * NaN where it is no class), entropy[n] of the softmax, and the `top` (0 to 32, at most C) most probable classes in order, the
+ * lower class first among equals (NaN logits before all others).  Logits of -inf have no probability; a row of nothing else has
+ * logp -inf and entropy 0; a NaN or +inf logit makes its row's results NaN.  `stats` fp32 [N, 3] is for the backward pass:
+ * grad[n,c] = g_logp (1[c = target] - p_c) - g_entropy p_c (log p_c + entropy), g_logp and g_entropy fp32 [N] or NULL.
+ */
+size_t lutgemm_token_logprobs_scratch_bytes(long N, int C, int top);
+int lutgemm_token_logprobs(const void *logits, int dtype, long pitch, long N, int C, const long long *target, long long ignore, int top,
+                           float *logp, float *entropy, float *stats, float *top_logp, long long *top_index, void *scratch,
+                           size_t scratch_bytes, void *stream);
+int lutgemm_token_logprobs_backward(const void *logits, int dtype, long pitch, long N, int C, const long long *target,
+                                    long long ignore, const float *stats, const float *g_logp, const float *g_entropy, void *grad,
+                                    void *stream);
+
 /*
  * Reads and clears the device-side error word of the pipelined kernels into *value (0 = no error).
  * Their warps hand slabs to each other through shared-memory barriers; every wait on such a barrier is
