@@ -120,7 +120,9 @@ def _load():
     lib.lutgemm_norm_rotate_backward.argtypes = [vp, cl, cl, cl] * 4 + [vp] * 4 + [ci] + [vp] * 5 + [ci] * 8 + [cf, vp, sz, vp]
     masks = [cf, cf, vp, ci, vp, vp, cl, vp, cl]
     lib.lutgemm_attention.restype = ci
-    lib.lutgemm_attention.argtypes = [vp, cl, cl, cl] * 3 + [vp, vp] + [ci] * 7 + masks + [vp]
+    lib.lutgemm_attention.argtypes = [vp, cl, cl, cl] * 3 + [vp] * 3 + [ci] * 7 + masks + [vp, sz, vp]
+    lib.lutgemm_attention_scratch_bytes.restype = sz
+    lib.lutgemm_attention_scratch_bytes.argtypes = [ci] * 8
     lib.lutgemm_attention_backward.restype = ci
     lib.lutgemm_attention_backward.argtypes = [vp, cl, cl, cl] * 4 + [vp] * 6 + [ci] * 7 + masks + [vp]
     lib.lutgemm_token_logprobs_scratch_bytes.restype = sz

@@ -1162,15 +1162,39 @@ static int attention_args(lutgemm::AttnProblem *p, int dtype, int B, int Tq, int
     return LUTGEMM_OK;
 }
 
+// 16-byte vectors of 16-bit operands: strides of axes that have more than one element
+static bool attention_vectors(const lutgemm::AttnTensor &t, int B, int T, int heads) {
+    return !(reinterpret_cast<uintptr_t>(t.p) & 15) && (B == 1 || t.sb % 8 == 0) && (T == 1 || t.st % 8 == 0) &&
+           (heads == 1 || t.sh % 8 == 0);
+}
+
+size_t lutgemm_attention_scratch_bytes(int dtype, int B, int Tq, int Tk, int H, int G, int D, int documents) {
+    lutgemm::AttnProblem p{};
+    const int *ids = documents ? reinterpret_cast<const int *>(16) : nullptr;
+    if (dtype == LUTGEMM_F32 || attention_args(&p, dtype, B, Tq, Tk, H, G, D, 1.f, 0.f, nullptr, 0, nullptr, ids, 0, ids, 0) != LUTGEMM_OK)
+        return 0;
+    const int sms = current_num_sms();
+    return sms <= 0 ? 0 : lutgemm::attention_tc_scratch_bytes(p, sms);
+}
+
 int lutgemm_attention(const void *q, long q_sb, long q_st, long q_sh, const void *k, long k_sb, long k_st, long k_sh, const void *v,
-                      long v_sb, long v_st, long v_sh, void *out, float *lse, int dtype, int B, int Tq, int Tk, int H, int G, int D,
-                      float scale, float cap, const float *slopes, int causal, const int *prefix, const int *doc_q, long doc_q_sb,
-                      const int *doc_k, long doc_k_sb, void *stream) {
+                      long v_sb, long v_st, long v_sh, void *out, void *out_rest, float *lse, int dtype, int B, int Tq, int Tk, int H,
+                      int G, int D, float scale, float cap, const float *slopes, int causal, const int *prefix, const int *doc_q,
+                      long doc_q_sb, const int *doc_k, long doc_k_sb, void *scratch, size_t scratch_bytes, void *stream) {
     if (!q || !k || !v || !out || !lse) return LUTGEMM_E_BADARG;
     lutgemm::AttnProblem p{{q, q_sb, q_st, q_sh}, {k, k_sb, k_st, k_sh}, {v, v_sb, v_st, v_sh}};
     const int rc = attention_args(&p, dtype, B, Tq, Tk, H, G, D, scale, cap, slopes, causal, prefix, doc_q, doc_q_sb, doc_k, doc_k_sb);
     if (rc != LUTGEMM_OK) return rc;
-    return lutgemm::attention_f32_forward(p, dtype, out, lse, static_cast<cudaStream_t>(stream));
+    if (dtype == LUTGEMM_F32) return lutgemm::attention_f32_forward(p, dtype, out, lse, static_cast<cudaStream_t>(stream));
+    if (!attention_vectors(p.q, B, Tq, H) || !attention_vectors(p.k, B, Tk, G) || !attention_vectors(p.v, B, Tk, G) ||
+        ((reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(out_rest)) & 15))
+        return LUTGEMM_E_BADARG;
+    const int sms = current_num_sms();
+    if (sms <= 0) return LUTGEMM_E_CUDA;
+    const size_t need = lutgemm::attention_tc_scratch_bytes(p, sms);
+    if (scratch_bytes < need) return LUTGEMM_E_SCRATCH;
+    if (need && (!scratch || (reinterpret_cast<uintptr_t>(scratch) & 15))) return LUTGEMM_E_BADARG;
+    return lutgemm::attention_tc_forward(p, dtype, out, out_rest, lse, scratch, sms, static_cast<cudaStream_t>(stream));
 }
 
 int lutgemm_attention_backward(const void *go, long go_sb, long go_st, long go_sh, const void *q, long q_sb, long q_st, long q_sh,

@@ -285,6 +285,10 @@ int backward_gw(const float *gc, const uint8_t *a, const uint8_t *w, float *gw, 
 struct AttnProblem;  // lutgemm_attention.cuh
 struct AttnTensor;
 
+// lutgemm_attention_tc.cu: 16-bit operands; rest (null or as out): what the rounding of out leaves
+size_t attention_tc_scratch_bytes(const AttnProblem &p, int num_sms);
+int attention_tc_forward(const AttnProblem &p, int dtype, void *out, void *rest, float *lse, void *scratch, int num_sms, cudaStream_t stream);
+
 // lutgemm_attention_f32.cu
 int attention_f32_forward(const AttnProblem &p, int dtype, void *out, float *lse, cudaStream_t stream);
 int attention_f32_backward(const AttnProblem &p, int dtype, const AttnTensor &go, const void *out, const float *lse, float *delta, void *gq,

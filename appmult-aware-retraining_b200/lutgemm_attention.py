@@ -44,6 +44,19 @@ def _rows(x: torch.Tensor) -> torch.Tensor:
     return x if x.stride(3) == 1 or x.shape[3] == 1 else x.contiguous()
 
 
+def _vectors(x: torch.Tensor) -> torch.Tensor:
+    """The same where 16-bit operands are read in vectors of eight values: a copy of one that lies differently."""
+    if x.dtype is torch.float32:
+        return _rows(x)
+    sb, st, sh, sd = x.stride()
+    if sd == 1 and not ((sb | st | sh) & 7 or x.data_ptr() & 15):
+        return x
+    B, T, heads, D = x.shape
+    if (sd != 1 and D > 1) or (sb & 7 and B > 1) or (st & 7 and T > 1) or (sh & 7 and heads > 1) or x.data_ptr() & 15:
+        return x.clone(memory_format=torch.contiguous_format)
+    return x
+
+
 def _at(x: torch.Tensor):
     return (x.data_ptr(), *x.stride()[:3])
 
@@ -172,10 +185,12 @@ class _Attention(torch.autograd.Function):
                  *((doc_q.data_ptr(), doc_q.stride(0), doc_k.data_ptr(), doc_k.stride(0)) if doc_q is not None else (None, 0, None, 0)))
         out = torch.empty((B, Tq, H, D), dtype=q.dtype, device=q.device)
         lse = torch.empty((B, G, Tq * H // G), dtype=torch.float32, device=q.device)
-        lib = approx_ops.library()
+        lib, dtype = approx_ops.library(), _DTYPES[q.dtype]
         with approx_ops._guard(q.device):
-            rc = lib.lutgemm_attention(*_at(q), *_at(k), *_at(v), out.data_ptr(), lse.data_ptr(), _DTYPES[q.dtype], B, Tq, Tk, H, G, D,
-                                       *masks, approx_ops._stream_ptr(q.device))
+            nbytes = lib.lutgemm_attention_scratch_bytes(dtype, B, Tq, Tk, H, G, D, doc_k is not None) if dtype else 0
+            scratch = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
+            rc = lib.lutgemm_attention(*_at(q), *_at(k), *_at(v), out.data_ptr(), None, lse.data_ptr(), dtype, B, Tq, Tk, H, G, D, *masks,
+                                       scratch.data_ptr() if nbytes else None, nbytes, approx_ops._stream_ptr(q.device))
         approx_ops._check(rc, "attention")
         ctx.save_for_backward(q, k, v, out, lse, slopes, prefix, doc_q, doc_k)
         ctx.cfg = (scale, cap, causal)
@@ -191,7 +206,7 @@ class _Attention(torch.autograd.Function):
         masks = (scale, cap, slopes.data_ptr() if slopes is not None else None, causal,
                  prefix.data_ptr() if prefix is not None else None,
                  *((doc_q.data_ptr(), doc_q.stride(0), doc_k.data_ptr(), doc_k.stride(0)) if doc_q is not None else (None, 0, None, 0)))
-        go = _rows(go)
+        go = _vectors(go)
         dq = torch.empty((B, Tq, H, D), dtype=q.dtype, device=q.device)
         dk = torch.empty((B, Tk, G, D), dtype=q.dtype, device=q.device)
         dv = torch.empty((B, Tk, G, D), dtype=q.dtype, device=q.device)
@@ -273,4 +288,4 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: float = 
             query_documents = query_documents if query_documents.stride(1) == 1 or Tq <= 1 else query_documents.contiguous()
     if B * Tq == 0 or Tk == 0:  # nothing to see: zeros, whose gradients are zeros
         return _Empty.apply(q, k, v)
-    return _Attention.apply(_rows(q), _rows(k), _rows(v), scale, cap, slopes, bool(causal), prefix, query_documents, documents)
+    return _Attention.apply(_vectors(q), _vectors(k), _vectors(v), scale, cap, slopes, bool(causal), prefix, query_documents, documents)

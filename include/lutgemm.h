@@ -400,13 +400,15 @@ int lutgemm_norm_rotate_backward(const void *gq, long gq_sb, long gq_st, long gq
  * doc_q [B, Tq], doc_k [B, Tk] (int32, rows doc_*_sb apart, NULL = one document): queries see keys of their own id; ids below
  * zero are padding, which is never read as a value.  A query that sees nothing gives zeros and has no gradient.
  * `lse` fp32 [B, G, Tq * H/G]: statistics for the backward pass (log 2 of the sum of exponentials, rows ordered query by query).
- * H a multiple of G, D a multiple of 8 up to 128.
+ * H a multiple of G, D a multiple of 8 up to 128.  16-bit operands are read in 16-byte vectors: their addresses and strides are
+ * multiples of that.  `out_rest` (16-bit types; NULL where no backward pass follows): what the rounding of `out` leaves, as `out`.
  * `delta`: fp32 scratch of the size of `lse`.
  */
+size_t lutgemm_attention_scratch_bytes(int dtype, int B, int Tq, int Tk, int H, int G, int D, int documents);
 int lutgemm_attention(const void *q, long q_sb, long q_st, long q_sh, const void *k, long k_sb, long k_st, long k_sh, const void *v,
-                      long v_sb, long v_st, long v_sh, void *out, float *lse, int dtype, int B, int Tq, int Tk, int H, int G, int D,
-                      float scale, float cap, const float *slopes, int causal, const int *prefix, const int *doc_q, long doc_q_sb,
-                      const int *doc_k, long doc_k_sb, void *stream);
+                      long v_sb, long v_st, long v_sh, void *out, void *out_rest, float *lse, int dtype, int B, int Tq, int Tk, int H,
+                      int G, int D, float scale, float cap, const float *slopes, int causal, const int *prefix, const int *doc_q,
+                      long doc_q_sb, const int *doc_k, long doc_k_sb, void *scratch, size_t scratch_bytes, void *stream);
 int lutgemm_attention_backward(const void *go, long go_sb, long go_st, long go_sh, const void *q, long q_sb, long q_st, long q_sh,
                                const void *k, long k_sb, long k_st, long k_sh, const void *v, long v_sb, long v_st, long v_sh,
                                const void *out, const float *lse, float *delta, void *dq, void *dk, void *dv, int dtype, int B, int Tq,
