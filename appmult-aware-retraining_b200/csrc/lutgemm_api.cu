@@ -1151,7 +1151,7 @@ static int attention_args(lutgemm::AttnProblem *p, int dtype, int B, int Tq, int
                           long doc_k_sb) {
     if (!dtype_supported(dtype) || B <= 0 || Tq <= 0 || Tk <= 0 || H <= 0 || G <= 0 || D <= 0 || H % G || D % 8) return LUTGEMM_E_BADARG;
     if (!(cap >= 0.f) || !isfinite(cap) || !isfinite(scale) || !doc_q != !doc_k) return LUTGEMM_E_BADARG;
-    if (D > 128 || B > 65535 || G > 65535 || (long)Tq * (H / G) > 0x7fffff00L || Tk > 0x7fffff00) return LUTGEMM_E_TOOLARGE;
+    if (D > 128 || B > 65535 || G > 65535 || H / G > 64 || (long)Tq * (H / G) > 0x7fffff00L || Tk > 0x7fffff00) return LUTGEMM_E_TOOLARGE;
     p->B = B; p->Tq = Tq; p->Tk = Tk; p->H = H; p->G = G; p->R = H / G; p->D = D;
     p->M = Tq * p->R;
     p->shift = Tk - Tq;
@@ -1164,8 +1164,8 @@ static int attention_args(lutgemm::AttnProblem *p, int dtype, int B, int Tq, int
 
 // 16-byte vectors of 16-bit operands: strides of axes that have more than one element
 static bool attention_vectors(const lutgemm::AttnTensor &t, int B, int T, int heads) {
-    return !(reinterpret_cast<uintptr_t>(t.p) & 15) && (B == 1 || t.sb % 8 == 0) && (T == 1 || t.st % 8 == 0) &&
-           (heads == 1 || t.sh % 8 == 0);
+    const auto fits = [](long stride, int count) { return count == 1 || (stride > 0 && stride % 8 == 0); };
+    return !(reinterpret_cast<uintptr_t>(t.p) & 15) && fits(t.sb, B) && fits(t.st, T) && fits(t.sh, heads);
 }
 
 size_t lutgemm_attention_scratch_bytes(int dtype, int B, int Tq, int Tk, int H, int G, int D, int documents) {

@@ -3,7 +3,9 @@
 
 #include "lutgemm.h"
 #include "lutgemm_attention.cuh"
+#include "lutgemm_f32x2.cuh"
 #include "lutgemm_tcgen.cuh"
+#include "lutgemm_tma.cuh"
 
 namespace lutgemm {
 
@@ -30,7 +32,7 @@ __device__ __forceinline__ float fast_rcp(float x) {
     return y;
 }
 template <typename T>
-__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+__device__ __forceinline__ uint32_t pack_pair(float lo, float hi) {
     uint32_t r;
     if (IsBf16<T>::value)
         asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
@@ -39,7 +41,7 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
     return r;
 }
 template <typename T>
-__device__ __forceinline__ float2 unpack2(uint32_t v) {
+__device__ __forceinline__ float2 unpack_pair(uint32_t v) {
     if (IsBf16<T>::value) return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
     return __half22float2(*reinterpret_cast<const __half2 *>(&v));
 }
@@ -56,43 +58,46 @@ __device__ __forceinline__ int key_limit(const AttnProblem &p, int place, int pr
     return min(lim, p.Tk - 1);
 }
 
-// `ROWS` rows of 64 * BLOCKS values (16-byte pieces c of a row at c ^ (row & 7)) by 128 threads; row r comes from row(r), null = zeros
-template <int ROWS, int BLOCKS, typename Row>
-__device__ __forceinline__ void copy_tile(uint32_t dst, int D, int thread, const void *any, Row row) {
-    const int c = thread & 7;
+// keys of the tile from j0 on that are not padding (beyond the last key: set), for one warp
+__device__ __forceinline__ unsigned long long key_mask(const AttnProblem &p, int b, int j0) {
+    if (!p.doc_k) return ~0ull;
+    const int lane = threadIdx.x & 31;
+    const int *ids = p.doc_k + b * p.doc_k_sb + j0;
+    const bool lo = j0 + lane >= p.Tk || ids[lane] >= 0, hi = j0 + 32 + lane >= p.Tk || ids[lane + 32] >= 0;
+    return __ballot_sync(0xffffffffu, lo) | (unsigned long long)__ballot_sync(0xffffffffu, hi) << 32;
+}
+// zeros into the rows of a tile (64 rows of 64 * BLOCKS values) that `mask` leaves out; one warp
+template <int BLOCKS>
+__device__ __forceinline__ void clear_rows(uint8_t *tile, unsigned long long mask) {
+    for (unsigned long long left = ~mask; left; left &= left - 1) {
+        const int r = __ffsll(left) - 1;
 #pragma unroll
-    for (int n = 0; n < ROWS / 16; ++n) {
-        const int r = (thread >> 3) + 16 * n;
-        const char *src = static_cast<const char *>(row(r));
-#pragma unroll
-        for (int k = 0; k < BLOCKS; ++k) {
-            const int at = k * 64 + c * 8;
-            const bool real = src != nullptr && at < D;
-            copy16(dst + k * ROWS * 128 + r * 128 + ((c ^ (r & 7)) << 4), real ? src + 2 * at : any, real);
-        }
+        for (int k = 0; k < BLOCKS; ++k) reinterpret_cast<float *>(tile + k * 64 * 128 + r * 128)[threadIdx.x & 31] = 0.f;
     }
 }
-// the tile of keys from j0 on
+// tile of 64 keys from j0 on, by one thread; `map` by key_map
 template <int BLOCKS>
-__device__ __forceinline__ void copy_keys(uint32_t dst, const AttnProblem &p, const AttnTensor &t, int b, int g, int j0, int thread) {
-    const char *base = static_cast<const char *>(t.p) + 2 * (b * t.sb + g * t.sh);
-    copy_tile<kKeyTile, BLOCKS>(dst, p.D, thread, t.p, [&](int r) -> const void * {
-        const int j = j0 + r;
-        if (j >= p.Tk || (p.doc_k && p.doc_k[b * p.doc_k_sb + j] < 0)) return nullptr;
-        return base + 2 * (j * t.st);
-    });
+__device__ __forceinline__ void load_keys(uint32_t dst, const CUtensorMap *map, int b, int g, int j0, uint32_t bar) {
+    tma_expect_bytes(bar, BLOCKS * 64 * 128);
+#pragma unroll
+    for (int k = 0; k < BLOCKS; ++k) tma_load_5d(dst + k * 64 * 128, map, 64 * k, 0, j0, g, b, bar);
 }
-// the ROWS packed rows from m0 on
-template <int ROWS, int BLOCKS>
-__device__ __forceinline__ void copy_rows(uint32_t dst, const AttnProblem &p, const AttnTensor &t, int b, int g, int m0, int thread) {
+// the 128 packed rows from m0 on of a query-side operand, by 128 threads; zeros beyond the end and for padding
+template <int BLOCKS>
+__device__ __forceinline__ void copy_row_tile(uint32_t dst, const AttnProblem &p, const AttnTensor &t, int b, int g, int m0, int thread) {
     const char *base = static_cast<const char *>(t.p) + 2 * (b * t.sb + (long)g * p.R * t.sh);
-    copy_tile<ROWS, BLOCKS>(dst, p.D, thread, t.p, [&](int r) -> const void * {
-        const int m = m0 + r;
-        if (m >= p.M) return nullptr;
-        const int i = p.R == 1 ? m : m / p.R;
-        if (p.doc_q && p.doc_q[b * p.doc_q_sb + i] < 0) return nullptr;
-        return base + 2 * (i * t.st + (m - i * p.R) * t.sh);
-    });
+    const int c = thread & 7;
+#pragma unroll 4
+    for (int n = 0; n < kRowTile / 16; ++n) {
+        const int r = (thread >> 3) + 16 * n, m = m0 + r, i = m / p.R;
+        const bool in = m < p.M && (!p.doc_q || p.doc_q[b * p.doc_q_sb + i] >= 0);
+        const char *src = base + 2 * (i * t.st + (m - i * p.R) * t.sh) + 16 * c;
+#pragma unroll
+        for (int k = 0; k < BLOCKS; ++k) {
+            const bool real = in && k * 64 + c * 8 < p.D;
+            copy16(dst + k * kRowTile * 128 + r * 128 + ((c ^ (r & 7)) << 4), real ? src + 128 * k : t.p, real);
+        }
+    }
 }
 
 // what a thread knows of its row
@@ -131,6 +136,16 @@ __device__ __forceinline__ Bend make_bend(const AttnProblem &p) {
 }
 
 int *device_error_word();
+
+// Tensor map of an operand whose heads come in groups of R: packed rows of a key head in boxes of 64 / R * R (a box of keys: R = 1)
+inline bool attention_map(CUtensorMap *map, bool bf16, const AttnTensor &t, int B, int T, int G, int R, int D) {
+    const auto bytes = [](long stride, long count) { return (unsigned long long)(count > 1 ? 2 * stride : 16); };
+    const unsigned long long dims[5] = {(unsigned long long)D, (unsigned long long)R, (unsigned long long)T, (unsigned long long)G,
+                                        (unsigned long long)B};
+    const unsigned long long strides[4] = {bytes(t.sh, R), bytes(t.st, T), bytes(R * t.sh, G), bytes(t.sb, B)};
+    const unsigned box[5] = {64, (unsigned)R, (unsigned)(64 / R), 1, 1};
+    return make_tensor_map_16bit_5d(map, bf16, t.p, dims, strides, box);
+}
 
 // lutgemm_attention_tc.cu: ranges of the documents of tiles of 64 keys and 64 packed rows ([B][tiles] each); nullptr where nothing
 // is gained by them

@@ -41,4 +41,25 @@ bool make_tensor_map_u8_2d(CUtensorMap *map, const void *base, unsigned long lon
               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+bool make_tensor_map_16bit_5d(CUtensorMap *map, bool bf16, const void *base, const unsigned long long (&dims)[5],
+                              const unsigned long long (&strides)[4], const unsigned (&box)[5]) {
+    EncodeTiledFn fn = encode_fn();
+    if (!fn || !base || (reinterpret_cast<uintptr_t>(base) & 15)) return false;
+    cuuint64_t d[5], st[4];
+    cuuint32_t bx[5], elem[5];
+    for (int i = 0; i < 5; ++i) {
+        if (dims[i] == 0 || box[i] == 0 || box[i] > 256) return false;
+        d[i] = dims[i];
+        bx[i] = box[i];
+        elem[i] = 1;
+    }
+    for (int i = 0; i < 4; ++i) {
+        if (strides[i] & 15) return false;
+        st[i] = strides[i];
+    }
+    return fn(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 5, const_cast<void *>(base), d, st, bx, elem,
+              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 }  // namespace lutgemm

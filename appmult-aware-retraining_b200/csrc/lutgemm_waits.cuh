@@ -49,6 +49,13 @@ __device__ __forceinline__ void mbar_wait(uint32_t bar, uint32_t parity, int wha
     atomicExch(error_word, what);
 }
 
+// After a wait that ran out: time for the block's copies and products in flight to end before its memory is given back.
+__device__ __forceinline__ void settle(volatile int *abort_word) {
+    if (!*abort_word) return;
+    const unsigned long long t0 = wait_clock_ns();
+    while (wait_clock_ns() - t0 < 10000000ull) __nanosleep(1000);  // ten milliseconds
+}
+
 // address of the device error word on the current device (nullptr if the lookup failed)
 int *device_error_word();
 

@@ -45,14 +45,15 @@ def _rows(x: torch.Tensor) -> torch.Tensor:
 
 
 def _vectors(x: torch.Tensor) -> torch.Tensor:
-    """The same where 16-bit operands are read in vectors of eight values: a copy of one that lies differently."""
+    """The same where 16-bit operands are read by bulk copies of eight values and more: a copy of one that lies differently or repeats
+    itself."""
     if x.dtype is torch.float32:
         return _rows(x)
     sb, st, sh, sd = x.stride()
-    if sd == 1 and not ((sb | st | sh) & 7 or x.data_ptr() & 15):
+    if sd == 1 and sb and st and sh and not ((sb | st | sh) & 7 or x.data_ptr() & 15):
         return x
     B, T, heads, D = x.shape
-    if (sd != 1 and D > 1) or (sb & 7 and B > 1) or (st & 7 and T > 1) or (sh & 7 and heads > 1) or x.data_ptr() & 15:
+    if (sd != 1 and D > 1) or x.data_ptr() & 15 or any(n > 1 and (s & 7 or not s) for n, s in ((B, sb), (T, st), (heads, sh))):
         return x.clone(memory_format=torch.contiguous_format)
     return x
 
@@ -236,7 +237,7 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: float = 
               causal: bool = False, prefix: torch.Tensor = None, documents: torch.Tensor = None,
               query_documents: torch.Tensor = None) -> torch.Tensor:
     """Softmax attention, [B, Tq, H, D]: q [B, Tq, H, D], k and v [B, Tk, G, D], G a divisor of H (query head h reads key head
-    h / (H/G)), D a multiple of 8 up to 128.
+    h / (H/G), at most 64 read one), D a multiple of 8 up to 128.
 
     scale      of the scores q.k, by default D^-0.5
     cap        above zero: scores s become cap * tanh(s / cap)
@@ -256,8 +257,8 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: float = 
     Tk, G = k.shape[1], k.shape[2]
     if tuple(k.shape) != (B, Tk, G, D) or k.shape != v.shape:
         raise RuntimeError(f"k and v must both be {(B, 'Tk', 'heads', D)}, got {tuple(k.shape)} and {tuple(v.shape)}")
-    if G == 0 or H == 0 or H % G:
-        raise RuntimeError(f"q's {H} heads must be a multiple of the {G} heads of k and v")
+    if G == 0 or H == 0 or H % G or H // G > 64:
+        raise RuntimeError(f"q's {H} heads must be a multiple of the {G} heads of k and v, at most 64 to one")
     if D == 0 or D % 8 or D > 128:
         raise RuntimeError(f"the size of a head must be a multiple of 8 up to 128, got {D}")
     cap = float(cap)

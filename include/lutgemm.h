@@ -400,8 +400,8 @@ int lutgemm_norm_rotate_backward(const void *gq, long gq_sb, long gq_st, long gq
  * doc_q [B, Tq], doc_k [B, Tk] (int32, rows doc_*_sb apart, NULL = one document): queries see keys of their own id; ids below
  * zero are padding, which is never read as a value.  A query that sees nothing gives zeros and has no gradient.
  * `lse` fp32 [B, G, Tq * H/G]: statistics for the backward pass (log 2 of the sum of exponentials, rows ordered query by query).
- * H a multiple of G, D a multiple of 8 up to 128.  16-bit operands are read in 16-byte vectors: their addresses and strides are
- * multiples of that.  `out_rest` (16-bit types; NULL where no backward pass follows): what the rounding of `out` leaves, as `out`.
+ * H a multiple of G and at most 64 G, D a multiple of 8 up to 128.  16-bit operands are read by bulk copies: their addresses and strides
+ * are multiples of 16 bytes, and no stride of an axis of several elements is 0.  `out_rest` (16-bit types; NULL where no backward pass follows): what the rounding of `out` leaves, as `out`.
  * `delta`: fp32 scratch of the size of `lse`.
  */
 size_t lutgemm_attention_scratch_bytes(int dtype, int B, int Tq, int Tk, int H, int G, int D, int documents);
