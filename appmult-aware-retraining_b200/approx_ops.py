@@ -124,7 +124,9 @@ def _load():
     lib.lutgemm_attention_scratch_bytes.restype = sz
     lib.lutgemm_attention_scratch_bytes.argtypes = [ci] * 8
     lib.lutgemm_attention_backward.restype = ci
-    lib.lutgemm_attention_backward.argtypes = [vp, cl, cl, cl] * 4 + [vp] * 6 + [ci] * 7 + masks + [vp]
+    lib.lutgemm_attention_backward.argtypes = [vp, cl, cl, cl] * 4 + [vp] * 6 + [ci] * 7 + masks + [vp, sz, vp]
+    lib.lutgemm_attention_backward_scratch_bytes.restype = sz
+    lib.lutgemm_attention_backward_scratch_bytes.argtypes = [ci] * 8
     lib.lutgemm_token_logprobs_scratch_bytes.restype = sz
     lib.lutgemm_token_logprobs_scratch_bytes.argtypes = [cl, ci, ci]
     lib.lutgemm_token_logprobs.restype = ci

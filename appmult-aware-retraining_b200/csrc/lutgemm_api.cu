@@ -1185,7 +1185,7 @@ int lutgemm_attention(const void *q, long q_sb, long q_st, long q_sh, const void
     lutgemm::AttnProblem p{{q, q_sb, q_st, q_sh}, {k, k_sb, k_st, k_sh}, {v, v_sb, v_st, v_sh}};
     const int rc = attention_args(&p, dtype, B, Tq, Tk, H, G, D, scale, cap, slopes, causal, prefix, doc_q, doc_q_sb, doc_k, doc_k_sb);
     if (rc != LUTGEMM_OK) return rc;
-    if (dtype == LUTGEMM_F32) return lutgemm::attention_f32_forward(p, dtype, out, lse, static_cast<cudaStream_t>(stream));
+    if (dtype == LUTGEMM_F32) return lutgemm::attention_f32_forward(p, static_cast<float *>(out), lse, static_cast<cudaStream_t>(stream));
     if (!attention_vectors(p.q, B, Tq, H) || !attention_vectors(p.k, B, Tk, G) || !attention_vectors(p.v, B, Tk, G) ||
         ((reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(out_rest)) & 15))
         return LUTGEMM_E_BADARG;
@@ -1197,17 +1197,36 @@ int lutgemm_attention(const void *q, long q_sb, long q_st, long q_sh, const void
     return lutgemm::attention_tc_forward(p, dtype, out, out_rest, lse, scratch, sms, static_cast<cudaStream_t>(stream));
 }
 
+size_t lutgemm_attention_backward_scratch_bytes(int dtype, int B, int Tq, int Tk, int H, int G, int D, int documents) {
+    lutgemm::AttnProblem p{};
+    const int *ids = documents ? reinterpret_cast<const int *>(16) : nullptr;
+    if (attention_args(&p, dtype, B, Tq, Tk, H, G, D, 1.f, 0.f, nullptr, 0, nullptr, ids, 0, ids, 0) != LUTGEMM_OK) return 0;
+    return dtype == LUTGEMM_F32 ? sizeof(float) * (size_t)B * G * p.M : lutgemm::attention_tc_backward_scratch_bytes(p);
+}
+
 int lutgemm_attention_backward(const void *go, long go_sb, long go_st, long go_sh, const void *q, long q_sb, long q_st, long q_sh,
                                const void *k, long k_sb, long k_st, long k_sh, const void *v, long v_sb, long v_st, long v_sh,
-                               const void *out, const float *lse, float *delta, void *dq, void *dk, void *dv, int dtype, int B, int Tq,
-                               int Tk, int H, int G, int D, float scale, float cap, const float *slopes, int causal, const int *prefix,
-                               const int *doc_q, long doc_q_sb, const int *doc_k, long doc_k_sb, void *stream) {
-    if (!go || !q || !k || !v || !out || !lse || !delta || !dq || !dk || !dv) return LUTGEMM_E_BADARG;
+                               const void *out, const void *out_rest, const float *lse, void *dq, void *dk, void *dv, int dtype, int B,
+                               int Tq, int Tk, int H, int G, int D, float scale, float cap, const float *slopes, int causal,
+                               const int *prefix, const int *doc_q, long doc_q_sb, const int *doc_k, long doc_k_sb, void *scratch,
+                               size_t scratch_bytes, void *stream) {
+    if (!go || !q || !k || !v || !out || !lse || !dq || !dk || !dv) return LUTGEMM_E_BADARG;
     lutgemm::AttnProblem p{{q, q_sb, q_st, q_sh}, {k, k_sb, k_st, k_sh}, {v, v_sb, v_st, v_sh}};
     const int rc = attention_args(&p, dtype, B, Tq, Tk, H, G, D, scale, cap, slopes, causal, prefix, doc_q, doc_q_sb, doc_k, doc_k_sb);
     if (rc != LUTGEMM_OK) return rc;
+    if (scratch_bytes < lutgemm_attention_backward_scratch_bytes(dtype, B, Tq, Tk, H, G, D, doc_k != nullptr)) return LUTGEMM_E_SCRATCH;
+    if (!scratch || (reinterpret_cast<uintptr_t>(scratch) & 15)) return LUTGEMM_E_BADARG;
     const lutgemm::AttnTensor g{go, go_sb, go_st, go_sh};
-    return lutgemm::attention_f32_backward(p, dtype, g, out, lse, delta, dq, dk, dv, static_cast<cudaStream_t>(stream));
+    const cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (dtype == LUTGEMM_F32)
+        return lutgemm::attention_f32_backward(p, g, static_cast<const float *>(out), lse, static_cast<float *>(scratch),
+                                               static_cast<float *>(dq), static_cast<float *>(dk), static_cast<float *>(dv), s);
+    if (!attention_vectors(p.q, B, Tq, H) || !attention_vectors(p.k, B, Tk, G) || !attention_vectors(p.v, B, Tk, G) ||
+        !attention_vectors(g, B, Tq, H) || !out_rest ||
+        ((reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(out_rest) | reinterpret_cast<uintptr_t>(dq) |
+          reinterpret_cast<uintptr_t>(dk) | reinterpret_cast<uintptr_t>(dv)) & 15))
+        return LUTGEMM_E_BADARG;
+    return lutgemm::attention_tc_backward(p, dtype, g, out, out_rest, lse, dq, dk, dv, scratch, s);
 }
 
 size_t lutgemm_token_logprobs_scratch_bytes(long N, int C, int top) {

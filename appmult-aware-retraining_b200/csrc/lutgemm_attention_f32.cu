@@ -1,4 +1,4 @@
-// Attention on the fp32 pipes, for every type.
+// Attention of fp32 operands on the fp32 pipes.
 #include "lutgemm.h"
 #include "lutgemm_attention.cuh"
 #include "lutgemm_kernels.h"
@@ -10,31 +10,30 @@ namespace {
 constexpr int kT = 64;        // rows and keys of a tile
 constexpr int kThreads = 256; // 16 x 16, each with 4 x 4 scores
 
-template <typename T>
-__device__ __forceinline__ const T *row_ptr(const AttnTensor &t, int b, int i, int h) {
-    return reinterpret_cast<const T *>(t.p) + b * t.sb + i * t.st + h * t.sh;
+__device__ __forceinline__ const float *row_ptr(const AttnTensor &t, int b, int i, int h) {
+    return reinterpret_cast<const float *>(t.p) + b * t.sb + i * t.st + h * t.sh;
 }
 
 // the 64 rows from m0 on (packed rows of key head g) of a query-side operand, as fp32, rows DP + 4 apart; zeros beyond the end
 // and for padding
-template <typename T, int DP>
+template <int DP>
 __device__ __forceinline__ void load_rows(float *dst, const AttnProblem &p, const AttnTensor &t, int b, int g, int m0) {
     for (int idx = threadIdx.x; idx < kT * DP; idx += kThreads) {
         const int r = idx / DP, d = idx - r * DP, m = m0 + r;
         float x = 0.f;
         if (m < p.M && d < p.D) {
             const int i = m / p.R, h = g * p.R + m - i * p.R;
-            if (!p.doc_q || p.doc_q[b * p.doc_q_sb + i] >= 0) x = to_f32<T>(row_ptr<T>(t, b, i, h)[d]);
+            if (!p.doc_q || p.doc_q[b * p.doc_q_sb + i] >= 0) x = row_ptr(t, b, i, h)[d];
         }
         dst[r * (DP + 4) + d] = x;
     }
 }
-template <typename T, int DP>
+template <int DP>
 __device__ __forceinline__ void load_keys(float *dst, const AttnProblem &p, const AttnTensor &t, int b, int g, int j0) {
     for (int idx = threadIdx.x; idx < kT * DP; idx += kThreads) {
         const int r = idx / DP, d = idx - r * DP, j = j0 + r;
         float x = 0.f;
-        if (j < p.Tk && d < p.D && (!p.doc_k || p.doc_k[b * p.doc_k_sb + j] >= 0)) x = to_f32<T>(row_ptr<T>(t, b, j, g)[d]);
+        if (j < p.Tk && d < p.D && (!p.doc_k || p.doc_k[b * p.doc_k_sb + j] >= 0)) x = row_ptr(t, b, j, g)[d];
         dst[r * (DP + 4) + d] = x;
     }
 }
@@ -138,12 +137,12 @@ __device__ __forceinline__ float logit(const AttnProblem &p, float dot, float sl
     return s;
 }
 
-template <typename T, int DP>
-__global__ void __launch_bounds__(kThreads) attention_f32_kernel(const AttnProblem p, T *out, float *lse) {
+template <int DP>
+__global__ void __launch_bounds__(kThreads) attention_f32_kernel(const AttnProblem p, float *out, float *lse) {
     extern __shared__ float4 smem4[];
     float *Q = reinterpret_cast<float *>(smem4), *K = Q + kT * (DP + 4), *V = K + kT * (DP + 4), *P = V + kT * (DP + 4);
     const int b = blockIdx.z, g = blockIdx.y, m0 = (gridDim.x - 1 - blockIdx.x) * kT, ty = threadIdx.x >> 4, tx = threadIdx.x & 15;
-    load_rows<T, DP>(Q, p, p.q, b, g, m0);
+    load_rows<DP>(Q, p, p.q, b, g, m0);
     RowInfo row[4];
     float most[4], sum[4];
     float4 acc[4][DP / 64];
@@ -158,8 +157,8 @@ __global__ void __launch_bounds__(kThreads) attention_f32_kernel(const AttnProbl
     const int end = key_end(p, b, m0), pre = p.prefix ? p.prefix[b] : 0;
     for (int j0 = 0; j0 < end; j0 += kT) {
         __syncthreads();
-        load_keys<T, DP>(K, p, p.k, b, g, j0);
-        load_keys<T, DP>(V, p, p.v, b, g, j0);
+        load_keys<DP>(K, p, p.k, b, g, j0);
+        load_keys<DP>(V, p, p.v, b, g, j0);
         __syncthreads();
         float s[4][4];
         products<DP>(s, Q, K, ty, tx);
@@ -202,14 +201,14 @@ __global__ void __launch_bounds__(kThreads) attention_f32_kernel(const AttnProbl
         if (m >= p.M) continue;
         const float inv = sum[i] > 0.f ? 1.f / sum[i] : sum[i] == 0.f ? 0.f : NAN;
         const int q = m / p.R, h = g * p.R + m - q * p.R;
-        T *o = out + (((size_t)b * p.Tq + q) * p.H + h) * p.D;
+        float *o = out + (((size_t)b * p.Tq + q) * p.H + h) * p.D;
 #pragma unroll
         for (int c = 0; c < DP / 64; ++c) {
             const float v[4] = {acc[i][c].x, acc[i][c].y, acc[i][c].z, acc[i][c].w};
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const int d = tx * 4 + 64 * c + e;
-                if (d < p.D) o[d] = from_f32<T>(v[e] * inv);
+                if (d < p.D) o[d] = v[e] * inv;
             }
         }
         if (tx == 0) lse[((size_t)b * p.G + g) * p.M + m] = sum[i] == 0.f ? INFINITY : most[i] + log2f(sum[i]);
@@ -243,15 +242,15 @@ __device__ __forceinline__ void tile_gradients(const AttnProblem &p, const float
     }
 }
 
-template <typename T, int DP>
-__global__ void __launch_bounds__(kThreads) attention_f32_grad_q_kernel(const AttnProblem p, const AttnTensor go, const T *out,
-                                                                        const float *lse, float *delta, T *gq) {
+template <int DP>
+__global__ void __launch_bounds__(kThreads) attention_f32_grad_q_kernel(const AttnProblem p, const AttnTensor go, const float *out,
+                                                                        const float *lse, float *delta, float *gq) {
     extern __shared__ float4 smem4[];
     float *Q = reinterpret_cast<float *>(smem4), *K = Q + kT * (DP + 4), *V = K + kT * (DP + 4), *GO = V + kT * (DP + 4),
           *DS = GO + kT * (DP + 4);
     const int b = blockIdx.z, g = blockIdx.y, m0 = (gridDim.x - 1 - blockIdx.x) * kT, ty = threadIdx.x >> 4, tx = threadIdx.x & 15;
-    load_rows<T, DP>(Q, p, p.q, b, g, m0);
-    load_rows<T, DP>(GO, p, go, b, g, m0);
+    load_rows<DP>(Q, p, p.q, b, g, m0);
+    load_rows<DP>(GO, p, go, b, g, m0);
     __syncthreads();
     // delta = sum_d grad_o * o, four threads to a row
     {
@@ -259,8 +258,8 @@ __global__ void __launch_bounds__(kThreads) attention_f32_grad_q_kernel(const At
         float s = 0.f;
         if (m < p.M) {
             const int i = m / p.R, h = g * p.R + m - i * p.R;
-            const T *o = out + (((size_t)b * p.Tq + i) * p.H + h) * p.D;
-            for (int d = threadIdx.x & 3; d < p.D; d += 4) s += to_f32<T>(o[d]) * GO[r * (DP + 4) + d];
+            const float *o = out + (((size_t)b * p.Tq + i) * p.H + h) * p.D;
+            for (int d = threadIdx.x & 3; d < p.D; d += 4) s += o[d] * GO[r * (DP + 4) + d];
         }
         s += __shfl_xor_sync(0xffffffffu, s, 1);
         s += __shfl_xor_sync(0xffffffffu, s, 2);
@@ -274,8 +273,8 @@ __global__ void __launch_bounds__(kThreads) attention_f32_grad_q_kernel(const At
     const int end = key_end(p, b, m0), pre = p.prefix ? p.prefix[b] : 0;
     for (int j0 = 0; j0 < end; j0 += kT) {
         __syncthreads();
-        load_keys<T, DP>(K, p, p.k, b, g, j0);
-        load_keys<T, DP>(V, p, p.v, b, g, j0);
+        load_keys<DP>(K, p, p.k, b, g, j0);
+        load_keys<DP>(V, p, p.v, b, g, j0);
         __syncthreads();
         tile_gradients<DP>(p, Q, K, V, GO, nullptr, DS, lse, delta, b, g, m0, j0, pre, ty, tx);
         __syncthreads();
@@ -286,28 +285,28 @@ __global__ void __launch_bounds__(kThreads) attention_f32_grad_q_kernel(const At
         const int m = m0 + ty * 4 + i;
         if (m >= p.M) continue;
         const int q = m / p.R, h = g * p.R + m - q * p.R;
-        T *o = gq + (((size_t)b * p.Tq + q) * p.H + h) * p.D;
+        float *o = gq + (((size_t)b * p.Tq + q) * p.H + h) * p.D;
 #pragma unroll
         for (int c = 0; c < DP / 64; ++c) {
             const float v[4] = {acc[i][c].x, acc[i][c].y, acc[i][c].z, acc[i][c].w};
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const int d = tx * 4 + 64 * c + e;
-                if (d < p.D) o[d] = from_f32<T>(v[e]);
+                if (d < p.D) o[d] = v[e];
             }
         }
     }
 }
 
-template <typename T, int DP>
+template <int DP>
 __global__ void __launch_bounds__(kThreads) attention_f32_grad_kv_kernel(const AttnProblem p, const AttnTensor go, const float *lse,
-                                                                         const float *delta, T *gk, T *gv) {
+                                                                         const float *delta, float *gk, float *gv) {
     extern __shared__ float4 smem4[];
     float *Q = reinterpret_cast<float *>(smem4), *K = Q + kT * (DP + 4), *V = K + kT * (DP + 4), *GO = V + kT * (DP + 4),
           *DS = GO + kT * (DP + 4), *P = DS + kT * (kT + 4);
     const int b = blockIdx.z, g = blockIdx.y, j0 = blockIdx.x * kT, ty = threadIdx.x >> 4, tx = threadIdx.x & 15;
-    load_keys<T, DP>(K, p, p.k, b, g, j0);
-    load_keys<T, DP>(V, p, p.v, b, g, j0);
+    load_keys<DP>(K, p, p.k, b, g, j0);
+    load_keys<DP>(V, p, p.v, b, g, j0);
     float4 ak[4][DP / 64], av[4][DP / 64];
 #pragma unroll
     for (int i = 0; i < 4; ++i)
@@ -319,8 +318,8 @@ __global__ void __launch_bounds__(kThreads) attention_f32_grad_kv_kernel(const A
     if (p.causal && j0 >= pre) first = max(0, j0 - p.shift) * p.R / kT * kT;
     for (int m0 = first; m0 < p.M; m0 += kT) {
         __syncthreads();
-        load_rows<T, DP>(Q, p, p.q, b, g, m0);
-        load_rows<T, DP>(GO, p, go, b, g, m0);
+        load_rows<DP>(Q, p, p.q, b, g, m0);
+        load_rows<DP>(GO, p, go, b, g, m0);
         __syncthreads();
         tile_gradients<DP>(p, Q, K, V, GO, P, DS, lse, delta, b, g, m0, j0, pre, ty, tx);
         __syncthreads();
@@ -338,35 +337,35 @@ __global__ void __launch_bounds__(kThreads) attention_f32_grad_kv_kernel(const A
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const int d = tx * 4 + 64 * c + e;
-                if (d < p.D) { gk[at + d] = from_f32<T>(x[e]); gv[at + d] = from_f32<T>(y[e]); }
+                if (d < p.D) { gk[at + d] = x[e]; gv[at + d] = y[e]; }
             }
         }
     }
 }
 
-template <typename T, int DP>
-int forward(const AttnProblem &p, void *out, float *lse, cudaStream_t stream) {
+template <int DP>
+int forward(const AttnProblem &p, float *out, float *lse, cudaStream_t stream) {
     const size_t smem = sizeof(float) * (3 * kT * (DP + 4) + kT * (kT + 4));
-    if (!cuda_ok(cudaFuncSetAttribute(attention_f32_kernel<T, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem))) return LUTGEMM_E_CUDA;
-    attention_f32_kernel<T, DP><<<dim3((p.M + kT - 1) / kT, p.G, p.B), kThreads, smem, stream>>>(p, static_cast<T *>(out), lse);
+    if (!cuda_ok(cudaFuncSetAttribute(attention_f32_kernel<DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem))) return LUTGEMM_E_CUDA;
+    attention_f32_kernel<DP><<<dim3((p.M + kT - 1) / kT, p.G, p.B), kThreads, smem, stream>>>(p, out, lse);
     return launch_status();
 }
-template <typename T, int DP>
-int backward(const AttnProblem &p, const AttnTensor &go, const void *out, const float *lse, float *delta, void *gq, void *gk, void *gv,
+template <int DP>
+int backward(const AttnProblem &p, const AttnTensor &go, const float *out, const float *lse, float *delta, float *gq, float *gk, float *gv,
              cudaStream_t stream) {
     const size_t smem_q = sizeof(float) * (4 * kT * (DP + 4) + kT * (kT + 4)), smem_kv = sizeof(float) * (4 * kT * (DP + 4) + 2 * kT * (kT + 4));
-    if (!cuda_ok(cudaFuncSetAttribute(attention_f32_grad_q_kernel<T, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem_q)) ||
-        !cuda_ok(cudaFuncSetAttribute(attention_f32_grad_kv_kernel<T, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem_kv)))
+    if (!cuda_ok(cudaFuncSetAttribute(attention_f32_grad_q_kernel<DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem_q)) ||
+        !cuda_ok(cudaFuncSetAttribute(attention_f32_grad_kv_kernel<DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem_kv)))
         return LUTGEMM_E_CUDA;
     if (p.M > 0) {
-        attention_f32_grad_q_kernel<T, DP><<<dim3((p.M + kT - 1) / kT, p.G, p.B), kThreads, smem_q, stream>>>(
-            p, go, static_cast<const T *>(out), lse, delta, static_cast<T *>(gq));
+        attention_f32_grad_q_kernel<DP><<<dim3((p.M + kT - 1) / kT, p.G, p.B), kThreads, smem_q, stream>>>(
+            p, go, out, lse, delta, gq);
         const int rc = launch_status();
         if (rc != LUTGEMM_OK) return rc;
     }
     if (p.Tk > 0) {
-        attention_f32_grad_kv_kernel<T, DP><<<dim3((p.Tk + kT - 1) / kT, p.G, p.B), kThreads, smem_kv, stream>>>(
-            p, go, lse, delta, static_cast<T *>(gk), static_cast<T *>(gv));
+        attention_f32_grad_kv_kernel<DP><<<dim3((p.Tk + kT - 1) / kT, p.G, p.B), kThreads, smem_kv, stream>>>(
+            p, go, lse, delta, gk, gv);
         return launch_status();
     }
     return LUTGEMM_OK;
@@ -374,22 +373,13 @@ int backward(const AttnProblem &p, const AttnTensor &go, const void *out, const 
 
 }  // namespace
 
-int attention_f32_forward(const AttnProblem &p, int dtype, void *out, float *lse, cudaStream_t stream) {
-    const bool wide = p.D > 64;
-    if (dtype == LUTGEMM_F32) return wide ? forward<float, 128>(p, out, lse, stream) : forward<float, 64>(p, out, lse, stream);
-    if (dtype == LUTGEMM_BF16) return wide ? forward<__nv_bfloat16, 128>(p, out, lse, stream) : forward<__nv_bfloat16, 64>(p, out, lse, stream);
-    return wide ? forward<__half, 128>(p, out, lse, stream) : forward<__half, 64>(p, out, lse, stream);
+int attention_f32_forward(const AttnProblem &p, float *out, float *lse, cudaStream_t stream) {
+    return p.D > 64 ? forward<128>(p, out, lse, stream) : forward<64>(p, out, lse, stream);
 }
 
-int attention_f32_backward(const AttnProblem &p, int dtype, const AttnTensor &go, const void *out, const float *lse, float *delta, void *gq,
-                           void *gk, void *gv, cudaStream_t stream) {
-    const bool wide = p.D > 64;
-    if (dtype == LUTGEMM_F32)
-        return wide ? backward<float, 128>(p, go, out, lse, delta, gq, gk, gv, stream) : backward<float, 64>(p, go, out, lse, delta, gq, gk, gv, stream);
-    if (dtype == LUTGEMM_BF16)
-        return wide ? backward<__nv_bfloat16, 128>(p, go, out, lse, delta, gq, gk, gv, stream)
-                    : backward<__nv_bfloat16, 64>(p, go, out, lse, delta, gq, gk, gv, stream);
-    return wide ? backward<__half, 128>(p, go, out, lse, delta, gq, gk, gv, stream) : backward<__half, 64>(p, go, out, lse, delta, gq, gk, gv, stream);
+int attention_f32_backward(const AttnProblem &p, const AttnTensor &go, const float *out, const float *lse, float *delta, float *gq, float *gk,
+                           float *gv, cudaStream_t stream) {
+    return p.D > 64 ? backward<128>(p, go, out, lse, delta, gq, gk, gv, stream) : backward<64>(p, go, out, lse, delta, gq, gk, gv, stream);
 }
 
 }  // namespace lutgemm

@@ -8,42 +8,6 @@ namespace {
 
 constexpr int kThreads = 160;  // four warps with a row to a thread, one that brings tiles and issues products
 
-// Tiles of 64 keys that a tile of rows has to visit, in ascending order: all up to the last visible key, or, with ranges of
-// documents, those whose documents overlap the rows'.  For one warp, every lane alike.
-struct TileWalk {
-    const DocRange *ranges;  // of this row of the batch, or null
-    int qleast, qmost, qpadding, least_limit, at, end;  // end: one past the last tile
-    int base = 0;
-    uint32_t visit = 0, whole = 0;  // with ranges: tiles of [base - 32, base) that are left, and those of them without a mask
-
-    __device__ __forceinline__ bool whole_by_limit(int t) const { return t * kKeyTile + kKeyTile - 1 <= least_limit; }
-    // the next tile times two, plus one where no element of it is masked; -1: none
-    __device__ __forceinline__ int next(bool docs) {
-        if (!ranges) {
-            if (at >= end) return -1;
-            const int t = at++;
-            return 2 * t + (!docs && whole_by_limit(t));
-        }
-        while (!visit) {
-            if (base < at) base = at;  // (the first time)
-            if (base >= end) return -1;
-            const int t = base + (threadIdx.x & 31);
-            bool see = false, all = false;
-            if (t < end) {
-                const DocRange r = ranges[t];
-                see = r.least <= qmost && r.most >= qleast;
-                all = see && qleast == qmost && r.least == r.most && !r.padding && !qpadding && whole_by_limit(t);
-            }
-            visit = __ballot_sync(0xffffffffu, see);
-            whole = __ballot_sync(0xffffffffu, all);
-            base += 32;
-        }
-        const int bit = __ffs(visit) - 1;
-        visit &= visit - 1;
-        return 2 * (base - 32 + bit) + (whole >> bit & 1);
-    }
-};
-
 // A block has 128 packed rows, one to a thread of its first four warps and a lane of tensor memory, and goes over the keys in tiles
 // of 64:
 //     S = Q K^T (tcgen05, into tensor memory) -> the thread's 64 scores to registers, mask, maximum, P = exp2 -> P back to tensor
@@ -97,24 +61,19 @@ __global__ void __launch_bounds__(kThreads, Layout<T, DP>::kPerSm)
     if (warp == 4) {
         tmem_alloc(smem_u32(slot), L::kColumns);
         TileWalk walk;
-        walk.ranges = key_ranges ? key_ranges + (long)b * ((p.Tk + kKeyTile - 1) / kKeyTile) : nullptr;
-        walk.least_limit = key_limit(p, m0 / p.R + p.shift, pre);
         const int last = min(m0 + kRowTile, p.M) - 1;
         const int all = max(0, key_limit(p, last / p.R + p.shift, pre) + kKeyTile) / kKeyTile;  // up to the last visible key
-        walk.at = 0;
         walk.end = all;
+        walk.whole_last = max(0, key_limit(p, m0 / p.R + p.shift, pre) + 1) / kKeyTile - 1;
         if (splits > 1) {
             const int per = (all + splits - 1) / splits;
             walk.at = min(split * per, all);
             walk.end = min(walk.at + per, all);
         }
-        if (walk.ranges) {
-            const int tiles64 = (p.M + kKeyTile - 1) / kKeyTile;
-            const DocRange *r = row_ranges + (long)b * tiles64 + m0 / kKeyTile;
-            const DocRange x = r[0], y = m0 / kKeyTile + 1 < tiles64 ? r[1] : DocRange{kNoLeast, -1, 0, 0};
-            walk.qleast = min(x.least, y.least);
-            walk.qmost = max(x.most, y.most);
-            walk.qpadding = x.padding | y.padding;
+        if (key_ranges) {
+            const int size = packed_tile(p.R);
+            walk.ranges = key_ranges + (long)b * ((p.Tk + kKeyTile - 1) / kKeyTile);
+            walk.own = own_range(row_ranges + (long)b * ((p.M + size - 1) / size), m0, last + 1, size);
         }
         int queue[L::kKStages + 1] = {};  // this round's tile and those behind it
         auto bring = [&](int i) {
@@ -283,7 +242,7 @@ __global__ void __launch_bounds__(kThreads, Layout<T, DP>::kPerSm)
                         tmem_loads_done();
 #pragma unroll
                         for (int j = 0; j < 16; ++j) o[j] *= factor;
-                        tmem_store16(mine + L::kO + 16 * c, reinterpret_cast<const uint32_t(&)[16]>(o));
+                        tmem_store16(mine + L::kO + 16 * c, o);
                     }
                 }
             }
@@ -412,17 +371,13 @@ __global__ void __launch_bounds__(128) attention_doc_ranges_kernel(const AttnPro
     const int b = blockIdx.y, w = blockIdx.x * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
     if (w >= key_tiles + row_tiles) return;
     const bool key = w < key_tiles;
-    const int t = key ? w : w - key_tiles, end = key ? p.Tk : p.M;
+    const int t = key ? w : w - key_tiles, size = key ? kKeyTile : packed_tile(p.R), end = min((t + 1) * size, key ? p.Tk : p.M);
     const int *ids = key ? p.doc_k + b * p.doc_k_sb : p.doc_q + b * p.doc_q_sb;
     int least = kNoLeast, most = -1, padding = 0;
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-        const int x = t * kKeyTile + lane + 32 * k;
-        if (x < end) {
-            const int id = ids[key || p.R == 1 ? x : x / p.R];
-            if (id < 0) padding = 1;
-            else { least = min(least, id); most = max(most, id); }
-        }
+    for (int x = t * size + lane; x < end; x += 32) {
+        const int id = ids[key ? x : x / p.R];
+        if (id < 0) padding = 1;
+        else { least = min(least, id); most = max(most, id); }
     }
     least = __reduce_min_sync(0xffffffffu, least);
     most = __reduce_max_sync(0xffffffffu, most);
@@ -461,11 +416,17 @@ int key_splits(const AttnProblem &p, int sms) {
 
 size_t doc_range_bytes(const AttnProblem &p) {
     if (!p.doc_k || p.Tk <= 4 * kKeyTile) return 0;  // a launch costs more than the few tiles that it might spare
-    return sizeof(DocRange) * p.B * ((size_t)(p.Tk + kKeyTile - 1) / kKeyTile + (size_t)(p.M + kKeyTile - 1) / kKeyTile);
+    const int size = packed_tile(p.R);
+    return sizeof(DocRange) * p.B * ((size_t)(p.Tk + kKeyTile - 1) / kKeyTile + (size_t)(p.M + size - 1) / size);
 }
-int doc_ranges(const AttnProblem &p, DocRange *keys, DocRange *rows, cudaStream_t stream) {
-    const int kt = (p.Tk + kKeyTile - 1) / kKeyTile, rt = (p.M + kKeyTile - 1) / kKeyTile;
-    attention_doc_ranges_kernel<<<dim3((kt + rt + 3) / 4, p.B), 128, 0, stream>>>(p, keys, rows, kt, rt);
+int doc_ranges(const AttnProblem &p, void *scratch, const DocRange **keys, const DocRange **rows, cudaStream_t stream) {
+    *keys = *rows = nullptr;
+    if (!doc_range_bytes(p)) return LUTGEMM_OK;
+    const int size = packed_tile(p.R), kt = (p.Tk + kKeyTile - 1) / kKeyTile, rt = (p.M + size - 1) / size;
+    DocRange *k = static_cast<DocRange *>(scratch), *r = k + (size_t)p.B * kt;
+    *keys = k;
+    *rows = r;
+    attention_doc_ranges_kernel<<<dim3((kt + rt + 3) / 4, p.B), 128, 0, stream>>>(p, k, r, kt, rt);
     return launch_status();
 }
 
@@ -482,15 +443,10 @@ int attention_tc_forward(const AttnProblem &p, int dtype, void *out, void *rest,
     if (!attention_map(&map_k, bf16, p.k, p.B, p.Tk, p.G, 1, p.D) || !attention_map(&map_v, bf16, p.v, p.B, p.Tk, p.G, 1, p.D))
         return LUTGEMM_E_BADARG;
     const int splits = key_splits(p, sms), dp = p.D <= 64 ? 64 : 128;
-    DocRange *kr = nullptr, *rr = nullptr;
-    const size_t ranges = doc_range_bytes(p);
-    if (ranges) {
-        kr = static_cast<DocRange *>(scratch);
-        rr = kr + (size_t)p.B * ((p.Tk + kKeyTile - 1) / kKeyTile);
-        const int rc = doc_ranges(p, kr, rr, stream);
-        if (rc != LUTGEMM_OK) return rc;
-    }
-    float *part = reinterpret_cast<float *>(static_cast<uint8_t *>(scratch) + ranges), *part_lse = part + (size_t)splits * p.B * p.G * p.M * dp;
+    const DocRange *kr, *rr;
+    const int rc = doc_ranges(p, scratch, &kr, &rr, stream);
+    if (rc != LUTGEMM_OK) return rc;
+    float *part = reinterpret_cast<float *>(static_cast<uint8_t *>(scratch) + doc_range_bytes(p)), *part_lse = part + (size_t)splits * p.B * p.G * p.M * dp;
     const bool bent = p.cap > 0.f || p.slopes || !(p.scale > 0.f);
 #define RUN(T, DP) (bent ? launch<T, DP, true>(p, map_k, map_v, kr, rr, out, rest, lse, part, part_lse, splits, error_word, stream) \
                          : launch<T, DP, false>(p, map_k, map_v, kr, rr, out, rest, lse, part, part_lse, splits, error_word, stream))

@@ -100,6 +100,55 @@ __device__ __forceinline__ void copy_row_tile(uint32_t dst, const AttnProblem &p
     }
 }
 
+// Tiles that a block has to visit, in ascending order: [at, end), or, with ranges of documents, those of them whose documents overlap
+// the block's own.  For one warp, every lane alike.
+struct TileWalk {
+    const DocRange *ranges = nullptr;  // of this row of the batch, or null
+    DocRange own{};                    // documents of the block's rows or keys
+    int at = 0, end = 0;
+    int whole_first = 0, whole_last = 0;  // tiles of which the masks by place leave everything
+    int base = 0;
+    uint32_t visit = 0, whole = 0;  // with ranges: tiles of [base - 32, base) that are left, and those of them without a mask
+
+    // the next tile times two, plus one where no element of it is masked; -1: none
+    __device__ __forceinline__ int next(bool docs) {
+        if (!ranges) {
+            if (at >= end) return -1;
+            const int t = at++;
+            return 2 * t + (!docs && t >= whole_first && t <= whole_last);
+        }
+        while (!visit) {
+            if (base < at) base = at;  // (the first time)
+            if (base >= end) return -1;
+            const int t = base + (threadIdx.x & 31);
+            bool see = false, all = false;
+            if (t < end) {
+                const DocRange r = ranges[t];
+                see = r.least <= own.most && r.most >= own.least;
+                all = see && own.least == own.most && r.least == r.most && !r.padding && !own.padding && t >= whole_first &&
+                      t <= whole_last;
+            }
+            visit = __ballot_sync(0xffffffffu, see);
+            whole = __ballot_sync(0xffffffffu, all);
+            base += 32;
+        }
+        const int bit = __ffs(visit) - 1;
+        visit &= visit - 1;
+        return 2 * (base - 32 + bit) + (whole >> bit & 1);
+    }
+};
+// documents of [first, end) of an axis cut into tiles of `size`
+__device__ __forceinline__ DocRange own_range(const DocRange *ranges, int first, int end, int size) {
+    DocRange r{kNoLeast, -1, 0, 0};
+    for (int t = first / size; t <= (end - 1) / size; ++t) {
+        r.least = min(r.least, ranges[t].least);
+        r.most = max(r.most, ranges[t].most);
+        r.padding |= ranges[t].padding;
+    }
+    return r;
+}
+__host__ __device__ constexpr int packed_tile(int R) { return 64 / R * R; }  // rows of a bulk copy of packed rows: whole tokens
+
 // what a thread knows of its row
 struct TileRow {
     int limit, doc;  // last key (-1: none), document
@@ -147,9 +196,9 @@ inline bool attention_map(CUtensorMap *map, bool bf16, const AttnTensor &t, int 
     return make_tensor_map_16bit_5d(map, bf16, t.p, dims, strides, box);
 }
 
-// lutgemm_attention_tc.cu: ranges of the documents of tiles of 64 keys and 64 packed rows ([B][tiles] each); nullptr where nothing
-// is gained by them
+// lutgemm_attention_tc.cu: ranges of the documents of tiles of 64 keys and of packed_tile(R) rows ([B][tiles] each); no bytes where
+// nothing is gained by them
 size_t doc_range_bytes(const AttnProblem &p);
-int doc_ranges(const AttnProblem &p, DocRange *keys, DocRange *rows, cudaStream_t stream);
+int doc_ranges(const AttnProblem &p, void *scratch, const DocRange **keys, const DocRange **rows, cudaStream_t stream);
 
 }  // namespace lutgemm

@@ -289,10 +289,15 @@ struct AttnTensor;
 size_t attention_tc_scratch_bytes(const AttnProblem &p, int num_sms);
 int attention_tc_forward(const AttnProblem &p, int dtype, void *out, void *rest, float *lse, void *scratch, int num_sms, cudaStream_t stream);
 
+// lutgemm_attention_tc_grad.cu
+size_t attention_tc_backward_scratch_bytes(const AttnProblem &p);
+int attention_tc_backward(const AttnProblem &p, int dtype, const AttnTensor &go, const void *out, const void *rest, const float *lse, void *gq,
+                          void *gk, void *gv, void *scratch, cudaStream_t stream);
+
 // lutgemm_attention_f32.cu
-int attention_f32_forward(const AttnProblem &p, int dtype, void *out, float *lse, cudaStream_t stream);
-int attention_f32_backward(const AttnProblem &p, int dtype, const AttnTensor &go, const void *out, const float *lse, float *delta, void *gq,
-                           void *gk, void *gv, cudaStream_t stream);
+int attention_f32_forward(const AttnProblem &p, float *out, float *lse, cudaStream_t stream);
+int attention_f32_backward(const AttnProblem &p, const AttnTensor &go, const float *out, const float *lse, float *delta, float *gq, float *gk,
+                           float *gv, cudaStream_t stream);
 
 // lutgemm_norm_rotate.cu; index 0: queries, 1: keys
 struct NormOperand {

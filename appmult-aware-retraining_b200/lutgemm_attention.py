@@ -186,21 +186,24 @@ class _Attention(torch.autograd.Function):
                  *((doc_q.data_ptr(), doc_q.stride(0), doc_k.data_ptr(), doc_k.stride(0)) if doc_q is not None else (None, 0, None, 0)))
         out = torch.empty((B, Tq, H, D), dtype=q.dtype, device=q.device)
         lse = torch.empty((B, G, Tq * H // G), dtype=torch.float32, device=q.device)
+        # (the backward pass of 16-bit operands wants what the rounding of out leaves, too)
+        rest = torch.empty_like(out) if q.dtype is not torch.float32 and any(ctx.needs_input_grad[:3]) else None
         lib, dtype = approx_ops.library(), _DTYPES[q.dtype]
         with approx_ops._guard(q.device):
             nbytes = lib.lutgemm_attention_scratch_bytes(dtype, B, Tq, Tk, H, G, D, doc_k is not None) if dtype else 0
             scratch = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
-            rc = lib.lutgemm_attention(*_at(q), *_at(k), *_at(v), out.data_ptr(), None, lse.data_ptr(), dtype, B, Tq, Tk, H, G, D, *masks,
+            rc = lib.lutgemm_attention(*_at(q), *_at(k), *_at(v), out.data_ptr(),
+                                       rest.data_ptr() if rest is not None else None, lse.data_ptr(), dtype, B, Tq, Tk, H, G, D, *masks,
                                        scratch.data_ptr() if nbytes else None, nbytes, approx_ops._stream_ptr(q.device))
         approx_ops._check(rc, "attention")
-        ctx.save_for_backward(q, k, v, out, lse, slopes, prefix, doc_q, doc_k)
+        ctx.save_for_backward(q, k, v, out, rest, lse, slopes, prefix, doc_q, doc_k)
         ctx.cfg = (scale, cap, causal)
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, go):
-        q, k, v, out, lse, slopes, prefix, doc_q, doc_k = ctx.saved_tensors
+        q, k, v, out, rest, lse, slopes, prefix, doc_q, doc_k = ctx.saved_tensors
         scale, cap, causal = ctx.cfg
         B, Tq, H, D = q.shape
         Tk, G = k.shape[1], k.shape[2]
@@ -211,11 +214,13 @@ class _Attention(torch.autograd.Function):
         dq = torch.empty((B, Tq, H, D), dtype=q.dtype, device=q.device)
         dk = torch.empty((B, Tk, G, D), dtype=q.dtype, device=q.device)
         dv = torch.empty((B, Tk, G, D), dtype=q.dtype, device=q.device)
-        delta = torch.empty_like(lse)
-        lib = approx_ops.library()
+        lib, dtype = approx_ops.library(), _DTYPES[q.dtype]
         with approx_ops._guard(q.device):
-            rc = lib.lutgemm_attention_backward(*_at(go), *_at(q), *_at(k), *_at(v), out.data_ptr(), lse.data_ptr(), delta.data_ptr(),
-                                                dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _DTYPES[q.dtype], B, Tq, Tk, H, G, D, *masks,
+            nbytes = lib.lutgemm_attention_backward_scratch_bytes(dtype, B, Tq, Tk, H, G, D, doc_k is not None)
+            scratch = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
+            rc = lib.lutgemm_attention_backward(*_at(go), *_at(q), *_at(k), *_at(v), out.data_ptr(),
+                                                rest.data_ptr() if rest is not None else None, lse.data_ptr(), dq.data_ptr(),
+                                                dk.data_ptr(), dv.data_ptr(), dtype, B, Tq, Tk, H, G, D, *masks, scratch.data_ptr(), nbytes,
                                                 approx_ops._stream_ptr(q.device))
         approx_ops._check(rc, "attention (backward)")
         return dq, dk, dv, None, None, None, None, None, None, None

@@ -402,18 +402,19 @@ int lutgemm_norm_rotate_backward(const void *gq, long gq_sb, long gq_st, long gq
  * `lse` fp32 [B, G, Tq * H/G]: statistics for the backward pass (log 2 of the sum of exponentials, rows ordered query by query).
  * H a multiple of G and at most 64 G, D a multiple of 8 up to 128.  16-bit operands are read by bulk copies: their addresses and strides
  * are multiples of 16 bytes, and no stride of an axis of several elements is 0.  `out_rest` (16-bit types; NULL where no backward pass follows): what the rounding of `out` leaves, as `out`.
- * `delta`: fp32 scratch of the size of `lse`.
  */
 size_t lutgemm_attention_scratch_bytes(int dtype, int B, int Tq, int Tk, int H, int G, int D, int documents);
 int lutgemm_attention(const void *q, long q_sb, long q_st, long q_sh, const void *k, long k_sb, long k_st, long k_sh, const void *v,
                       long v_sb, long v_st, long v_sh, void *out, void *out_rest, float *lse, int dtype, int B, int Tq, int Tk, int H,
                       int G, int D, float scale, float cap, const float *slopes, int causal, const int *prefix, const int *doc_q,
                       long doc_q_sb, const int *doc_k, long doc_k_sb, void *scratch, size_t scratch_bytes, void *stream);
+size_t lutgemm_attention_backward_scratch_bytes(int dtype, int B, int Tq, int Tk, int H, int G, int D, int documents);
 int lutgemm_attention_backward(const void *go, long go_sb, long go_st, long go_sh, const void *q, long q_sb, long q_st, long q_sh,
                                const void *k, long k_sb, long k_st, long k_sh, const void *v, long v_sb, long v_st, long v_sh,
-                               const void *out, const float *lse, float *delta, void *dq, void *dk, void *dv, int dtype, int B, int Tq,
-                               int Tk, int H, int G, int D, float scale, float cap, const float *slopes, int causal,
-                               const int *prefix, const int *doc_q, long doc_q_sb, const int *doc_k, long doc_k_sb, void *stream);
+                               const void *out, const void *out_rest, const float *lse, void *dq, void *dk, void *dv, int dtype, int B,
+                               int Tq, int Tk, int H, int G, int D, float scale, float cap, const float *slopes, int causal,
+                               const int *prefix, const int *doc_q, long doc_q_sb, const int *doc_k, long doc_k_sb, void *scratch,
+                               size_t scratch_bytes, void *stream);
 
 /*
  * For each of N rows of C logits, `pitch` elements apart: logp[n] = log softmax(logits[n])[target[n]] (0 where the target is `ignore`,
