@@ -1162,6 +1162,9 @@ static int attention_args(lutgemm::AttnProblem *p, int dtype, int B, int Tq, int
     return LUTGEMM_OK;
 }
 
+// fp32 heads of more than 64 values, whose planes do not fit shared memory, run on the fp32 pipes
+static bool attention_on_fp32_pipes(int dtype, int D) { return dtype == LUTGEMM_F32 && D > 64; }
+
 // 16-byte vectors of 16-bit operands: strides of axes that have more than one element
 static bool attention_vectors(const lutgemm::AttnTensor &t, int B, int T, int heads) {
     const auto fits = [](long stride, int count) { return count == 1 || (stride > 0 && stride % 8 == 0); };
@@ -1171,10 +1174,11 @@ static bool attention_vectors(const lutgemm::AttnTensor &t, int B, int T, int he
 size_t lutgemm_attention_scratch_bytes(int dtype, int B, int Tq, int Tk, int H, int G, int D, int documents) {
     lutgemm::AttnProblem p{};
     const int *ids = documents ? reinterpret_cast<const int *>(16) : nullptr;
-    if (dtype == LUTGEMM_F32 || attention_args(&p, dtype, B, Tq, Tk, H, G, D, 1.f, 0.f, nullptr, 0, nullptr, ids, 0, ids, 0) != LUTGEMM_OK)
+    if (attention_on_fp32_pipes(dtype, D) ||
+        attention_args(&p, dtype, B, Tq, Tk, H, G, D, 1.f, 0.f, nullptr, 0, nullptr, ids, 0, ids, 0) != LUTGEMM_OK)
         return 0;
     const int sms = current_num_sms();
-    return sms <= 0 ? 0 : lutgemm::attention_tc_scratch_bytes(p, sms);
+    return sms <= 0 ? 0 : lutgemm::attention_tc_scratch_bytes(p, dtype, sms);
 }
 
 int lutgemm_attention(const void *q, long q_sb, long q_st, long q_sh, const void *k, long k_sb, long k_st, long k_sh, const void *v,
@@ -1185,13 +1189,15 @@ int lutgemm_attention(const void *q, long q_sb, long q_st, long q_sh, const void
     lutgemm::AttnProblem p{{q, q_sb, q_st, q_sh}, {k, k_sb, k_st, k_sh}, {v, v_sb, v_st, v_sh}};
     const int rc = attention_args(&p, dtype, B, Tq, Tk, H, G, D, scale, cap, slopes, causal, prefix, doc_q, doc_q_sb, doc_k, doc_k_sb);
     if (rc != LUTGEMM_OK) return rc;
-    if (dtype == LUTGEMM_F32) return lutgemm::attention_f32_forward(p, static_cast<float *>(out), lse, static_cast<cudaStream_t>(stream));
-    if (!attention_vectors(p.q, B, Tq, H) || !attention_vectors(p.k, B, Tk, G) || !attention_vectors(p.v, B, Tk, G) ||
+    if (attention_on_fp32_pipes(dtype, D))
+        return lutgemm::attention_f32_forward(p, static_cast<float *>(out), lse, static_cast<cudaStream_t>(stream));
+    if ((dtype != LUTGEMM_F32 &&
+         (!attention_vectors(p.q, B, Tq, H) || !attention_vectors(p.k, B, Tk, G) || !attention_vectors(p.v, B, Tk, G))) ||
         ((reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(out_rest)) & 15))
         return LUTGEMM_E_BADARG;
     const int sms = current_num_sms();
     if (sms <= 0) return LUTGEMM_E_CUDA;
-    const size_t need = lutgemm::attention_tc_scratch_bytes(p, sms);
+    const size_t need = lutgemm::attention_tc_scratch_bytes(p, dtype, sms);
     if (scratch_bytes < need) return LUTGEMM_E_SCRATCH;
     if (need && (!scratch || (reinterpret_cast<uintptr_t>(scratch) & 15))) return LUTGEMM_E_BADARG;
     return lutgemm::attention_tc_forward(p, dtype, out, out_rest, lse, scratch, sms, static_cast<cudaStream_t>(stream));
@@ -1201,7 +1207,7 @@ size_t lutgemm_attention_backward_scratch_bytes(int dtype, int B, int Tq, int Tk
     lutgemm::AttnProblem p{};
     const int *ids = documents ? reinterpret_cast<const int *>(16) : nullptr;
     if (attention_args(&p, dtype, B, Tq, Tk, H, G, D, 1.f, 0.f, nullptr, 0, nullptr, ids, 0, ids, 0) != LUTGEMM_OK) return 0;
-    return dtype == LUTGEMM_F32 ? sizeof(float) * (size_t)B * G * p.M : lutgemm::attention_tc_backward_scratch_bytes(p);
+    return attention_on_fp32_pipes(dtype, D) ? sizeof(float) * (size_t)B * G * p.M : lutgemm::attention_tc_backward_scratch_bytes(p, dtype);
 }
 
 int lutgemm_attention_backward(const void *go, long go_sb, long go_st, long go_sh, const void *q, long q_sb, long q_st, long q_sh,
@@ -1218,11 +1224,11 @@ int lutgemm_attention_backward(const void *go, long go_sb, long go_st, long go_s
     if (!scratch || (reinterpret_cast<uintptr_t>(scratch) & 15)) return LUTGEMM_E_BADARG;
     const lutgemm::AttnTensor g{go, go_sb, go_st, go_sh};
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
-    if (dtype == LUTGEMM_F32)
+    if (attention_on_fp32_pipes(dtype, D))
         return lutgemm::attention_f32_backward(p, g, static_cast<const float *>(out), lse, static_cast<float *>(scratch),
                                                static_cast<float *>(dq), static_cast<float *>(dk), static_cast<float *>(dv), s);
-    if (!attention_vectors(p.q, B, Tq, H) || !attention_vectors(p.k, B, Tk, G) || !attention_vectors(p.v, B, Tk, G) ||
-        !attention_vectors(g, B, Tq, H) || !out_rest ||
+    if ((dtype != LUTGEMM_F32 && (!attention_vectors(p.q, B, Tq, H) || !attention_vectors(p.k, B, Tk, G) ||
+                                  !attention_vectors(p.v, B, Tk, G) || !attention_vectors(g, B, Tq, H) || !out_rest)) ||
         ((reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(out_rest) | reinterpret_cast<uintptr_t>(dq) |
           reinterpret_cast<uintptr_t>(dk) | reinterpret_cast<uintptr_t>(dv)) & 15))
         return LUTGEMM_E_BADARG;

@@ -1,4 +1,4 @@
-// Attention of fp32 operands on the fp32 pipes.
+// Attention of fp32 operands on the fp32 pipes: heads of 65 to 128 values.
 #include "lutgemm.h"
 #include "lutgemm_attention.cuh"
 #include "lutgemm_kernels.h"
@@ -374,12 +374,12 @@ int backward(const AttnProblem &p, const AttnTensor &go, const float *out, const
 }  // namespace
 
 int attention_f32_forward(const AttnProblem &p, float *out, float *lse, cudaStream_t stream) {
-    return p.D > 64 ? forward<128>(p, out, lse, stream) : forward<64>(p, out, lse, stream);
+    return forward<128>(p, out, lse, stream);
 }
 
 int attention_f32_backward(const AttnProblem &p, const AttnTensor &go, const float *out, const float *lse, float *delta, float *gq, float *gk,
                            float *gv, cudaStream_t stream) {
-    return p.D > 64 ? backward<128>(p, go, out, lse, delta, gq, gk, gv, stream) : backward<64>(p, go, out, lse, delta, gq, gk, gv, stream);
+    return backward<128>(p, go, out, lse, delta, gq, gk, gv, stream);
 }
 
 }  // namespace lutgemm

@@ -1,4 +1,4 @@
-// Attention forward on the tensor cores, 16-bit operands.
+// Attention forward on the tensor cores: 16-bit operands, and fp32 ones as three bf16 planes.
 #include "lutgemm_attention_tc.cuh"
 #include "lutgemm_kernels.h"
 
@@ -18,12 +18,17 @@ constexpr int kThreads = 160;  // four warps with a row to a thread, one that br
 // The running maximum is only raised, and O rescaled, where a row's maximum grows by more than 8 in log 2: probabilities
 // then reach 2^8, sums are fp32.  fp16 probabilities are kept 2^7 larger, out of its subnormal range.
 // P is rounded to the operands' type, as the tensor cores take it; its row sums are of the unrounded values.
+// fp32: P is split into planes as the operands were, and each tile's products with V start from zero and are added up in registers: the
+// tensor cores cut off what an addition loses, which over a long row would add up.
 template <typename T, int DP>
 struct Layout {
-    static constexpr int kBlocks = DP / 64, kStages = DP == 64 ? 1 : 2, kKStages = kStages + 1, kPerSm = DP == 64 ? 3 : 2;
-    static constexpr uint32_t kQ = 0, kK = kRowTile * DP * 2, kTile = kKeyTile * DP * 2, kV = kK + kKStages * kTile,
-                              kBars = kV + 2 * kTile, kBytes = kBars + 128;
-    static constexpr uint32_t kColumns = DP == 64 ? 128 : 256, kO = kStages * 64;  // tensor memory: S, then O
+    using Op = Operand<T, DP>;
+    static constexpr int kBlocks = Op::kBlocks, kStages = DP == 64 && !Op::kPlanes ? 1 : 2, kKStages = kStages + 1;
+    static constexpr int kPerSm = Op::kPlanes ? 1 : DP == 64 ? 3 : 2;
+    static constexpr uint32_t kTile = kKeyTile * kBlocks * 128, kQ = 0, kK = 2 * kTile, kV = kK + kKStages * kTile, kBars = kV + 2 * kTile,
+                              kBytes = kBars + 128;
+    static constexpr uint32_t kS = Op::kPlanes ? 96 : 64, kO = kStages * kS;  // tensor memory: S or P of each stage, then O
+    static constexpr uint32_t kColumns = kO + DP <= 128 ? 128 : 256;
 };
 constexpr int kEnd = -1;  // in place of a tile: there are no more
 
@@ -33,7 +38,9 @@ __global__ void __launch_bounds__(kThreads, Layout<T, DP>::kPerSm)
                         const DocRange *key_ranges, const DocRange *row_ranges, T *out, T *rest, float *lse,
                         float *part, float *part_lse, int splits, int *error_word) {
     using L = Layout<T, DP>;
-    constexpr float kShift = IsBf16<T>::value ? 0.f : 7.f;
+    using Op = typename L::Op;
+    constexpr float kShift = Op::kBf16 ? 0.f : 7.f;
+    const int width = Op::kPlanes ? kPlaneWidth : p.D;
     extern __shared__ __align__(1024) uint8_t smem[];
     const uint32_t base = smem_u32(smem), bar_s = base + L::kBars, bar_o = bar_s + 16, bar_p = bar_s + 24, bar_k = bar_s + 32, bar_v = bar_s + 56;
     volatile int *abort_word = reinterpret_cast<int *>(smem + L::kBars + 72);
@@ -96,16 +103,16 @@ __global__ void __launch_bounds__(kThreads, Layout<T, DP>::kPerSm)
         bring_v(0, 0);
         tmem_after_sync();
         const uint32_t tmem = *slot;
-        constexpr uint32_t desc_s = mma_descriptor(IsBf16<T>::value, kKeyTile, false), desc_o = mma_descriptor(IsBf16<T>::value, DP, true);
+        constexpr uint32_t desc_s = mma_descriptor(Op::kBf16, kKeyTile, false), desc_o = mma_descriptor(Op::kBf16, DP, true);
         auto issue_scores = [&](int n, int tile) {  // S of round n, or word that there is none; one lane
             const uint32_t bar = bar_s + 8 * (n % L::kStages);
             tiles[n & 3] = tile;
             if (tile >= 0) {
-                const uint32_t k = base + L::kK + (n % L::kKStages) * L::kTile, d = tmem + (n % L::kStages) * 64;
+                const uint32_t k = base + L::kK + (n % L::kKStages) * L::kTile, d = tmem + (n % L::kStages) * L::kS;
 #pragma unroll
-                for (int i = 0; i < DP / 16; ++i)
-                    mma_ss(d, smem_descriptor(base + L::kQ + (i >> 2) * kRowTile * 128 + (i & 3) * 32, 0),
-                           smem_descriptor(k + (i >> 2) * kKeyTile * 128 + (i & 3) * 32, 0), desc_s, i > 0);
+                for (int i = 0; i < 4 * Op::kProducts; ++i)
+                    mma_ss(d, smem_descriptor(base + L::kQ + Op::a(i >> 2) * kRowTile * 128 + (i & 3) * 32, 0),
+                           smem_descriptor(k + Op::b(i >> 2) * kKeyTile * 128 + (i & 3) * 32, 0), desc_s, i > 0);
                 mma_commit(bar);
             } else {
                 mbar_arrive(bar);
@@ -121,7 +128,7 @@ __global__ void __launch_bounds__(kThreads, Layout<T, DP>::kPerSm)
         for (int n = 0; queue[0] >= 0; ++n) {
             bring(L::kStages + 1);
             mbar_wait(bar_v + 8 * (n & 1), n >> 1 & 1, 207, abort_word, error_word);
-            if (docs) {  // a probability of zero does not hide what padding may hold
+            if (docs && !Op::kPlanes) {  // a probability of zero does not hide what padding may hold
                 const unsigned long long mask = key_mask(p, b, (queue[0] >> 1) * kKeyTile);
                 if (~mask) {
                     clear_rows<L::kBlocks>(smem + L::kV + (n & 1) * L::kTile, mask);
@@ -134,10 +141,17 @@ __global__ void __launch_bounds__(kThreads, Layout<T, DP>::kPerSm)
             tmem_after_sync();
             __syncwarp();
             if ((tid & 31) == 0) {
-                const uint32_t v = base + L::kV + (n & 1) * L::kTile, a = tmem + (n % L::kStages) * 64;
+                const uint32_t v = base + L::kV + (n & 1) * L::kTile, a = tmem + (n % L::kStages) * L::kS;
+                if constexpr (Op::kPlanes) {
 #pragma unroll
-                for (int i = 0; i < kKeyTile / 16; ++i)
-                    mma_ts(tmem + L::kO, a + 8 * i, smem_descriptor(v + i * 16 * 128, kKeyTile * 128), desc_o, n > 0 || i > 0);
+                    for (int i = 0; i < 4 * Op::kProducts; ++i)
+                        mma_ts(tmem + L::kO, a + 32 * Op::a(i >> 2) + 8 * (i & 3),
+                               smem_descriptor(v + Op::b(i >> 2) * kKeyTile * 128 + (i & 3) * 16 * 128, 0), desc_o, i > 0);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < kKeyTile / 16; ++i)
+                        mma_ts(tmem + L::kO, a + 8 * i, smem_descriptor(v + i * 16 * 128, kKeyTile * 128), desc_o, n > 0 || i > 0);
+                }
                 mma_commit(bar_o);
                 if (queue[L::kStages - 1] >= 0) issue_scores(n + L::kStages, queue[L::kStages]);
             }
@@ -149,7 +163,7 @@ __global__ void __launch_bounds__(kThreads, Layout<T, DP>::kPerSm)
             for (int i = 0; i <= L::kStages; ++i) queue[i] = queue[i + 1];
         }
     } else {
-        copy_row_tile<L::kBlocks>(base + L::kQ, p, p.q, b, g, m0, tid);
+        copy_row_tile<L::kBlocks>(base + L::kQ, p, p.q, width, b, g, m0, tid);
         copies_end_group();
         copies_wait<0>();
         writes_to_tensor_cores();
@@ -159,15 +173,30 @@ __global__ void __launch_bounds__(kThreads, Layout<T, DP>::kPerSm)
         const int m = m0 + tid;
         const TileRow row = tile_row(p, b, g, m, pre);
         const bool idle = __all_sync(0xffffffffu, row.limit < 0);  // the warp's rows see nothing
-        const Bend bend = make_bend(p);
+        const Bend bend = make_bend<Op::kPlanes>(p);
         float most = -INFINITY, sum = 0.f;  // the maximum that P is relative to, in log 2
+        f32x2 total_o[Op::kPlanes ? 32 : 1] = {};
+        auto add_tile = [&](float factor) {  // fp32: the products of the round before
+            const f32x2 f2 = pack2(factor, factor);
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                float o[32];
+                tmem_load32(mine + L::kO + 32 * c, o);
+                tmem_loads_done();
+#pragma unroll
+                for (int j = 0; j < 16; ++j) {
+                    f32x2 &t = total_o[Op::kPlanes ? 16 * c + j : 0];
+                    t = mul2(add2(t, pack2(o[2 * j], o[2 * j + 1])), f2);
+                }
+            }
+        };
         int n = 0;
         for (;; ++n) {
             mbar_wait(bar_s + 8 * (n % L::kStages), (n / L::kStages) & 1, 202, abort_word, error_word);
             const int tile = tiles[n & 3];
             if (tile < 0 || *abort_word) break;
             tmem_after_sync();
-            const uint32_t s_at = mine + (n % L::kStages) * 64;
+            const uint32_t s_at = mine + (n % L::kStages) * L::kS;
             if (idle) {
                 // whatever the P of these rows holds stays in their rows of O, which are not used
                 if (n > 0) mbar_wait(bar_o, (n - 1) & 1, 203, abort_word, error_word);
@@ -184,7 +213,10 @@ __global__ void __launch_bounds__(kThreads, Layout<T, DP>::kPerSm)
 #pragma unroll
                     for (int h = 0; h < 2; ++h)
 #pragma unroll
-                        for (int j = 0; j < 32; ++j) s[h][j] = bend.k1 - bend.k2 * fast_rcp(1.f + fast_exp2(s[h][j] * bend.in));
+                        for (int j = 0; j < 32; ++j) {
+                            float unused;
+                            s[h][j] = bend.capped<Op::kPlanes>(s[h][j], &unused);
+                        }
                 } else {
 #pragma unroll
                     for (int h = 0; h < 2; ++h)
@@ -233,7 +265,10 @@ __global__ void __launch_bounds__(kThreads, Layout<T, DP>::kPerSm)
             }
             if (n > 0) {
                 mbar_wait(bar_o, (n - 1) & 1, 204, abort_word, error_word);
-                if (__any_sync(0xffffffffu, raise)) {
+                if constexpr (Op::kPlanes) {
+                    tmem_after_sync();
+                    add_tile(factor);
+                } else if (__any_sync(0xffffffffu, raise)) {
                     tmem_after_sync();
 #pragma unroll
                     for (int c = 0; c < DP / 16; ++c) {
@@ -251,16 +286,17 @@ __global__ void __launch_bounds__(kThreads, Layout<T, DP>::kPerSm)
             f32x2 add[2] = {0ull, 0ull};
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                uint32_t w[16];
+                uint32_t w[Op::kPlanes ? 3 : 1][16];
 #pragma unroll
                 for (int j = 0; j < 32; j += 2) {
                     const f32x2 x = pack2(s[h][j], s[h][j + 1]);
                     const float2 y = unpack2(BENT ? add2(x, less2) : fma2(x, scale2, less2));
                     const float a = fast_exp2(y.x), c = fast_exp2(y.y);
                     add[j / 2 & 1] = add2(add[j / 2 & 1], pack2(a, c));
-                    w[j / 2] = pack_pair<T>(a, c);
+                    plane_words<T>(w, j / 2, a, c);
                 }
-                tmem_store16(s_at + 16 * h, w);
+#pragma unroll
+                for (int e = 0; e < (Op::kPlanes ? 3 : 1); ++e) tmem_store16(s_at + 32 * e + 16 * h, w[e]);
             }
             const float2 total = unpack2(add2(add[0], add[1]));
             sum += total.x + total.y;
@@ -271,6 +307,8 @@ __global__ void __launch_bounds__(kThreads, Layout<T, DP>::kPerSm)
         if (n > 0) {
             mbar_wait(bar_o, (n - 1) & 1, 205, abort_word, error_word);
             tmem_after_sync();
+            if constexpr (Op::kPlanes)
+                if (!idle) add_tile(1.f);
         }
         const float inv = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : NAN;
         const float stat = sum == 0.f ? INFINITY : most - kShift + log2f(sum);
@@ -279,7 +317,14 @@ __global__ void __launch_bounds__(kThreads, Layout<T, DP>::kPerSm)
 #pragma unroll
         for (int c = 0; c < DP / 32; ++c) {
             float o[32];
-            if (n > 0) {
+            if constexpr (Op::kPlanes) {
+#pragma unroll
+                for (int j = 0; j < 16; ++j) {
+                    const float2 t = unpack2(total_o[16 * c + j]);
+                    o[2 * j] = t.x;
+                    o[2 * j + 1] = t.y;
+                }
+            } else if (n > 0) {
                 tmem_load32(mine + L::kO + 32 * c, o);
                 tmem_loads_done();
             }
@@ -295,6 +340,10 @@ __global__ void __launch_bounds__(kThreads, Layout<T, DP>::kPerSm)
 #pragma unroll
                     for (int j = 0; j < 32; j += 8) {
                         if (32 * c + j >= p.D) break;
+                        if constexpr (Op::kPlanes) {
+                            *reinterpret_cast<float4 *>(out + to + j) = make_float4(o[j], o[j + 1], o[j + 2], o[j + 3]);
+                            *reinterpret_cast<float4 *>(out + to + j + 4) = make_float4(o[j + 4], o[j + 5], o[j + 6], o[j + 7]);
+                        } else {
                         uint4 v;
                         uint32_t *r = &v.x;
 #pragma unroll
@@ -307,6 +356,7 @@ __global__ void __launch_bounds__(kThreads, Layout<T, DP>::kPerSm)
                                 r[e] = pack_pair<T>(o[j + 2 * e] - hi.x, o[j + 2 * e + 1] - hi.y);
                             }
                             *reinterpret_cast<uint4 *>(rest + to + j) = v;
+                        }
                         }
                     }
                 }
@@ -406,8 +456,8 @@ int launch(const AttnProblem &p, const CUtensorMap &map_k, const CUtensorMap &ma
 }
 
 // Parts of the keys: as many as fill the blocks that the GPU holds at a time, of at least four tiles each.
-int key_splits(const AttnProblem &p, int sms) {
-    const long blocks = (long)((p.M + kRowTile - 1) / kRowTile) * p.B * p.G, slots = (long)sms * (p.D <= 64 ? 3 : 2);
+int key_splits(const AttnProblem &p, int dtype, int sms) {
+    const long blocks = (long)((p.M + kRowTile - 1) / kRowTile) * p.B * p.G, slots = (long)sms * (dtype == LUTGEMM_F32 ? 1 : p.D <= 64 ? 3 : 2);
     const long most = (p.Tk + 4 * kKeyTile - 1) / (4 * kKeyTile), want = slots / blocks;
     return (int)(want < 2 || most < 2 ? 1 : want < most ? want : most);
 }
@@ -430,26 +480,45 @@ int doc_ranges(const AttnProblem &p, void *scratch, const DocRange **keys, const
     return launch_status();
 }
 
-size_t attention_tc_scratch_bytes(const AttnProblem &p, int sms) {
-    const int splits = key_splits(p, sms), dp = p.D <= 64 ? 64 : 128;
-    return doc_range_bytes(p) + (splits > 1 ? sizeof(float) * (size_t)splits * p.B * p.G * p.M * (dp + 1) : 0);
+// fp32: the planes of q, k and v; then ranges of documents and the parts of split rows
+size_t attention_tc_scratch_bytes(const AttnProblem &p, int dtype, int sms) {
+    const int splits = key_splits(p, dtype, sms), dp = p.D <= 64 ? 64 : 128;
+    return (dtype == LUTGEMM_F32 ? plane_bytes(p.B, p.Tq, p.H) + 2 * plane_bytes(p.B, p.Tk, p.G) : 0) + doc_range_bytes(p) +
+           (splits > 1 ? sizeof(float) * (size_t)splits * p.B * p.G * p.M * (dp + 1) : 0);
 }
 
-int attention_tc_forward(const AttnProblem &p, int dtype, void *out, void *rest, float *lse, void *scratch, int sms, cudaStream_t stream) {
+int attention_tc_forward(const AttnProblem &problem, int dtype, void *out, void *rest, float *lse, void *scratch, int sms, cudaStream_t stream) {
+    AttnProblem p = problem;
     int *error_word = device_error_word();
     if (!error_word) return LUTGEMM_E_CUDA;
+    uint8_t *at = static_cast<uint8_t *>(scratch);
+    int rc;
+    if (dtype == LUTGEMM_F32) {
+        const size_t nq = plane_bytes(p.B, p.Tq, p.H), nk = plane_bytes(p.B, p.Tk, p.G);
+        const SplitOperand ops[3] = {{p.q, reinterpret_cast<__nv_bfloat16 *>(at), p.doc_q, p.doc_q_sb, p.Tq, p.H},
+                                     {p.k, reinterpret_cast<__nv_bfloat16 *>(at + nq), p.doc_k, p.doc_k_sb, p.Tk, p.G},
+                                     {p.v, reinterpret_cast<__nv_bfloat16 *>(at + nq + nk), p.doc_k, p.doc_k_sb, p.Tk, p.G}};
+        rc = attention_split(p, ops, 3, nullptr, nullptr, stream);
+        if (rc != LUTGEMM_OK) return rc;
+        p.q = plane_tensor(ops[0].to, p.Tq, p.H);
+        p.k = plane_tensor(ops[1].to, p.Tk, p.G);
+        p.v = plane_tensor(ops[2].to, p.Tk, p.G);
+        at += nq + 2 * nk;
+    }
     CUtensorMap map_k, map_v;
-    const bool bf16 = dtype == LUTGEMM_BF16;
-    if (!attention_map(&map_k, bf16, p.k, p.B, p.Tk, p.G, 1, p.D) || !attention_map(&map_v, bf16, p.v, p.B, p.Tk, p.G, 1, p.D))
+    const bool bf16 = dtype != LUTGEMM_F16;
+    const int width = dtype == LUTGEMM_F32 ? kPlaneWidth : p.D;
+    if (!attention_map(&map_k, bf16, p.k, p.B, p.Tk, p.G, 1, width) || !attention_map(&map_v, bf16, p.v, p.B, p.Tk, p.G, 1, width))
         return LUTGEMM_E_BADARG;
-    const int splits = key_splits(p, sms), dp = p.D <= 64 ? 64 : 128;
+    const int splits = key_splits(p, dtype, sms), dp = p.D <= 64 ? 64 : 128;
     const DocRange *kr, *rr;
-    const int rc = doc_ranges(p, scratch, &kr, &rr, stream);
+    rc = doc_ranges(p, at, &kr, &rr, stream);
     if (rc != LUTGEMM_OK) return rc;
-    float *part = reinterpret_cast<float *>(static_cast<uint8_t *>(scratch) + doc_range_bytes(p)), *part_lse = part + (size_t)splits * p.B * p.G * p.M * dp;
+    float *part = reinterpret_cast<float *>(at + doc_range_bytes(p)), *part_lse = part + (size_t)splits * p.B * p.G * p.M * dp;
     const bool bent = p.cap > 0.f || p.slopes || !(p.scale > 0.f);
 #define RUN(T, DP) (bent ? launch<T, DP, true>(p, map_k, map_v, kr, rr, out, rest, lse, part, part_lse, splits, error_word, stream) \
                          : launch<T, DP, false>(p, map_k, map_v, kr, rr, out, rest, lse, part, part_lse, splits, error_word, stream))
+    if (dtype == LUTGEMM_F32) return RUN(float, 64);
     if (dtype == LUTGEMM_BF16) return dp == 64 ? RUN(__nv_bfloat16, 64) : RUN(__nv_bfloat16, 128);
     return dp == 64 ? RUN(__half, 64) : RUN(__half, 128);
 #undef RUN

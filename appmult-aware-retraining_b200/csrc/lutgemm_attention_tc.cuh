@@ -21,6 +21,26 @@ struct IsBf16<__nv_bfloat16> {
     static constexpr bool value = true;
 };
 
+// How the tensor cores take operands of a type.  16-bit ones as they are; a tile's blocks are then blocks of 64 values of the head.  fp32
+// ones as three bf16 planes whose sum they are (8 bits each; attention_split writes them), heads of up to 64 values: the blocks
+// are the planes, and a product is the six products of planes that reach 2^-24 of it, the small ones first.
+template <typename T, int DP>
+struct Operand {
+    using Type = T;
+    static constexpr bool kPlanes = false, kBf16 = IsBf16<T>::value;
+    static constexpr int kBlocks = DP / 64, kProducts = DP / 64;
+    __host__ __device__ static constexpr int a(int i) { return i; }
+    __host__ __device__ static constexpr int b(int i) { return i; }
+};
+template <int DP>
+struct Operand<float, DP> {
+    using Type = __nv_bfloat16;
+    static constexpr bool kPlanes = true, kBf16 = true;
+    static constexpr int kBlocks = 3, kProducts = 6;
+    __host__ __device__ static constexpr int a(int i) { return i == 0 ? 2 : i == 2 || i == 3 ? 1 : 0; }
+    __host__ __device__ static constexpr int b(int i) { return i == 1 ? 2 : i == 2 || i == 4 ? 1 : 0; }
+};
+
 __device__ __forceinline__ float fast_exp2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -44,6 +64,21 @@ template <typename T>
 __device__ __forceinline__ float2 unpack_pair(uint32_t v) {
     if (IsBf16<T>::value) return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
     return __half22float2(*reinterpret_cast<const __half2 *>(&v));
+}
+
+// two values as words of the planes of their type (one of 16-bit types), for half a word row each
+template <typename T, int N>
+__device__ __forceinline__ void plane_words(uint32_t (&w)[N][16], int at, float a, float b) {
+    using O = typename Operand<T, 64>::Type;
+    w[0][at] = pack_pair<O>(a, b);
+    if constexpr (N == 3) {
+        float2 h = unpack_pair<O>(w[0][at]);
+        a -= h.x;
+        b -= h.y;
+        w[1][at] = pack_pair<O>(a, b);
+        h = unpack_pair<O>(w[1][at]);
+        w[2][at] = pack_pair<O>(a - h.x, b - h.y);
+    }
 }
 
 // documents of a tile of 64: the smallest and largest id that is not padding (0x7fffffff, -1: none), and whether any is
@@ -82,9 +117,10 @@ __device__ __forceinline__ void load_keys(uint32_t dst, const CUtensorMap *map, 
 #pragma unroll
     for (int k = 0; k < BLOCKS; ++k) tma_load_5d(dst + k * 64 * 128, map, 64 * k, 0, j0, g, b, bar);
 }
-// the 128 packed rows from m0 on of a query-side operand, by 128 threads; zeros beyond the end and for padding
+// the 128 packed rows of `width` values from m0 on of a query-side operand, by 128 threads; zeros beyond the end and for padding
 template <int BLOCKS>
-__device__ __forceinline__ void copy_row_tile(uint32_t dst, const AttnProblem &p, const AttnTensor &t, int b, int g, int m0, int thread) {
+__device__ __forceinline__ void copy_row_tile(uint32_t dst, const AttnProblem &p, const AttnTensor &t, int width, int b, int g, int m0,
+                                              int thread) {
     const char *base = static_cast<const char *>(t.p) + 2 * (b * t.sb + (long)g * p.R * t.sh);
     const int c = thread & 7;
 #pragma unroll 4
@@ -94,7 +130,7 @@ __device__ __forceinline__ void copy_row_tile(uint32_t dst, const AttnProblem &p
         const char *src = base + 2 * (i * t.st + (m - i * p.R) * t.sh) + 16 * c;
 #pragma unroll
         for (int k = 0; k < BLOCKS; ++k) {
-            const bool real = in && k * 64 + c * 8 < p.D;
+            const bool real = in && k * 64 + c * 8 < width;
             copy16(dst + k * kRowTile * 128 + r * 128 + ((c ^ (r & 7)) << 4), real ? src + 128 * k : t.p, real);
         }
     }
@@ -174,17 +210,48 @@ __device__ __forceinline__ TileRow tile_row(const AttnProblem &p, int b, int g, 
 struct Bend {
     float scale2;      // scale * log2 e
     float in, k1, k2;  // cap: k1 - k2 / (1 + 2^(in * s)) = log2 e * cap * tanh(scale * s / cap)
+
+    // a capped score, and the derivative of the cap.  16-bit operands: by 1 / (1 + 2^x), off by 2^-23 * cap, far below the operands' own
+    // roundings; fp32 ones by tanhf.
+    template <bool EXACT>
+    __device__ __forceinline__ float capped(float s, float *slope) const {
+        if (EXACT) {
+            const float t = tanhf(s * in);
+            *slope = 1.f - t * t;
+            return k1 * t;
+        }
+        const float q = fast_rcp(1.f + fast_exp2(s * in));
+        *slope = 4.f * q * (1.f - q);
+        return k1 - k2 * q;
+    }
 };
+template <bool EXACT>
 __device__ __forceinline__ Bend make_bend(const AttnProblem &p) {
     Bend b;
     b.scale2 = p.scale * kLog2e;
     b.k1 = p.cap * kLog2e;
     b.k2 = 2.f * b.k1;
-    b.in = p.cap > 0.f ? 2.f * b.scale2 / p.cap : 0.f;
+    b.in = p.cap > 0.f ? (EXACT ? p.scale : 2.f * b.scale2) / p.cap : 0.f;
     return b;
 }
 
 int *device_error_word();
+
+// lutgemm_attention_split.cu: fp32 operands [B, T, heads, D <= 64] as planes [B, T, heads, 3, 64] of bf16, rows of padding as zeros
+constexpr int kPlaneWidth = 3 * 64;
+struct SplitOperand {
+    AttnTensor from;
+    __nv_bfloat16 *to;
+    const int *doc;  // or null
+    long doc_sb;
+    int T, heads;
+};
+inline AttnTensor plane_tensor(const void *p, int T, int heads) {
+    return {p, (long)T * heads * kPlaneWidth, (long)heads * kPlaneWidth, kPlaneWidth};
+}
+inline size_t plane_bytes(int B, int T, int heads) { return 2 * (size_t)B * T * heads * kPlaneWidth; }
+// the last operand of four is grad_o, whose products with `out` go to delta
+int attention_split(const AttnProblem &p, const SplitOperand *operands, int count, const float *out, float *delta, cudaStream_t stream);
 
 // Tensor map of an operand whose heads come in groups of R: packed rows of a key head in boxes of 64 / R * R (a box of keys: R = 1)
 inline bool attention_map(CUtensorMap *map, bool bf16, const AttnTensor &t, int B, int T, int G, int R, int D) {

@@ -1,4 +1,4 @@
-// Attention backward on the tensor cores, 16-bit operands.
+// Attention backward on the tensor cores: 16-bit operands, and fp32 ones as three bf16 planes.
 //
 // With P the probabilities, recomputed from the scores and the forward pass's statistics, gP = grad_o v and delta = grad_o . out:
 //     dS = P (gP - delta) cap',   grad_v = P^T grad_o,   grad_k = scale dS^T q,   grad_q = scale dS k
@@ -68,20 +68,25 @@ __global__ void __launch_bounds__(256) attention_delta_kernel(const AttnProblem 
 //     S = X x^T, gP = Y y^T (tcgen05) -> a row to a thread: P, dS in registers -> P and dS in 16 bits to tensor memory, over S and gP ->
 //     KEYS: grad_v += P y;   grad_k or grad_q += dS x     (tcgen05, first operand from tensor memory; x and y, in shared memory as
 //     they were copied, serve as row and as column operands)
-// A further warp brings the tiles and issues the products.  Heads of up to 64 values leave room for two blocks on an SM; with
-// larger ones the accumulators fill the tensor memory of an SM, and the block has two groups of four warps that take rounds in
-// turn, each with its own S and gP.
+// Eight warps share a round, four with the first 32 columns and four with the others; a further warp brings the tiles and issues the
+// products.  Heads of up to 64 values leave room for two blocks on an SM; with larger ones the accumulators fill the tensor
+// memory of an SM, and the block has two groups of eight warps that take rounds in turn, each with its own S and gP.
 // fp16: P is kept 2^10 larger, and grad_o is taken in units of its largest value in this key head (a power of two), so that dS stays
 // out of fp16's subnormal range whatever the scale of the loss.
+// fp32: P and dS are split into planes as the operands were, and have tensor memory of their own; each round's sums start from zero and
+// are added up in registers while the next scores are formed (in the accumulators, what additions cut off came to 2e-5 of
+// the gradients of 4096 rows).  Its ring has one stage less, which is brought when the round's products are done.
 template <typename T, int DP, bool KEYS>
 struct GradLayout {
-    static constexpr int kBlocks = DP / 64, kGroups = DP / 64, kStages = kGroups + 2, kPerSm = DP == 64 ? 2 : 1;
-    static constexpr int kThreads = 128 * kGroups + 32;
-    static constexpr uint32_t kTile = 64 * DP * 2, kX = 0, kY = 2 * kTile, kRing = 4 * kTile;  // a stage of the ring: x, y
+    using Op = Operand<T, DP>;
+    static constexpr int kBlocks = Op::kBlocks, kGroups = DP / 64, kStages = kGroups + (Op::kPlanes ? 1 : 2), kPerSm = DP == 64 && !Op::kPlanes ? 2 : 1;
+    static constexpr int kWorkers = 256 * kGroups, kThreads = kWorkers + 32, kSums = KEYS ? 2 : 1;
+    static constexpr uint32_t kTile = 64 * kBlocks * 128, kX = 0, kY = 2 * kTile, kRing = 4 * kTile;  // a stage of the ring: x, y
     static constexpr uint32_t kCols = kRing + kStages * 2 * kTile;  // KEYS: for each stage -lse, -delta, documents, slopes and places of 64 rows
-    static constexpr uint32_t kBars = kCols + (KEYS ? kStages * 64 * 20 : 0), kBytes = kBars + 192;
-    static constexpr int kSums = KEYS ? 2 : 1;
-    static constexpr uint32_t kAcc = kGroups * 128, kColumns = kAcc + kSums * DP <= 256 ? 256 : 512;
+    static constexpr uint32_t kBars = kCols + (KEYS ? kStages * 64 * 20 : 0), kBytes = kBars + 256;
+    // tensor memory of a group: S, gP and, over them or behind them, P and dS; then the sums
+    static constexpr uint32_t kP = Op::kPlanes ? 128 : 0, kDS = Op::kPlanes ? 224 : 64, kGroup = Op::kPlanes ? 320 : 128;
+    static constexpr uint32_t kAcc = kGroups * kGroup, kColumns = kAcc + kSums * DP <= 256 ? 256 : 512;
 };
 
 template <typename T, int DP, bool BENT, bool KEYS>
@@ -91,7 +96,8 @@ __global__ void __launch_bounds__(GradLayout<T, DP, KEYS>::kThreads, GradLayout<
                              const float *lse, const float *delta, const float *most, int most_parts, T *g1, T *g2, int *error_word) {
     using L = GradLayout<T, DP, KEYS>;
     constexpr int G = L::kGroups;
-    constexpr bool kBf16 = IsBf16<T>::value;
+    using Op = typename L::Op;
+    constexpr bool kBf16 = Op::kBf16;
     constexpr float kShift = kBf16 ? 0.f : 10.f;
     extern __shared__ __align__(1024) uint8_t smem[];
     const uint32_t base = smem_u32(smem), bars = base + L::kBars;
@@ -109,12 +115,13 @@ __global__ void __launch_bounds__(GradLayout<T, DP, KEYS>::kThreads, GradLayout<
     const int o0 = (KEYS ? bid / p.B : own_tiles - 1 - bid / p.B) * 128;
     const int pre = p.prefix ? p.prefix[b] : 0, size = packed_tile(p.R);
     const bool docs = p.doc_k != nullptr;
+    const int width = Op::kPlanes ? kPlaneWidth : p.D;
     const long stat0 = ((long)b * p.G + g) * p.M;
     if (tid == 0) {
         *abort_word = 0;
         for (int i = 0; i < 2; ++i) {
             mbar_init(bar_s + 8 * i, 2);  // the products' arrival and the issuing lane's own, which orders what it wrote
-            mbar_init(bar_p + 8 * i, 128);
+            mbar_init(bar_p + 8 * i, 256);
         }
         mbar_init(bar_acc, 1);
         for (int i = 0; i < L::kStages; ++i) mbar_init(bar_full + 8 * i, 1);
@@ -129,13 +136,15 @@ __global__ void __launch_bounds__(GradLayout<T, DP, KEYS>::kThreads, GradLayout<
         for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
         if ((tid & 31) == 0) tops[warp] = top;
     }
-    if (warp == 4 * G) tmem_alloc(smem_u32(slot), L::kColumns);
+    if (warp == 8 * G) tmem_alloc(smem_u32(slot), L::kColumns);
     if (KEYS && size < 64) {  // rows of a tile that bulk copies never write
         for (int i = tid; i < (int)(L::kStages * 2 * L::kTile / 16); i += L::kThreads)
             *reinterpret_cast<uint4 *>(smem + L::kRing + 16 * i) = make_uint4(0, 0, 0, 0);
         writes_to_tensor_cores();
     }
-    if (warp < 4) {
+    if (warp < 8) {  // X by four warps, Y by four
+        const bool y = warp >= 4;
+        const uint32_t to = base + (y ? L::kY : L::kX);
         if (KEYS) {
             // (like rows of one head)
             AttnProblem keys = p;
@@ -143,11 +152,9 @@ __global__ void __launch_bounds__(GradLayout<T, DP, KEYS>::kThreads, GradLayout<
             keys.R = 1;
             keys.doc_q = p.doc_k;
             keys.doc_q_sb = p.doc_k_sb;
-            copy_row_tile<L::kBlocks>(base + L::kX, keys, p.k, b, g, o0, tid);
-            copy_row_tile<L::kBlocks>(base + L::kY, keys, p.v, b, g, o0, tid);
+            copy_row_tile<L::kBlocks>(to, keys, y ? p.v : p.k, width, b, g, o0, tid & 127);
         } else {
-            copy_row_tile<L::kBlocks>(base + L::kX, p, p.q, b, g, o0, tid);
-            copy_row_tile<L::kBlocks>(base + L::kY, p, go, b, g, o0, tid);
+            copy_row_tile<L::kBlocks>(to, p, y ? go : p.q, width, b, g, o0, tid & 127);
         }
         copies_end_group();
         copies_wait<0>();
@@ -159,13 +166,16 @@ __global__ void __launch_bounds__(GradLayout<T, DP, KEYS>::kThreads, GradLayout<
     if (!kBf16) {
         float top = 0.f;
 #pragma unroll
-        for (int w = 0; w < 4 * G + 1; ++w) top = fmaxf(top, tops[w]);
+        for (int w = 0; w < 8 * G + 1; ++w) top = fmaxf(top, tops[w]);
         // (an infinite or NaN gradient, or none at all: as it is)
         const int e = (int)(__float_as_uint(top) >> 23);
         if (e > 0 && e < 254) unit = __uint_as_float((uint32_t)(e + 1) << 23);
     }
 
-    if (warp == 4 * G) {
+    // of the workers: the round group, the half of a round's columns, the row
+    const int group = warp >> 3, h = warp >> 2 & 1, r = tid & 127;
+    f32x2 sums[Op::kPlanes ? 16 * L::kSums : 1] = {};  // fp32: the worker's half of its row's sums
+    if (warp == 8 * G) {
         const int lane = tid & 31;
         TileWalk walk;
         if (KEYS) {
@@ -228,7 +238,7 @@ __global__ void __launch_bounds__(GradLayout<T, DP, KEYS>::kThreads, GradLayout<
         auto arrived = [&](int i, int n) {
             if (queue[i] < 0) return;
             mbar_wait(bar_full + 8 * (n % L::kStages), n / L::kStages & 1, 211, abort_word, error_word);
-            if (!docs) return;
+            if (!docs || Op::kPlanes) return;  // (planes of padding are zeros)
             uint8_t *at = smem + L::kRing + n % L::kStages * 2 * L::kTile;
             if (KEYS) {
                 const int *ids = reinterpret_cast<const int *>(smem + L::kCols + n % L::kStages * 64 * 20) + 128;
@@ -252,15 +262,13 @@ __global__ void __launch_bounds__(GradLayout<T, DP, KEYS>::kThreads, GradLayout<
             const uint32_t bar = bar_s + 8 * (n % G);
             tiles[n & 7] = tile;
             if (tile >= 0) {
-                const uint32_t x = base + L::kRing + n % L::kStages * 2 * L::kTile, d = tmem + n % G * 128;
+                const uint32_t x = base + L::kRing + n % L::kStages * 2 * L::kTile, d = tmem + n % G * L::kGroup;
 #pragma unroll
-                for (int i = 0; i < DP / 16; ++i)
-                    mma_ss(d, smem_descriptor(base + L::kX + (i >> 2) * 128 * 128 + (i & 3) * 32, 0),
-                           smem_descriptor(x + (i >> 2) * 64 * 128 + (i & 3) * 32, 0), desc_s, i > 0);
+                for (int e = 0; e < 2; ++e)
 #pragma unroll
-                for (int i = 0; i < DP / 16; ++i)
-                    mma_ss(d + 64, smem_descriptor(base + L::kY + (i >> 2) * 128 * 128 + (i & 3) * 32, 0),
-                           smem_descriptor(x + L::kTile + (i >> 2) * 64 * 128 + (i & 3) * 32, 0), desc_s, i > 0);
+                    for (int i = 0; i < 4 * Op::kProducts; ++i)
+                        mma_ss(d + 64 * e, smem_descriptor(base + (e ? L::kY : L::kX) + Op::a(i >> 2) * 128 * 128 + (i & 3) * 32, 0),
+                               smem_descriptor(x + e * L::kTile + Op::b(i >> 2) * 64 * 128 + (i & 3) * 32, 0), desc_s, i > 0);
                 mma_commit(bar);
             } else {
                 mbar_arrive(bar);
@@ -270,7 +278,7 @@ __global__ void __launch_bounds__(GradLayout<T, DP, KEYS>::kThreads, GradLayout<
 #pragma unroll
         for (int i = 0; i < L::kStages; ++i) next(i);
 #pragma unroll
-        for (int i = 0; i < L::kStages - 1; ++i) bring(i, i);
+        for (int i = 0; i < L::kStages - (Op::kPlanes ? 0 : 1); ++i) bring(i, i);
         __syncwarp();
 #pragma unroll
         for (int i = 0; i < G; ++i) {
@@ -287,34 +295,46 @@ __global__ void __launch_bounds__(GradLayout<T, DP, KEYS>::kThreads, GradLayout<
             mbar_wait(bar_p + 8 * (n % G), n / G & 1, 212, abort_word, error_word);
             // the products of the round before are done, and with them its stage (before this round's commit: the barrier's parity
             // tells two phases apart, not three)
-            if (n > 0) mbar_wait(bar_acc, (n - 1) & 1, 213, abort_word, error_word);
+            if (!Op::kPlanes && n > 0) mbar_wait(bar_acc, (n - 1) & 1, 213, abort_word, error_word);
             tmem_after_sync();
             __syncwarp();
             if (lane == 0) {
-                const uint32_t x = base + L::kRing + n % L::kStages * 2 * L::kTile, d = tmem + n % G * 128;
-                if (KEYS)
+                const uint32_t x = base + L::kRing + n % L::kStages * 2 * L::kTile, d = tmem + n % G * L::kGroup;
 #pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        mma_ts(tmem + L::kAcc, d + 8 * i, smem_descriptor(x + L::kTile + i * 16 * 128, 64 * 128), desc_acc, n > 0 || i > 0);
+                for (int e = 0; e < L::kSums; ++e) {  // grad_v with KEYS, then grad_k or grad_q
+                    const bool first = KEYS && e == 0;
+                    const uint32_t from = d + (first ? L::kP : L::kDS), with = x + (first ? L::kTile : 0);
+                    if constexpr (Op::kPlanes) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    mma_ts(tmem + L::kAcc + (KEYS ? DP : 0), d + 64 + 8 * i, smem_descriptor(x + i * 16 * 128, 64 * 128), desc_acc,
-                           n > 0 || i > 0);
+                        for (int i = 0; i < 4 * Op::kProducts; ++i)
+                            mma_ts(tmem + L::kAcc + e * DP, from + 32 * Op::a(i >> 2) + 8 * (i & 3),
+                                   smem_descriptor(with + Op::b(i >> 2) * 64 * 128 + (i & 3) * 16 * 128, 0), desc_acc, i > 0);
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            mma_ts(tmem + L::kAcc + e * DP, from + 32 * (i >> 1) + 8 * (i & 1),
+                                   smem_descriptor(with + i * 16 * 128, 64 * 128), desc_acc, n > 0 || i > 0);
+                    }
+                }
                 mma_commit(bar_acc);
                 issue_scores(n + G, queue[G]);
             }
             __syncwarp();
-            bring(L::kStages - 1, n + L::kStages - 1);
+            if (Op::kPlanes) {
+                mbar_wait(bar_acc, n & 1, 214, abort_word, error_word);
+                bring(L::kStages, n + L::kStages);
+            } else {
+                bring(L::kStages - 1, n + L::kStages - 1);
+            }
             __syncwarp();
 #pragma unroll
             for (int i = 0; i < L::kStages; ++i) queue[i] = queue[i + 1];
         }
-        if (n > 0) mbar_wait(bar_acc, (n - 1) & 1, 214, abort_word, error_word);
+        if (!Op::kPlanes && n > 0) mbar_wait(bar_acc, (n - 1) & 1, 216, abort_word, error_word);
         if (lane == 0) tiles[8] = n;  // rounds done
     } else {
-        const int group = warp >> 2, r = tid & 127;
         const uint32_t mine = tmem + ((uint32_t)((warp & 3) * 32) << 16);
-        const Bend bend = make_bend(p);
+        const Bend bend = make_bend<Op::kPlanes>(p);
         const float per_unit = kBf16 ? 1.f : 1.f / (unit * 1024.f);
         TileRow row{-1, -1, 0, 0.f};
         float less = 0.f, less_delta = 0.f;  // of the row
@@ -335,11 +355,26 @@ __global__ void __launch_bounds__(GradLayout<T, DP, KEYS>::kThreads, GradLayout<
         }
         const bool idle = __all_sync(0xffffffffu, KEYS ? from == 0x7fffffff : row.limit < 0);
         for (int n = group;; n += G) {
+            if constexpr (Op::kPlanes) {
+                if (n > 0) {
+                    mbar_wait(bar_acc, (n - 1) & 1, 217, abort_word, error_word);
+                    tmem_after_sync();
+#pragma unroll
+                    for (int c = 0; c < L::kSums; ++c) {
+                        float v[32];
+                        tmem_load32(mine + L::kAcc + 32 * (L::kSums * h + c), v);
+                        tmem_loads_done();
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) sums[16 * c + j] = add2(sums[16 * c + j], pack2(v[2 * j], v[2 * j + 1]));
+                    }
+                    tmem_before_sync();
+                }
+            }
             mbar_wait(bar_s + 8 * group, n / G & 1, 215, abort_word, error_word);
             const int tile = tiles[n & 7];
             if (tile < 0 || *abort_word) break;
             tmem_after_sync();
-            const uint32_t at = mine + group * 128;
+            const uint32_t at = mine + group * L::kGroup;
             if (idle) {
                 mbar_arrive(bar_p + 8 * group);
                 continue;
@@ -348,8 +383,7 @@ __global__ void __launch_bounds__(GradLayout<T, DP, KEYS>::kThreads, GradLayout<
             const int t0 = (tile >> 1) * (KEYS ? size : 64);
             const bool masked = !(tile & 1);
             const f32x2 scale2 = pack2(bend.scale2, bend.scale2), unit2 = pack2(per_unit, per_unit);
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
+            {
                 float s[32], gp[32];
                 tmem_load32(at + 32 * h, s);
                 tmem_load32(at + 64 + 32 * h, gp);
@@ -383,7 +417,7 @@ __global__ void __launch_bounds__(GradLayout<T, DP, KEYS>::kThreads, GradLayout<
                         seen &= same;
                     }
                 }
-                uint32_t wp[KEYS ? 16 : 1], ws[16];
+                uint32_t wp[Op::kPlanes ? 3 : 1][16], ws[Op::kPlanes ? 3 : 1][16];
 #pragma unroll
                 for (int j = 0; j < 32; j += 2) {
                     f32x2 l2, d2;
@@ -401,9 +435,7 @@ __global__ void __launch_bounds__(GradLayout<T, DP, KEYS>::kThreads, GradLayout<
 #pragma unroll
                         for (int e = 0; e < 2; ++e) {
                             if (p.cap > 0.f) {
-                                const float q = fast_rcp(1.f + fast_exp2(y[e] * bend.in));
-                                y[e] = bend.k1 - bend.k2 * q;
-                                (e ? b2.y : b2.x) = 4.f * q * (1.f - q);
+                                y[e] = bend.capped<Op::kPlanes>(y[e], e ? &b2.y : &b2.x);
                             } else {
                                 y[e] *= bend.scale2;
                             }
@@ -432,11 +464,16 @@ __global__ void __launch_bounds__(GradLayout<T, DP, KEYS>::kThreads, GradLayout<
                         ds.x = sa ? ds.x : 0.f;
                         ds.y = sc ? ds.y : 0.f;
                     }
-                    if (KEYS) wp[KEYS ? j / 2 : 0] = pack_pair<T>(a, c);
-                    ws[j / 2] = pack_pair<T>(ds.x, ds.y);
+                    if (KEYS) plane_words<T>(wp, j / 2, a, c);
+                    plane_words<T>(ws, j / 2, ds.x, ds.y);
                 }
-                if constexpr (KEYS) tmem_store16(at + 16 * h, wp);
-                tmem_store16(at + 64 + 16 * h, ws);
+#pragma unroll
+                for (int e = 0; e < (Op::kPlanes ? 3 : 1); ++e) {
+                    // (16-bit: over what these warps alone have read)
+                    const uint32_t half = Op::kPlanes ? 32 * e + 16 * h : 32 * h;
+                    if constexpr (KEYS) tmem_store16(at + L::kP + half, wp[e]);
+                    tmem_store16(at + L::kDS + half, ws[e]);
+                }
             }
             tmem_stores_done();
             tmem_before_sync();
@@ -447,21 +484,32 @@ __global__ void __launch_bounds__(GradLayout<T, DP, KEYS>::kThreads, GradLayout<
     tmem_before_sync();
     __syncthreads();
     tmem_after_sync();
-    if (warp < 4 * G) {
-        const int rounds = tiles[8], group = warp >> 2, r = tid & 127, o = o0 + r;
+    if (warp < 8 * G) {
+        const int rounds = tiles[8], o = o0 + r;
         const bool in = o < (KEYS ? p.Tk : p.M);
         bool real = in && rounds > 0;
         if (in && docs) real = real && (KEYS ? p.doc_k[b * p.doc_k_sb + o] : p.doc_q[b * p.doc_q_sb + o / p.R]) >= 0;
         if (!KEYS && in && lse[stat0 + o] == INFINITY) real = false;  // a row that sees nothing
-        const int i = KEYS ? o : o / p.R, h = KEYS ? g : g * p.R + o - i * p.R;
-        const long to = (((long)b * (KEYS ? p.Tk : p.Tq) + i) * (KEYS ? p.G : p.H) + h) * p.D;
+        const int i = KEYS ? o : o / p.R, head = KEYS ? g : g * p.R + o - i * p.R;
+        const long to = (((long)b * (KEYS ? p.Tk : p.Tq) + i) * (KEYS ? p.G : p.H) + head) * p.D;
         const float f1 = kBf16 ? 1.f : 1.f / 1024.f, f2 = kBf16 ? p.scale : p.scale * unit;
+        constexpr int kChunks = L::kSums * DP / 32, kOwn = (kChunks + 2 * G - 1) / (2 * G);  // 32 columns each
 #pragma unroll
-        for (int c = 0; c < L::kSums * DP / 32; ++c) {
-            if (c % G != group) continue;
+        for (int k = 0; k < kOwn; ++k) {
+            const int c = kOwn * (2 * group + h) + k;
+            if (c >= kChunks) break;
             float v[32];
-            tmem_load32(tmem + ((uint32_t)((warp & 3) * 32) << 16) + L::kAcc + 32 * c, v);
-            tmem_loads_done();
+            if constexpr (Op::kPlanes) {
+#pragma unroll
+                for (int j = 0; j < 16; ++j) {
+                    const float2 t = unpack2(sums[16 * k + j]);
+                    v[2 * j] = t.x;
+                    v[2 * j + 1] = t.y;
+                }
+            } else {
+                tmem_load32(tmem + ((uint32_t)((warp & 3) * 32) << 16) + L::kAcc + 32 * c, v);
+                tmem_loads_done();
+            }
             const bool second = KEYS && c < DP / 32;  // grad_v
             const int d0 = (second || !KEYS ? c : c - DP / 32) * 32;
             T *dst = second ? g2 : g1;
@@ -470,18 +518,25 @@ __global__ void __launch_bounds__(GradLayout<T, DP, KEYS>::kThreads, GradLayout<
 #pragma unroll
                 for (int j = 0; j < 32; j += 8) {
                     if (d0 + j >= p.D) break;
-                    uint4 w;
-                    uint32_t *q = &w.x;
+                    if constexpr (Op::kPlanes) {
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) q[e] = real ? pack_pair<T>(v[j + 2 * e] * f, v[j + 2 * e + 1] * f) : 0u;
-                    *reinterpret_cast<uint4 *>(dst + to + d0 + j) = w;
+                        for (int e = 0; e < 8; e += 4)
+                            *reinterpret_cast<float4 *>(dst + to + d0 + j + e) =
+                                real ? make_float4(v[j + e] * f, v[j + e + 1] * f, v[j + e + 2] * f, v[j + e + 3] * f) : make_float4(0.f, 0.f, 0.f, 0.f);
+                    } else {
+                        uint4 w;
+                        uint32_t *q = &w.x;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) q[e] = real ? pack_pair<T>(v[j + 2 * e] * f, v[j + 2 * e + 1] * f) : 0u;
+                        *reinterpret_cast<uint4 *>(dst + to + d0 + j) = w;
+                    }
                 }
             __syncwarp();
         }
         tmem_before_sync();
     }
     __syncthreads();
-    if (warp == 4 * G) {
+    if (warp == 8 * G) {
         tmem_after_sync();
         tmem_free(tmem, L::kColumns);
     }
@@ -500,48 +555,70 @@ int launch(const AttnProblem &p, const AttnTensor &go, const CUtensorMap &map_x,
     return launch_status();
 }
 
+// the two kernels; delta and, for fp16, the largest gradients stand in scratch
 template <typename T, int DP>
-int backward(const AttnProblem &p, const AttnTensor &go, const void *out, const void *rest, const float *lse, float *delta, float *most,
-             const DocRange *kr, const DocRange *rr, void *gq, void *gk, void *gv, int *error_word, cudaStream_t stream) {
-    constexpr bool bf16 = IsBf16<T>::value;
+int gradients(const AttnProblem &p, const AttnTensor &go, const float *lse, const float *delta, const float *most, int parts, const DocRange *kr,
+              const DocRange *rr, void *gq, void *gk, void *gv, int *error_word, cudaStream_t stream) {
+    using Op = Operand<T, DP>;
+    const int width = Op::kPlanes ? kPlaneWidth : p.D;
     CUtensorMap map_q, map_go, map_k, map_v;
-    if (!attention_map(&map_q, bf16, p.q, p.B, p.Tq, p.G, p.R, p.D) || !attention_map(&map_go, bf16, go, p.B, p.Tq, p.G, p.R, p.D) ||
-        !attention_map(&map_k, bf16, p.k, p.B, p.Tk, p.G, 1, p.D) || !attention_map(&map_v, bf16, p.v, p.B, p.Tk, p.G, 1, p.D))
+    if (!attention_map(&map_q, Op::kBf16, p.q, p.B, p.Tq, p.G, p.R, width) || !attention_map(&map_go, Op::kBf16, go, p.B, p.Tq, p.G, p.R, width) ||
+        !attention_map(&map_k, Op::kBf16, p.k, p.B, p.Tk, p.G, 1, width) || !attention_map(&map_v, Op::kBf16, p.v, p.B, p.Tk, p.G, 1, width))
         return LUTGEMM_E_BADARG;
-    const int parts = (p.M + kDeltaRows - 1) / kDeltaRows;
-    attention_delta_kernel<T><<<dim3(parts, p.G, p.B), 256, 0, stream>>>(p, go, static_cast<const T *>(out), static_cast<const T *>(rest), delta,
-                                                                        bf16 ? nullptr : most);
-    int rc = launch_status();
-    if (rc != LUTGEMM_OK) return rc;
     const bool bent = p.cap > 0.f || p.slopes;
-    rc = bent ? launch<T, DP, true, true>(p, go, map_q, map_go, kr, rr, lse, delta, most, parts, gk, gv, error_word, stream)
-              : launch<T, DP, false, true>(p, go, map_q, map_go, kr, rr, lse, delta, most, parts, gk, gv, error_word, stream);
+    const int rc = bent ? launch<T, DP, true, true>(p, go, map_q, map_go, kr, rr, lse, delta, most, parts, gk, gv, error_word, stream)
+                        : launch<T, DP, false, true>(p, go, map_q, map_go, kr, rr, lse, delta, most, parts, gk, gv, error_word, stream);
     if (rc != LUTGEMM_OK) return rc;
     return bent ? launch<T, DP, true, false>(p, go, map_k, map_v, kr, rr, lse, delta, most, parts, gq, nullptr, error_word, stream)
                 : launch<T, DP, false, false>(p, go, map_k, map_v, kr, rr, lse, delta, most, parts, gq, nullptr, error_word, stream);
 }
 
-}  // namespace
-
-// delta, the largest gradients, ranges of documents
-size_t attention_tc_backward_scratch_bytes(const AttnProblem &p) {
-    const size_t parts = (p.M + kDeltaRows - 1) / kDeltaRows;
-    return doc_range_bytes(p) + sizeof(float) * p.B * p.G * (p.M + parts);
+template <typename T>
+int backward(const AttnProblem &p, const AttnTensor &go, const void *out, const void *rest, const float *lse, float *delta, float *most,
+             const DocRange *kr, const DocRange *rr, void *gq, void *gk, void *gv, int *error_word, cudaStream_t stream) {
+    const int parts = (p.M + kDeltaRows - 1) / kDeltaRows;
+    attention_delta_kernel<T><<<dim3(parts, p.G, p.B), 256, 0, stream>>>(p, go, static_cast<const T *>(out), static_cast<const T *>(rest), delta,
+                                                                        IsBf16<T>::value ? nullptr : most);
+    const int rc = launch_status();
+    if (rc != LUTGEMM_OK) return rc;
+    return p.D <= 64 ? gradients<T, 64>(p, go, lse, delta, most, parts, kr, rr, gq, gk, gv, error_word, stream)
+                     : gradients<T, 128>(p, go, lse, delta, most, parts, kr, rr, gq, gk, gv, error_word, stream);
 }
 
-int attention_tc_backward(const AttnProblem &p, int dtype, const AttnTensor &go, const void *out, const void *rest, const float *lse, void *gq,
-                          void *gk, void *gv, void *scratch, cudaStream_t stream) {
+}  // namespace
+
+// fp32: the planes of q, grad_o, k and v; ranges of documents, delta, fp16's largest gradients
+size_t attention_tc_backward_scratch_bytes(const AttnProblem &p, int dtype) {
+    const size_t parts = (p.M + kDeltaRows - 1) / kDeltaRows;
+    return (dtype == LUTGEMM_F32 ? 2 * plane_bytes(p.B, p.Tq, p.H) + 2 * plane_bytes(p.B, p.Tk, p.G) : 0) + doc_range_bytes(p) +
+           sizeof(float) * p.B * p.G * (p.M + parts);
+}
+
+int attention_tc_backward(const AttnProblem &problem, int dtype, const AttnTensor &grad, const void *out, const void *rest, const float *lse,
+                          void *gq, void *gk, void *gv, void *scratch, cudaStream_t stream) {
+    AttnProblem p = problem;
     int *error_word = device_error_word();
     if (!error_word) return LUTGEMM_E_CUDA;
+    uint8_t *at = static_cast<uint8_t *>(scratch);
+    const size_t nq = plane_bytes(p.B, p.Tq, p.H), nk = plane_bytes(p.B, p.Tk, p.G);
+    if (dtype == LUTGEMM_F32) at += 2 * nq + 2 * nk;
     const DocRange *kr, *rr;
-    const int rc = doc_ranges(p, scratch, &kr, &rr, stream);
+    int rc = doc_ranges(p, at, &kr, &rr, stream);
     if (rc != LUTGEMM_OK) return rc;
-    float *delta = reinterpret_cast<float *>(static_cast<uint8_t *>(scratch) + doc_range_bytes(p)), *most = delta + (size_t)p.B * p.G * p.M;
-    if (dtype == LUTGEMM_BF16)
-        return p.D <= 64 ? backward<__nv_bfloat16, 64>(p, go, out, rest, lse, delta, most, kr, rr, gq, gk, gv, error_word, stream)
-                         : backward<__nv_bfloat16, 128>(p, go, out, rest, lse, delta, most, kr, rr, gq, gk, gv, error_word, stream);
-    return p.D <= 64 ? backward<__half, 64>(p, go, out, rest, lse, delta, most, kr, rr, gq, gk, gv, error_word, stream)
-                     : backward<__half, 128>(p, go, out, rest, lse, delta, most, kr, rr, gq, gk, gv, error_word, stream);
+    float *delta = reinterpret_cast<float *>(at + doc_range_bytes(p)), *most = delta + (size_t)p.B * p.G * p.M;
+    if (dtype == LUTGEMM_BF16) return backward<__nv_bfloat16>(p, grad, out, rest, lse, delta, most, kr, rr, gq, gk, gv, error_word, stream);
+    if (dtype == LUTGEMM_F16) return backward<__half>(p, grad, out, rest, lse, delta, most, kr, rr, gq, gk, gv, error_word, stream);
+    __nv_bfloat16 *planes = static_cast<__nv_bfloat16 *>(scratch);
+    const SplitOperand ops[4] = {{p.q, planes, p.doc_q, p.doc_q_sb, p.Tq, p.H},
+                                 {p.k, planes + nq / 2, p.doc_k, p.doc_k_sb, p.Tk, p.G},
+                                 {p.v, planes + (nq + nk) / 2, p.doc_k, p.doc_k_sb, p.Tk, p.G},
+                                 {grad, planes + nq / 2 + nk, p.doc_q, p.doc_q_sb, p.Tq, p.H}};
+    rc = attention_split(p, ops, 4, static_cast<const float *>(out), delta, stream);
+    if (rc != LUTGEMM_OK) return rc;
+    p.q = plane_tensor(ops[0].to, p.Tq, p.H);
+    p.k = plane_tensor(ops[1].to, p.Tk, p.G);
+    p.v = plane_tensor(ops[2].to, p.Tk, p.G);
+    return gradients<float, 64>(p, plane_tensor(ops[3].to, p.Tq, p.H), lse, delta, most, 0, kr, rr, gq, gk, gv, error_word, stream);
 }
 
 }  // namespace lutgemm

@@ -285,16 +285,17 @@ int backward_gw(const float *gc, const uint8_t *a, const uint8_t *w, float *gw, 
 struct AttnProblem;  // lutgemm_attention.cuh
 struct AttnTensor;
 
-// lutgemm_attention_tc.cu: 16-bit operands; rest (null or as out): what the rounding of out leaves
-size_t attention_tc_scratch_bytes(const AttnProblem &p, int num_sms);
+// lutgemm_attention_tc.cu: 16-bit operands, and fp32 heads of up to 64 values; rest (16-bit types, null or as out): what the rounding
+// of out leaves
+size_t attention_tc_scratch_bytes(const AttnProblem &p, int dtype, int num_sms);
 int attention_tc_forward(const AttnProblem &p, int dtype, void *out, void *rest, float *lse, void *scratch, int num_sms, cudaStream_t stream);
 
 // lutgemm_attention_tc_grad.cu
-size_t attention_tc_backward_scratch_bytes(const AttnProblem &p);
+size_t attention_tc_backward_scratch_bytes(const AttnProblem &p, int dtype);
 int attention_tc_backward(const AttnProblem &p, int dtype, const AttnTensor &go, const void *out, const void *rest, const float *lse, void *gq,
                           void *gk, void *gv, void *scratch, cudaStream_t stream);
 
-// lutgemm_attention_f32.cu
+// lutgemm_attention_f32.cu: fp32 heads of more than 64 values
 int attention_f32_forward(const AttnProblem &p, float *out, float *lse, cudaStream_t stream);
 int attention_f32_backward(const AttnProblem &p, const AttnTensor &go, const float *out, const float *lse, float *delta, float *gq, float *gk,
                            float *gv, cudaStream_t stream);

@@ -190,7 +190,7 @@ class _Attention(torch.autograd.Function):
         rest = torch.empty_like(out) if q.dtype is not torch.float32 and any(ctx.needs_input_grad[:3]) else None
         lib, dtype = approx_ops.library(), _DTYPES[q.dtype]
         with approx_ops._guard(q.device):
-            nbytes = lib.lutgemm_attention_scratch_bytes(dtype, B, Tq, Tk, H, G, D, doc_k is not None) if dtype else 0
+            nbytes = lib.lutgemm_attention_scratch_bytes(dtype, B, Tq, Tk, H, G, D, doc_k is not None)
             scratch = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
             rc = lib.lutgemm_attention(*_at(q), *_at(k), *_at(v), out.data_ptr(),
                                        rest.data_ptr() if rest is not None else None, lse.data_ptr(), dtype, B, Tq, Tk, H, G, D, *masks,
