@@ -108,11 +108,12 @@ __global__ void __launch_bounds__(kThreads, Layout<T, DP>::kPerSm)
             const uint32_t bar = bar_s + 8 * (n % L::kStages);
             tiles[n & 3] = tile;
             if (tile >= 0) {
-                const uint32_t k = base + L::kK + (n % L::kKStages) * L::kTile, d = tmem + (n % L::kStages) * L::kS;
+                const uint32_t d = tmem + (n % L::kStages) * L::kS;
+                const uint64_t q = smem_descriptor(base + L::kQ, 0), k = smem_descriptor(base + L::kK + (n % L::kKStages) * L::kTile, 0);
 #pragma unroll
                 for (int i = 0; i < 4 * Op::kProducts; ++i)
-                    mma_ss(d, smem_descriptor(base + L::kQ + Op::a(i >> 2) * kRowTile * 128 + (i & 3) * 32, 0),
-                           smem_descriptor(k + Op::b(i >> 2) * kKeyTile * 128 + (i & 3) * 32, 0), desc_s, i > 0);
+                    mma_ss(d, descriptor_at(q, Op::a(i >> 2) * kRowTile * 128 + (i & 3) * 32),
+                           descriptor_at(k, Op::b(i >> 2) * kKeyTile * 128 + (i & 3) * 32), desc_s, i > 0);
                 mma_commit(bar);
             } else {
                 mbar_arrive(bar);
@@ -141,16 +142,17 @@ __global__ void __launch_bounds__(kThreads, Layout<T, DP>::kPerSm)
             tmem_after_sync();
             __syncwarp();
             if ((tid & 31) == 0) {
-                const uint32_t v = base + L::kV + (n & 1) * L::kTile, a = tmem + (n % L::kStages) * L::kS;
+                const uint64_t v = smem_descriptor(base + L::kV + (n & 1) * L::kTile, Op::kPlanes ? 0 : kKeyTile * 128);
+                const uint32_t a = tmem + (n % L::kStages) * L::kS;
                 if constexpr (Op::kPlanes) {
 #pragma unroll
                     for (int i = 0; i < 4 * Op::kProducts; ++i)
                         mma_ts(tmem + L::kO, a + 32 * Op::a(i >> 2) + 8 * (i & 3),
-                               smem_descriptor(v + Op::b(i >> 2) * kKeyTile * 128 + (i & 3) * 16 * 128, 0), desc_o, i > 0);
+                               descriptor_at(v, Op::b(i >> 2) * kKeyTile * 128 + (i & 3) * 16 * 128), desc_o, i > 0);
                 } else {
 #pragma unroll
                     for (int i = 0; i < kKeyTile / 16; ++i)
-                        mma_ts(tmem + L::kO, a + 8 * i, smem_descriptor(v + i * 16 * 128, kKeyTile * 128), desc_o, n > 0 || i > 0);
+                        mma_ts(tmem + L::kO, a + 8 * i, descriptor_at(v, i * 16 * 128), desc_o, n > 0 || i > 0);
                 }
                 mma_commit(bar_o);
                 if (queue[L::kStages - 1] >= 0) issue_scores(n + L::kStages, queue[L::kStages]);

@@ -204,6 +204,27 @@ __global__ void __launch_bounds__(GradLayout<T, DP, KEYS>::kThreads, GradLayout<
             const bool more = i == 0 || queue[i - 1] >= 0;
             queue[i] = more ? walk.next(docs) : -1;
         };
+        // KEYS: what a round needs of its rows, two to a lane; asked for ahead of `bring`, which hands it on
+        float row_stat[2], row_delta[2], row_slope[2], row_place[2];
+        int row_doc[2];
+        auto ask = [&](int i) {
+            if (!KEYS || queue[i] < 0) return;
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                const int c = lane + 32 * k, m = (queue[i] >> 1) * size + c;
+                const bool in = c < size && m < p.M;
+                row_stat[k] = in ? lse[stat0 + m] : INFINITY;
+                row_delta[k] = in ? delta[stat0 + m] : 0.f;
+                if (docs || (BENT && p.slopes)) {
+                    const int t = in ? m / p.R : 0;
+                    if (docs) row_doc[k] = in ? p.doc_q[b * p.doc_q_sb + t] : -1;
+                    if (BENT && p.slopes) {
+                        row_slope[k] = in ? p.slopes[g * p.R + m - t * p.R] * kLog2e : 0.f;
+                        row_place[k] = (float)(t + p.shift);
+                    }
+                }
+            }
+        };
         auto bring = [&](int i, int n) {  // queue[i], which is round n's
             if (queue[i] < 0) return;
             const int t = queue[i] >> 1, stage = n % L::kStages;
@@ -212,15 +233,13 @@ __global__ void __launch_bounds__(GradLayout<T, DP, KEYS>::kThreads, GradLayout<
                 float *cols = reinterpret_cast<float *>(smem + L::kCols + stage * 64 * 20);
 #pragma unroll
                 for (int k = 0; k < 2; ++k) {
-                    const int c = lane + 32 * k, m = t * size + c;
-                    const bool in = c < size && m < p.M;
-                    cols[c] = in ? kShift - lse[stat0 + m] : -INFINITY;
-                    cols[64 + c] = in ? -delta[stat0 + m] : 0.f;
-                    const int i = in ? m / p.R : 0;
-                    if (docs) reinterpret_cast<int *>(cols)[128 + c] = in ? p.doc_q[b * p.doc_q_sb + i] : -1;
+                    const int c = lane + 32 * k;
+                    cols[c] = kShift - row_stat[k];
+                    cols[64 + c] = -row_delta[k];
+                    if (docs) reinterpret_cast<int *>(cols)[128 + c] = row_doc[k];
                     if (BENT && p.slopes) {
-                        cols[192 + c] = in ? p.slopes[g * p.R + m - i * p.R] * kLog2e : 0.f;
-                        cols[256 + c] = (float)(i + p.shift);
+                        cols[192 + c] = row_slope[k];
+                        cols[256 + c] = row_place[k];
                     }
                 }
             }
@@ -262,13 +281,14 @@ __global__ void __launch_bounds__(GradLayout<T, DP, KEYS>::kThreads, GradLayout<
             const uint32_t bar = bar_s + 8 * (n % G);
             tiles[n & 7] = tile;
             if (tile >= 0) {
-                const uint32_t x = base + L::kRing + n % L::kStages * 2 * L::kTile, d = tmem + n % G * L::kGroup;
+                const uint32_t d = tmem + n % G * L::kGroup;
+                const uint64_t own = smem_descriptor(base + L::kX, 0), x = smem_descriptor(base + L::kRing + n % L::kStages * 2 * L::kTile, 0);
 #pragma unroll
                 for (int e = 0; e < 2; ++e)
 #pragma unroll
                     for (int i = 0; i < 4 * Op::kProducts; ++i)
-                        mma_ss(d + 64 * e, smem_descriptor(base + (e ? L::kY : L::kX) + Op::a(i >> 2) * 128 * 128 + (i & 3) * 32, 0),
-                               smem_descriptor(x + e * L::kTile + Op::b(i >> 2) * 64 * 128 + (i & 3) * 32, 0), desc_s, i > 0);
+                        mma_ss(d + 64 * e, descriptor_at(own, (e ? L::kY : L::kX) + Op::a(i >> 2) * 128 * 128 + (i & 3) * 32),
+                               descriptor_at(x, e * L::kTile + Op::b(i >> 2) * 64 * 128 + (i & 3) * 32), desc_s, i > 0);
                 mma_commit(bar);
             } else {
                 mbar_arrive(bar);
@@ -278,7 +298,10 @@ __global__ void __launch_bounds__(GradLayout<T, DP, KEYS>::kThreads, GradLayout<
 #pragma unroll
         for (int i = 0; i < L::kStages; ++i) next(i);
 #pragma unroll
-        for (int i = 0; i < L::kStages - (Op::kPlanes ? 0 : 1); ++i) bring(i, i);
+        for (int i = 0; i < L::kStages - (Op::kPlanes ? 0 : 1); ++i) {
+            ask(i);
+            bring(i, i);
+        }
         __syncwarp();
 #pragma unroll
         for (int i = 0; i < G; ++i) {
@@ -291,6 +314,7 @@ __global__ void __launch_bounds__(GradLayout<T, DP, KEYS>::kThreads, GradLayout<
         int n = 0;
         for (; queue[0] >= 0; ++n) {
             next(L::kStages);
+            ask(L::kStages - (Op::kPlanes ? 0 : 1));
             arrived(G, n + G);
             mbar_wait(bar_p + 8 * (n % G), n / G & 1, 212, abort_word, error_word);
             // the products of the round before are done, and with them its stage (before this round's commit: the barrier's parity
@@ -299,21 +323,23 @@ __global__ void __launch_bounds__(GradLayout<T, DP, KEYS>::kThreads, GradLayout<
             tmem_after_sync();
             __syncwarp();
             if (lane == 0) {
-                const uint32_t x = base + L::kRing + n % L::kStages * 2 * L::kTile, d = tmem + n % G * L::kGroup;
+                const uint32_t d = tmem + n % G * L::kGroup;
+                const uint64_t x = smem_descriptor(base + L::kRing + n % L::kStages * 2 * L::kTile, Op::kPlanes ? 0 : 64 * 128);
 #pragma unroll
                 for (int e = 0; e < L::kSums; ++e) {  // grad_v with KEYS, then grad_k or grad_q
                     const bool first = KEYS && e == 0;
-                    const uint32_t from = d + (first ? L::kP : L::kDS), with = x + (first ? L::kTile : 0);
+                    const uint32_t from = d + (first ? L::kP : L::kDS);
+                    const uint64_t with = descriptor_at(x, first ? L::kTile : 0);
                     if constexpr (Op::kPlanes) {
 #pragma unroll
                         for (int i = 0; i < 4 * Op::kProducts; ++i)
                             mma_ts(tmem + L::kAcc + e * DP, from + 32 * Op::a(i >> 2) + 8 * (i & 3),
-                                   smem_descriptor(with + Op::b(i >> 2) * 64 * 128 + (i & 3) * 16 * 128, 0), desc_acc, i > 0);
+                                   descriptor_at(with, Op::b(i >> 2) * 64 * 128 + (i & 3) * 16 * 128), desc_acc, i > 0);
                     } else {
 #pragma unroll
                         for (int i = 0; i < 4; ++i)
                             mma_ts(tmem + L::kAcc + e * DP, from + 32 * (i >> 1) + 8 * (i & 1),
-                                   smem_descriptor(with + i * 16 * 128, 64 * 128), desc_acc, n > 0 || i > 0);
+                                   descriptor_at(with, i * 16 * 128), desc_acc, n > 0 || i > 0);
                     }
                 }
                 mma_commit(bar_acc);

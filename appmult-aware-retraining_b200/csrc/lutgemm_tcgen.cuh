@@ -65,6 +65,9 @@ __device__ __forceinline__ void tmem_store16(uint32_t addr, const uint32_t (&r)[
 __device__ __forceinline__ uint64_t smem_descriptor(uint32_t addr, uint32_t block) {
     return (uint64_t)((addr & 0x3ffffu) >> 4) | (uint64_t)(block >> 4) << 16 | (uint64_t)(1024u >> 4) << 32 | 1ull << 46 | 2ull << 61;
 }
+// the descriptor of the operand `bytes` further on (a product's operands lie at fixed distances from the first: one thread issues them all, and
+// building every descriptor anew would take longer than the products)
+__device__ __forceinline__ uint64_t descriptor_at(uint64_t descriptor, uint32_t bytes) { return descriptor + (bytes >> 4); }
 // 128 x N products of two operands of one 16-bit type into fp32; `b_mn`: the second operand is MN-major
 constexpr uint32_t mma_descriptor(bool bf16, int N, bool b_mn) {
     return 1u << 4 | (bf16 ? 1u << 7 | 1u << 10 : 0u) | (b_mn ? 1u << 16 : 0u) | (uint32_t)(N >> 3) << 17 | (128u >> 4) << 24;
