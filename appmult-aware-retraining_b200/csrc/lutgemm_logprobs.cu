@@ -5,54 +5,44 @@
 //     s = sum_j exp(-d_j),  u = sum_j exp(-d_j) d_j     (one occurrence of m left out of s; it adds nothing to u)
 //     log p_j = -d_j - L,  L = log1p(s);   entropy = L + U,  U = u / (1 + s);   log p_j + entropy = U - d_j
 // No difference of near values occurs, so a row in which one class has nearly all of the probability keeps its entropy and its
-// gradient, which are what is left beside it (with the sum over all classes both are lost from 1 - p = 2^-24 on).
+// gradient, which are what is left beside it (with the sum over all classes both are lost from 1 - p = 2^-24 on).  The pass itself
+// sums over all classes; where 1 + s comes out below 2, the one thread that has m sums those around it again without it.
 //     grad_j = g_logp (1[j is given] - p_j) - g_entropy p_j (log p_j + entropy);   1 - p = -expm1(log p) for the given class
 //
 // DRAM bounds both directions: logits once in, in the backward pass once more, and the gradient once out.  A block has a row, or
-// a part of one where there are few rows; every thread keeps (m, s, u) of its own values, and the block joins them.
-// The most probable classes come from the same pass at next to no cost: the k-th largest of the thread groups' largest logits is a
-// bound that at least k values reach, so only threads whose own largest value reaches it look at their values once more (a
-// few dozen of them, from the cache), and the candidates are ranked by counting.  Ties go to the lower class.  Rows with so many
+// a part of one where there are few rows; every thread keeps (m, 1 + s, u) of its own values, four vectors at a time, so that the
+// maximum is looked at once for 32 values of 16 bits, and the block joins them.  It also keeps which four vectors hold its
+// largest value and how large the others get: a second look at values (below, and above) is then one more load, not a pass.
+// The most probable classes come from the same pass at little cost: the k-th largest of the thread groups' largest logits is a
+// bound that at least k values reach, so only threads whose own largest value reaches it look at their values once more, and the
+// candidates are ranked by counting.  Ties go to the lower class.  Rows with so many
 // ties that the candidates do not fit are gone through once per answer instead.
 #include "lutgemm.h"
 #include "lutgemm_attention.cuh"
+#include "lutgemm_f32x2.cuh"
 #include "lutgemm_kernels.h"
 
 namespace lutgemm {
 
 namespace {
 
-constexpr int kMaxTop = 32, kCandidates = 512;
+constexpr int kMaxTop = 32, kMaxParts = 64, kCandidates = 512;
 
 // running sums of a set of logits; the empty set has m = -inf, s = -1
 struct RowState {
     float m, s, u;
 };
-__device__ __forceinline__ RowState empty_state() { return {-INFINITY, -1.f, 0.f}; }
+__device__ __forceinline__ float exp2_approx(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
 __device__ __forceinline__ RowState join(const RowState &a, const RowState &b) {
     const RowState &x = a.m >= b.m ? a : b, &y = a.m >= b.m ? b : a;
     if (y.m == -INFINITY) return {x.m, x.s + (y.s == -1.f ? 0.f : y.s), x.u};  // (a NaN in y.s stays)
     const float d = x.m - y.m, e = __expf(-d), n = 1.f + y.s;
     return {x.m, x.s + e * n, x.u + e * (y.u + d * n)};
 }
-// one more logit; -inf adds nothing, NaN makes s NaN
-__device__ __forceinline__ void add(RowState &a, float x) {
-    if (x > a.m) {
-        const float d = x - a.m, e = __expf(-d), n = 1.f + a.s;
-        if (a.m == -INFINITY) {
-            a.s = a.s == -1.f ? 0.f : a.s;
-        } else {
-            a.u = e * (a.u + d * n);
-            a.s = e * n;
-        }
-        a.m = x;
-    } else if (x != -INFINITY) {
-        const float d = a.m - x, e = __expf(-d);
-        a.s += e;
-        a.u += e * d;
-    }
-}
-
 // order of values by whole numbers: NaN above +inf, -0 as 0 (no key is all ones: that is where the search for ties begins)
 constexpr uint32_t kNanOrder = 0xfffffffeu;
 __device__ __forceinline__ uint32_t order_of(float x) {
@@ -94,36 +84,117 @@ struct Wide {
         const unsigned short hs = (unsigned short)h;
         return to_f32<T>(*reinterpret_cast<const T *>(&hs));
     }
+    __device__ __forceinline__ f32x2 pair(int i) const { return pack2(get(2 * i), get(2 * i + 1)); }
 };
 
-// the values of [first, end) of a row in this thread's order: a scalar head up to the first 16-byte boundary, vectors, a scalar tail
-template <typename T, int THREADS, typename One, typename Many>
-__device__ __forceinline__ void walk(const T *x, int first, int end, One one, Many many) {
-    constexpr int n = Wide<T>::n;
-    const uintptr_t a = reinterpret_cast<uintptr_t>(x + first);
-    const int head = min(end - first, (int)(((16 - (a & 15)) & 15) / sizeof(T)));
-    const int vecs = (end - first - head) / n, tail = first + head + vecs * n;
-    if ((int)threadIdx.x < head) one(first + threadIdx.x, to_f32<T>(x[first + threadIdx.x]));
-    const uint4 *v = reinterpret_cast<const uint4 *>(x + first + head);
-    int i = threadIdx.x;
-    for (; i + 3 * THREADS < vecs; i += 4 * THREADS) {
+// How THREADS threads share the values of [first, end) of a row: up to the first 16-byte boundary and behind the last one a value each (round
+// -1), in between four vectors to a thread and round.
+template <typename T, int THREADS>
+struct Share {
+    static constexpr int n = Wide<T>::n;
+    const T *x;
+    int first, end, head, vecs;
+
+    __device__ __forceinline__ Share(const T *row, int from, int to) : x(row), first(from), end(to) {
+        const uintptr_t a = reinterpret_cast<uintptr_t>(x + first);
+        head = min(end - first, (int)(((16 - (a & 15)) & 15) / sizeof(T)));
+        vecs = (end - first - head) / n;
+    }
+    __device__ __forceinline__ int tail() const { return first + head + vecs * n; }
+    __device__ __forceinline__ int rounds() const { return max(0, (vecs - (int)threadIdx.x + 4 * THREADS - 1) / (4 * THREADS)); }
+    // one(place, value) for this thread's values outside the vectors
+    template <typename One>
+    __device__ __forceinline__ void ends(One one) const {
+        if ((int)threadIdx.x < head) one(first + threadIdx.x, to_f32<T>(x[first + threadIdx.x]));
+        if (tail() + (int)threadIdx.x < end) one(tail() + threadIdx.x, to_f32<T>(x[tail() + threadIdx.x]));
+    }
+    // the vectors of a round; how many there are
+    __device__ __forceinline__ int load(Wide<T> (&w)[4], int round) const {
+        const uint4 *v = reinterpret_cast<const uint4 *>(x + first + head);
+        const int i = threadIdx.x + round * 4 * THREADS;
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            if (i + k * THREADS < vecs) w[k].raw = v[i + k * THREADS];
+        return min(4, (vecs - i + THREADS - 1) / THREADS);
+    }
+    // one(place, value) for the values of a round
+    template <typename One>
+    __device__ __forceinline__ void round(int r, One one) const {
+        if (r < 0) {
+            ends(one);
+            return;
+        }
         Wide<T> w[4];
+        const int have = load(w, r);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) w[k].raw = v[i + k * THREADS];
+        for (int k = 0; k < 4; ++k)
+            if (k < have)
 #pragma unroll
-        for (int k = 0; k < 4; ++k) many(first + head + (i + k * THREADS) * n, w[k]);
+                for (int i = 0; i < n; ++i) one(first + head + (threadIdx.x + (r * 4 + k) * THREADS) * n + i, w[k].get(i));
     }
-    for (; i < vecs; i += THREADS) {
-        Wide<T> w;
-        w.raw = v[i];
-        many(first + head + i * n, w);
+    template <typename One>
+    __device__ __forceinline__ void every(One one) const {
+        for (int r = -1; r < rounds(); ++r) round(r, one);
     }
-    if (tail + (int)threadIdx.x < end) one(tail + threadIdx.x, to_f32<T>(x[tail + threadIdx.x]));
-}
+};
+
+// sums over this thread's values: 1 + s instead of s, in two parts; the round with the largest value, and the largest of the other rounds
+struct ThreadState {
+    float m = -INFINITY, second = -INFINITY;
+    float best = 0.f, rest = 0.f, u = 0.f;  // sums of the round with m, of the others
+    int at = -1;
+
+    // a round whose largest value is `top` begins: whether it holds m now
+    __device__ __forceinline__ bool raise(float top, int round) {
+        if (!(top > m)) {
+            second = fmaxf(second, top);
+            return false;
+        }
+        const float d = top - m, e = __expf(-d);  // (0 from -inf)
+        rest += best;
+        u = m == -INFINITY ? u : e * (u + d * rest);
+        rest *= e;
+        best = 0.f;
+        second = m;
+        m = top;
+        at = round;
+        return true;
+    }
+    __device__ __forceinline__ float base() const { return m == -INFINITY ? 0.f : m; }
+    __device__ __forceinline__ float all() const { return rest + best; }
+};
 
 template <int THREADS>
 __device__ __forceinline__ void block_sync() {
     if (THREADS == 32) __syncwarp(); else __syncthreads();
+}
+
+// the states of a block's threads joined, for all of them
+template <int THREADS>
+__device__ __forceinline__ RowState join_block(RowState all, RowState *shared) {
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+        const RowState other{__shfl_xor_sync(0xffffffffu, all.m, d), __shfl_xor_sync(0xffffffffu, all.s, d), __shfl_xor_sync(0xffffffffu, all.u, d)};
+        // (both lanes join in the same order, so that they agree)
+        all = threadIdx.x & d ? join(other, all) : join(all, other);
+    }
+    if (THREADS == 32) return all;
+    if (threadIdx.x % 32 == 0) shared[threadIdx.x / 32] = all;
+    __syncthreads();
+    all = shared[0];
+    for (int w = 1; w < THREADS / 32; ++w) all = join(all, shared[w]);
+    return all;
+}
+template <int THREADS>
+__device__ __forceinline__ float sum_block(float v, float *shared) {
+#pragma unroll
+    for (int d = 16; d; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
+    if (THREADS == 32) return v;
+    if (threadIdx.x % 32 == 0) shared[threadIdx.x / 32] = v;
+    __syncthreads();
+    v = 0.f;
+    for (int w = 0; w < THREADS / 32; ++w) v += shared[w];
+    return v;
 }
 
 // the `top` largest of the candidates in order, by counting; every thread of the block
@@ -163,32 +234,68 @@ __global__ void __launch_bounds__(THREADS) token_logprobs_kernel(const LogpArgs 
     const long row = blockIdx.x;
     const int part = blockIdx.y, first = part * p.part_len, end = min(p.C, first + p.part_len);
     const T *x = static_cast<const T *>(p.x) + row * p.pitch;
-    RowState st = empty_state();
-    walk<T, THREADS>(x, first, end, [&](int, float v) { add(st, v); },
-                     [&](int, const Wide<T> &w) {
-                         float v[Wide<T>::n], top = -INFINITY;
+    const Share<T, THREADS> share(x, first, end);
+    ThreadState st;
+    {
+        float top = -INFINITY, sum = 0.f;
+        share.ends([&](int, float v) { top = fmaxf(top, v); });
+        const bool best = st.raise(top, -1);
+        share.ends([&](int, float v) {
+            const float t = v - st.base(), e = __expf(t);
+            sum += e;
+            st.u += e * fminf(-t, 1e30f);  // (-inf: exp gives 0, and 0 * inf must not reach u; a NaN reaches both sums through e)
+        });
+        (best ? st.best : st.rest) += sum;
+    }
+    for (int r = 0, rounds = share.rounds(); r < rounds; ++r) {
+        constexpr int n = Wide<T>::n;
+        Wide<T> w[4];
+        const int have = share.load(w, r);
+        float top = -INFINITY;
 #pragma unroll
-                         for (int i = 0; i < Wide<T>::n; ++i) { v[i] = w.get(i); top = fmaxf(top, v[i]); }
-                         if (top > st.m || st.m == -INFINITY || st.m == INFINITY) {
+        for (int k = 0; k < 4; ++k)
+            if (k < have)
 #pragma unroll
-                             for (int i = 0; i < Wide<T>::n; ++i) add(st, v[i]);
-                         } else {
-                             // (-inf: exp gives 0, and 0 * inf must not reach u; a NaN reaches both sums through e)
+                for (int i = 0; i < n; ++i) top = fmaxf(top, w[k].get(i));
+        const bool best = st.raise(top, r);
+        const float from = -st.base();
+        const f32x2 from2 = pack2(from, from), log2e2 = pack2(kLog2e, kLog2e);
+        f32x2 sum2 = 0ull, u2 = 0ull;
 #pragma unroll
-                             for (int i = 0; i < Wide<T>::n; ++i) {
-                                 const float t = v[i] - st.m, e = __expf(t);
-                                 st.s += e;
-                                 st.u += e * fminf(-t, 1e30f);
-                             }
-                         }
-                     });
+        for (int k = 0; k < 4; ++k)
+            if (k < have)
+#pragma unroll
+                for (int i = 0; i < n / 2; ++i) {
+                    const f32x2 t = add2(w[k].pair(i), from2);
+                    const float2 z = unpack2(mul2(t, log2e2));
+                    const f32x2 e = pack2(exp2_approx(z.x), exp2_approx(z.y));
+                    sum2 = add2(sum2, e);
+                    u2 = fma2(e, t, u2);
+                }
+        const float2 sum = unpack2(sum2), u = unpack2(u2);
+        (best ? st.best : st.rest) += sum.x + sum.y;
+        st.u -= u.x + u.y;
+    }
+    if (st.u != st.u && st.all() == st.all()) {  // -inf among the values: 0 * inf reached u
+        st.u = 0.f;
+        share.every([&](int, float v) {
+            const float t = v - st.base();
+            st.u += __expf(t) * fminf(-t, 1e30f);
+        });
+    }
     const float mine = st.m;
-    RowState all = st;
-#pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-        const RowState other{__shfl_xor_sync(0xffffffffu, all.m, d), __shfl_xor_sync(0xffffffffu, all.s, d), __shfl_xor_sync(0xffffffffu, all.u, d)};
-        // (both lanes join in the same order, so that they agree)
-        all = threadIdx.x & d ? join(other, all) : join(all, other);
+    // (of nothing but -inf: the empty state; a NaN among them stays)
+    RowState all = mine == -INFINITY ? RowState{mine, st.all() == 0.f ? -1.f : st.all(), 0.f} : RowState{mine, st.all() - 1.f, st.u};
+    all = join_block<THREADS>(all, states);
+    if (all.m > -INFINITY && all.s < 1.f) {
+        // one class has m, and s may be all rounding of 1 + s: the sum around it without it
+        float sum = st.all() * __expf(mine - all.m);  // (0 where nothing was seen)
+        if (mine == all.m) {
+            sum = st.rest;
+            share.round(st.at, [&](int, float v) { sum += v == all.m ? 0.f : __expf(v - all.m); });
+        }
+        block_sync<THREADS>();
+        all.s = sum_block<THREADS>(sum, reinterpret_cast<float *>(states));
     }
     if (TOP) {
         float gt = mine;
@@ -197,20 +304,17 @@ __global__ void __launch_bounds__(THREADS) token_logprobs_kernel(const LogpArgs 
         if (threadIdx.x % kGroup == 0) group_top[threadIdx.x / kGroup] = gt;
         if (threadIdx.x == 0) { count = 0; bound = -INFINITY; }
     }
-    if (threadIdx.x % 32 == 0) states[threadIdx.x / 32] = all;
-    block_sync<THREADS>();
     if (threadIdx.x == 0) {
-        for (int w = 1; w < kWarps; ++w) all = join(all, states[w]);
         if (p.parts == 1) {
             const long long t = p.target[row];
             finish_row(p, row, all, t >= 0 && t < p.C ? to_f32<T>(x[t]) : 0.f);
         } else {
             p.part_state[row * p.parts + part] = all;
         }
-        states[0] = all;
     }
     if (!TOP) return;
     const int top = min(p.top, end - first);
+    block_sync<THREADS>();
     if ((int)threadIdx.x < kGroups) {
         // the top-th largest of the groups' largest values, where there are as many groups
         const float v = group_top[threadIdx.x];
@@ -223,7 +327,7 @@ __global__ void __launch_bounds__(THREADS) token_logprobs_kernel(const LogpArgs 
     }
     block_sync<THREADS>();
     const float least = bound;
-    const bool odd = isnan(states[0].s);  // NaN among the logits: the bound says nothing of them
+    const bool odd = isnan(all.s);  // NaN among the logits: the bound says nothing of them
     if (mine >= least || odd) {
         auto offer = [&](int j, float v) {
             if (v >= least || v != v) {
@@ -231,13 +335,13 @@ __global__ void __launch_bounds__(THREADS) token_logprobs_kernel(const LogpArgs 
                 if (at < kCandidates) cand[at] = key_of(v, j);
             }
         };
-        walk<T, THREADS>(x, first, end, offer, [&](int j, const Wide<T> &w) {
-#pragma unroll
-            for (int i = 0; i < Wide<T>::n; ++i) offer(j + i, w.get(i));
-        });
+        if (odd || st.second >= least)
+            share.every(offer);
+        else
+            share.round(st.at, offer);
     }
     block_sync<THREADS>();
-    const float m = states[0].m, L = p.parts == 1 ? p.stats[row * 3 + 1] : 0.f;
+    const float m = all.m, L = p.parts == 1 ? p.stats[row * 3 + 1] : 0.f;
     auto put = [&](int rank, unsigned long long key) {
         if (p.parts > 1) {
             p.part_keys[(row * p.parts + part) * p.top + rank] = key;
@@ -260,10 +364,7 @@ __global__ void __launch_bounds__(THREADS) token_logprobs_kernel(const LogpArgs 
             const unsigned long long k = key_of(v, j);
             if (k < last && k > best) best = k;
         };
-        walk<T, THREADS>(x, first, end, look, [&](int j, const Wide<T> &w) {
-#pragma unroll
-            for (int i = 0; i < Wide<T>::n; ++i) look(j + i, w.get(i));
-        });
+        share.every(look);
 #pragma unroll
         for (int d = 16; d; d >>= 1) {
             const unsigned long long o = __shfl_xor_sync(0xffffffffu, best, d);
@@ -281,32 +382,34 @@ __global__ void __launch_bounds__(THREADS) token_logprobs_kernel(const LogpArgs 
 // joins the parts of a row
 template <typename T>
 __global__ void __launch_bounds__(256) token_logprobs_join_kernel(const LogpArgs p) {
-    __shared__ unsigned long long cand[kCandidates];
+    __shared__ RowState states[8];
+    __shared__ unsigned long long keys[kMaxParts * kMaxTop], cand[kCandidates], bound;
     __shared__ int count;
-    __shared__ unsigned long long bound;
     const long row = blockIdx.x;
-    const unsigned long long *keys = p.part_keys + row * p.parts * p.top;
-    RowState all = empty_state();
-    for (int i = 0; i < p.parts; ++i) all = join(all, p.part_state[row * p.parts + i]);
+    const int total = p.parts * p.top;
+    for (int i = threadIdx.x; i < total; i += 256) keys[i] = p.part_keys[row * total + i];
+    const long long t = p.target[row];
+    const float given = threadIdx.x == 0 && t >= 0 && t < p.C ? to_f32<T>(static_cast<const T *>(p.x)[row * p.pitch + t]) : 0.f;
     if (threadIdx.x == 0) {
-        const long long t = p.target[row];
-        finish_row(p, row, all, t >= 0 && t < p.C ? to_f32<T>(static_cast<const T *>(p.x)[row * p.pitch + t]) : 0.f);
         count = 0;
         bound = 0;
     }
+    const RowState mine = (int)threadIdx.x < p.parts ? p.part_state[row * p.parts + threadIdx.x] : RowState{-INFINITY, -1.f, 0.f};
+    const RowState all = join_block<256>(mine, states);
+    if (threadIdx.x == 0) finish_row(p, row, all, given);
     if (!p.top) return;
     __syncthreads();
     // a key that at least `top` keys reach: the top-th largest of the parts' largest, where there are as many parts
-    for (int i = threadIdx.x; i < p.parts; i += 256) {
-        const unsigned long long k = keys[(long)i * p.top];
+    if ((int)threadIdx.x < p.parts) {
+        const unsigned long long k = keys[threadIdx.x * p.top];
         int above = 0;
-        for (int j = 0; j < p.parts; ++j) above += keys[(long)j * p.top] > k;
+        for (int j = 0; j < p.parts; ++j) above += keys[j * p.top] > k;
         if (above == p.top - 1) bound = k;
     }
     __syncthreads();
     const unsigned long long least = bound > 1 ? bound : 1;
     // (at most `top` parts reach it, with `top` keys each)
-    for (int i = threadIdx.x; i < p.parts * p.top; i += 256)
+    for (int i = threadIdx.x; i < total; i += 256)
         if (keys[i] >= least) {
             const int at = atomicAdd(&count, 1);
             if (at < kCandidates) cand[at] = keys[i];
@@ -321,11 +424,11 @@ __global__ void __launch_bounds__(256) token_logprobs_join_kernel(const LogpArgs
         rank_out<256>(cand, count, p.top, put);
         return;
     }
-    for (int i = threadIdx.x; i < p.parts * p.top; i += 256) {
+    for (int i = threadIdx.x; i < total; i += 256) {
         const unsigned long long k = keys[i];
         if (k < least) continue;
         int rank = 0;
-        for (int j = 0; j < p.parts * p.top; ++j) rank += keys[j] > k;
+        for (int j = 0; j < total; ++j) rank += keys[j] > k;
         if (rank < p.top) put(rank, k);
     }
 }
@@ -347,37 +450,41 @@ __global__ void __launch_bounds__(256) token_logprobs_grad_kernel(const GradArgs
     const int first = blockIdx.y * p.span, end = min(p.C, first + p.span);
     const T *x = static_cast<const T *>(p.x) + row * p.pitch;
     T *gx = static_cast<T *>(p.gx) + row * p.C;
+    constexpr int n = Wide<T>::n;
+    const uintptr_t a = reinterpret_cast<uintptr_t>(x + first), b = reinterpret_cast<uintptr_t>(gx + first);
+    const bool aligned = !((a ^ b) & 15);  // else rows lie differently on 16-byte boundaries
+    const int head = aligned ? min(end - first, (int)(((16 - (a & 15)) & 15) / sizeof(T))) : end - first;
+    const int vecs = (end - first - head) / n, tail = first + head + vecs * n;
+    const uint4 *v = reinterpret_cast<const uint4 *>(x + first + head);
+    uint4 *o = reinterpret_cast<uint4 *>(gx + first + head);
+    Wide<T> w[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+        if ((int)threadIdx.x + k * 256 < vecs) w[k].raw = v[threadIdx.x + k * 256];
     const float m = p.stats[row * 3], L = p.stats[row * 3 + 1], U = p.stats[row * 3 + 2];
     const long long t = p.target[row];
     const bool none = m == -INFINITY && L == 0.f;
     const float gl = t != p.ignore && p.g_logp ? p.g_logp[row] : 0.f, ge = p.g_entropy ? p.g_entropy[row] : 0.f;
     const bool bad = t != p.ignore && (t < 0 || t >= p.C);
-    auto grad = [&](int j, float v) {
-        if (none) return 0.f;
-        const float a = v - m, lp = a - L, pr = __expf(lp);
-        float g = j == t ? -gl * expm1f(lp) : -gl * pr;
-        if (pr != 0.f) g -= ge * pr * (a + U);  // (-inf: no probability, no gradient)
-        return bad ? NAN : g;
+    const int given = bad || t == p.ignore ? -1 : (int)t;
+    const float gu = gl + ge * U;
+    // -p (gl + ge (U - d)), and gl more for the given class: without the difference of near values for it
+    auto grad = [&](int j, float x) {
+        const float t = x - m, pr = __expf(t - L);
+        float g = pr != 0.f ? -pr * (gu + ge * t) : 0.f;  // (-inf: no probability, no gradient)
+        if (j == given) g = -gl * expm1f(t - L) - (pr != 0.f ? ge * pr * (t + U) : 0.f);
+        return none ? 0.f : bad ? NAN : g;
     };
-    constexpr int n = Wide<T>::n;
-    const uintptr_t a = reinterpret_cast<uintptr_t>(x + first), b = reinterpret_cast<uintptr_t>(gx + first);
-    if ((a ^ b) & 15) {  // rows that lie differently on 16-byte boundaries
-        for (int j = first + threadIdx.x; j < end; j += 256) gx[j] = from_f32<T>(grad(j, to_f32<T>(x[j])));
-        return;
-    }
-    const int head = min(end - first, (int)(((16 - (a & 15)) & 15) / sizeof(T))), vecs = (end - first - head) / n, tail = first + head + vecs * n;
-    if ((int)threadIdx.x < head) gx[first + threadIdx.x] = from_f32<T>(grad(first + threadIdx.x, to_f32<T>(x[first + threadIdx.x])));
+    for (int j = threadIdx.x; j < head; j += 256) gx[first + j] = from_f32<T>(grad(first + j, to_f32<T>(x[first + j])));
     if (tail + (int)threadIdx.x < end) gx[tail + threadIdx.x] = from_f32<T>(grad(tail + threadIdx.x, to_f32<T>(x[tail + threadIdx.x])));
-    const uint4 *v = reinterpret_cast<const uint4 *>(x + first + head);
-    uint4 *o = reinterpret_cast<uint4 *>(gx + first + head);
-    for (int i = threadIdx.x; i < vecs; i += 2 * 256) {
-        Wide<T> w[2];
-        w[0].raw = v[i];
-        const bool two = i + 256 < vecs;
-        if (two) w[1].raw = v[i + 256];
+    for (int i = threadIdx.x; i < vecs; i += 4 * 256) {
+        if (i != (int)threadIdx.x)
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-            if (k && !two) break;
+            for (int k = 0; k < 4; ++k)
+                if (i + k * 256 < vecs) w[k].raw = v[i + k * 256];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            if (i + k * 256 >= vecs) break;
             union {
                 uint4 raw;
                 T v[n];
@@ -399,10 +506,10 @@ void launch_forward(const LogpArgs &p, cudaStream_t stream) {
 
 template <typename T>
 int forward(LogpArgs &p, cudaStream_t stream) {
-    // a warp for short rows, four for rows of a few thousand classes, sixteen for long ones
+    // a warp for short rows, four warps for rows that fit many to an SM, sixteen for the longest
     if (p.part_len <= 512 && p.parts == 1)
         launch_forward<T, 32>(p, stream);
-    else if (p.part_len <= 4096)
+    else if (p.part_len <= 65536)
         launch_forward<T, 128>(p, stream);
     else
         launch_forward<T, 512>(p, stream);
@@ -426,7 +533,7 @@ int backward(const GradArgs &p, cudaStream_t stream) {
 int logprobs_parts(long N, int C, int sms) {
     const long want = (2L * sms) / (N > 0 ? N : 1), most = (C + 2047) / 2048;
     const long parts = want < most ? want : most;
-    return parts < 2 ? 1 : (int)(parts > 64 ? 64 : parts);
+    return parts < 2 ? 1 : (int)(parts > kMaxParts ? kMaxParts : parts);
 }
 size_t logprobs_scratch_bytes(long N, int C, int top, int sms) {
     const int parts = logprobs_parts(N, C, sms);
@@ -450,7 +557,9 @@ int logprobs_forward(const void *x, int dtype, long pitch, long N, int C, const 
 int logprobs_backward(const void *x, int dtype, long pitch, long N, int C, const long long *target, long long ignore, const float *stats,
                       const float *g_logp, const float *g_entropy, void *gx, cudaStream_t stream) {
     GradArgs p{x, pitch, N, C, target, ignore, stats, g_logp, g_entropy, gx, 0};
-    p.span = N * ((C + 8191) / 8192) < 512 ? 2048 : 8192;
+    // four vectors to a thread, fewer where the blocks would not fill the GPU
+    const int full = 4 * 256 * (dtype == LUTGEMM_F32 ? 4 : 8);
+    p.span = N * ((C + full - 1) / full) < 512 ? full / 4 : full;
     while ((long)(C + p.span - 1) / p.span > 65535) p.span *= 2;
     if (dtype == LUTGEMM_F32) return backward<float>(p, stream);
     if (dtype == LUTGEMM_BF16) return backward<__nv_bfloat16>(p, stream);

@@ -15,6 +15,7 @@
 // ascending order, so results do not depend on timing.
 #include "lutgemm.h"
 #include "lutgemm_attention.cuh"
+#include "lutgemm_f32x2.cuh"
 #include "lutgemm_kernels.h"
 
 namespace lutgemm {
@@ -78,171 +79,245 @@ __device__ __forceinline__ Slot slot_of(const NormArgs &p, int c) {
     }
     return s;
 }
-// pairs of a slot: the half layout pairs a[i] with b[i], the interleaved one neighbours in (a, b)
+// A slot's 2V values as packed pairs, in order a, b.  P is a pair of lanes of packed fp32 arithmetic; the partner of value e in a rotation is
+// the same place of the other vector (half layout) or its neighbour (interleaved).
 template <int V>
-__device__ __forceinline__ void turn(float (&a)[V], float (&b)[V], const float (&c)[V], const float (&s)[V], bool interleaved) {
-    if (!interleaved || V == 1) {
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-            const float x = a[i], y = b[i];
-            a[i] = x * c[i] - y * s[i];
-            b[i] = y * c[i] + x * s[i];
-        }
+struct Packed {
+    static constexpr int n = V == 1 ? 1 : V;  // pairs of 2V values
+    f32x2 v[n];
+};
+template <typename T, int V>
+__device__ __forceinline__ void widen(Packed<V> &d, const Vec<T, V> &a, const Vec<T, V> &b) {
+    if constexpr (V == 1) {
+        d.v[0] = pack2(to_f32<T>(a.v[0]), to_f32<T>(b.v[0]));
     } else {
 #pragma unroll
         for (int i = 0; i < V / 2; ++i) {
-            float x = a[2 * i], y = a[2 * i + 1];
-            a[2 * i] = x * c[i] - y * s[i];
-            a[2 * i + 1] = y * c[i] + x * s[i];
-            x = b[2 * i];
-            y = b[2 * i + 1];
-            b[2 * i] = x * c[V / 2 + i] - y * s[V / 2 + i];
-            b[2 * i + 1] = y * c[V / 2 + i] + x * s[V / 2 + i];
+            d.v[i] = pack2(to_f32<T>(a.v[2 * i]), to_f32<T>(a.v[2 * i + 1]));
+            d.v[V / 2 + i] = pack2(to_f32<T>(b.v[2 * i]), to_f32<T>(b.v[2 * i + 1]));
         }
     }
 }
+template <typename T, int V>
+__device__ __forceinline__ void store_slot(T *p, int a, int b, const Packed<V> &d) {
+    float x[V], y[V];
+    if constexpr (V == 1) {
+        const float2 t = unpack2(d.v[0]);
+        x[0] = t.x;
+        y[0] = t.y;
+    } else {
+#pragma unroll
+        for (int i = 0; i < V / 2; ++i) {
+            const float2 t = unpack2(d.v[i]), u = unpack2(d.v[V / 2 + i]);
+            x[2 * i] = t.x;
+            x[2 * i + 1] = t.y;
+            y[2 * i] = u.x;
+            y[2 * i + 1] = u.y;
+        }
+    }
+    store_vec<T, V>(p + a, x);
+    store_vec<T, V>(p + b, y);
+}
+// what the value in place i of a rotation is paired with
+template <int V>
+__device__ __forceinline__ f32x2 partner(const Packed<V> &d, int i, bool interleaved) {
+    if (V == 1 || interleaved) {  // (with one value to a vector both layouts pair a with b)
+        const float2 t = unpack2(d.v[i]);
+        return pack2(t.y, t.x);
+    }
+    return d.v[i < V / 2 ? i + V / 2 : i - V / 2];
+}
+// cosines and signed sines of a slot's values: turned = x * c + partner * s
+template <int V>
+__device__ __forceinline__ void angles(Packed<V> &c, Packed<V> &s, const float (&co)[V], const float (&si)[V], bool interleaved) {
+    if constexpr (V == 1) {
+        c.v[0] = pack2(co[0], co[0]);
+        s.v[0] = pack2(-si[0], si[0]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < V / 2; ++i) {
+            if (interleaved) {  // pair i of a, pair V/2 + i of b
+                c.v[i] = pack2(co[i], co[i]);
+                s.v[i] = pack2(-si[i], si[i]);
+                c.v[V / 2 + i] = pack2(co[V / 2 + i], co[V / 2 + i]);
+                s.v[V / 2 + i] = pack2(-si[V / 2 + i], si[V / 2 + i]);
+            } else {
+                c.v[i] = c.v[V / 2 + i] = pack2(co[2 * i], co[2 * i + 1]);
+                s.v[i] = pack2(-si[2 * i], -si[2 * i + 1]);
+                s.v[V / 2 + i] = pack2(si[2 * i], si[2 * i + 1]);
+            }
+        }
+    }
+}
+__device__ __forceinline__ float both(f32x2 v) {
+    const float2 t = unpack2(v);
+    return t.x + t.y;
+}
 
-// V values to a vector, SPL slots to a lane, HEADS heads of a token at a time
-template <typename T, int V, int SPL, int HEADS, bool BACKWARD>
-__global__ void __launch_bounds__(kBlock) norm_rotate_kernel(const NormArgs p) {
+// V values to a vector, SPL slots to a lane, HEADS heads of a token at a time.  INTER: the interleaved layout
+template <typename T, int V, int SPL, int HEADS, bool INTER, bool BACKWARD>
+__global__ void __launch_bounds__(kBlock, 2) norm_rotate_kernel(const NormArgs p) {
+    constexpr int N = Packed<V>::n;
     extern __shared__ float sums[];  // backward: [groups][D]
     const bool second = (int)blockIdx.x >= p.side[0].blocks;
     const Side &sd = p.side[second];
     const int block = blockIdx.x - (second ? p.side[0].blocks : 0);
     const int lane = threadIdx.x & (p.lanes - 1), group = threadIdx.x / p.lanes, groups = kBlock / p.lanes;
     const int chunks = (sd.heads + HEADS - 1) / HEADS, slots = p.D / (2 * V), half = p.rot / 2;
-    const long units = (long)p.B * p.T * chunks;
+    const unsigned units = (unsigned)p.B * p.T * chunks;
     const float inv_d = 1.f / (float)p.D;
     Slot slot[SPL];
-    float wa[SPL][V], wb[SPL][V], da[SPL][V], db[SPL][V];
+    Packed<V> w[SPL], dw[BACKWARD ? SPL : 1];
 #pragma unroll
     for (int s = 0; s < SPL; ++s) {
         const int c = lane + s * p.lanes;
         slot[s] = slot_of<V>(p, c);
         if (c >= slots) slot[s].a = -1;
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-            wa[s][i] = slot[s].a >= 0 && sd.w ? sd.w[slot[s].a + i] : 1.f;
-            wb[s][i] = slot[s].a >= 0 && sd.w ? sd.w[slot[s].b + i] : 1.f;
-            da[s][i] = db[s][i] = 0.f;
+        for (int i = 0; i < N; ++i) w[s].v[i] = pack2(1.f, 1.f);
+        if (slot[s].a >= 0 && sd.w) {
+            float x[V], y[V];
+#pragma unroll
+            for (int i = 0; i < V; ++i) {  // (weights may lie on any boundary)
+                x[i] = sd.w[slot[s].a + i];
+                y[i] = sd.w[slot[s].b + i];
+            }
+            if constexpr (V == 1) {
+                w[s].v[0] = pack2(x[0], y[0]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < V / 2; ++i) {
+                    w[s].v[i] = pack2(x[2 * i], x[2 * i + 1]);
+                    w[s].v[V / 2 + i] = pack2(y[2 * i], y[2 * i + 1]);
+                }
+            }
         }
+        if constexpr (BACKWARD)
+#pragma unroll
+            for (int i = 0; i < N; ++i) dw[s].v[i] = 0ull;
     }
     // (whole warps go round together: the shuffles below are over groups of lanes of one warp)
-    for (long u0 = (long)block * groups; u0 < units; u0 += (long)sd.blocks * groups) {
-        const long u = u0 + group;
+    for (unsigned u0 = (unsigned)block * groups; u0 < units; u0 += (unsigned)sd.blocks * groups) {
+        const unsigned u = u0 + group;
         const bool in = u < units;
-        const long token = in ? u / chunks : 0;
-        const int h0 = in ? (int)(u - token * chunks) * HEADS : 0, b = (int)(token / p.T), t = (int)(token - (long)b * p.T);
-        const int at = p.pos ? (in ? p.pos[token] : -1) : t;
-        const T *x = static_cast<const T *>(sd.x) + b * sd.sb + t * sd.st + h0 * sd.sh;
-        const T *g = BACKWARD ? static_cast<const T *>(sd.g) + b * sd.gb + t * sd.gt + h0 * sd.gh : nullptr;
-        T *y = static_cast<T *>(sd.y) + (token * sd.heads + h0) * p.D;
-        float xa[HEADS][SPL][V], xb[HEADS][SPL][V], ga[BACKWARD ? HEADS : 1][SPL][V], gb[BACKWARD ? HEADS : 1][SPL][V];
+        const unsigned token = in ? u / chunks : 0u, b = token / (unsigned)p.T, t = token - b * (unsigned)p.T;
+        const int h0 = in ? (int)(u - token * chunks) * HEADS : 0, heads = in ? min(HEADS, sd.heads - h0) : 0;
+        const T *x = static_cast<const T *>(sd.x) + (long)b * sd.sb + (long)t * sd.st + h0 * sd.sh;
+        const T *g = BACKWARD ? static_cast<const T *>(sd.g) + (long)b * sd.gb + (long)t * sd.gt + h0 * sd.gh : nullptr;
+        T *y = static_cast<T *>(sd.y) + ((long)token * sd.heads + h0) * p.D;
+        // as they lie in memory, all heads' loads in flight together
+        Vec<T, V> raw[HEADS][SPL][BACKWARD ? 4 : 2];
 #pragma unroll
         for (int h = 0; h < HEADS; ++h)
 #pragma unroll
             for (int s = 0; s < SPL; ++s) {
-                const bool ok = in && h0 + h < sd.heads && slot[s].a >= 0;
-                if (ok) {
-                    load_vec<T, V>(xa[h][s], x + h * sd.sh + slot[s].a);
-                    load_vec<T, V>(xb[h][s], x + h * sd.sh + slot[s].b);
-                    if (BACKWARD) {
-                        load_vec<T, V>(ga[h][s], g + h * sd.gh + slot[s].a);
-                        load_vec<T, V>(gb[h][s], g + h * sd.gh + slot[s].b);
-                    }
-                } else {
 #pragma unroll
-                    for (int i = 0; i < V; ++i) {
-                        xa[h][s][i] = xb[h][s][i] = 0.f;
-                        if (BACKWARD) ga[h][s][i] = gb[h][s][i] = 0.f;
+                for (int k = 0; k < (BACKWARD ? 4 : 2); ++k)
+#pragma unroll
+                    for (int i = 0; i < V; ++i) raw[h][s][k].v[i] = from_f32<T>(0.f);
+                if (h < heads && slot[s].a >= 0) {
+                    raw[h][s][0] = *reinterpret_cast<const Vec<T, V> *>(x + h * sd.sh + slot[s].a);
+                    raw[h][s][1] = *reinterpret_cast<const Vec<T, V> *>(x + h * sd.sh + slot[s].b);
+                    if constexpr (BACKWARD) {
+                        raw[h][s][2] = *reinterpret_cast<const Vec<T, V> *>(g + h * sd.gh + slot[s].a);
+                        raw[h][s][3] = *reinterpret_cast<const Vec<T, V> *>(g + h * sd.gh + slot[s].b);
                     }
                 }
             }
-        float c[SPL][V], sn[SPL][V];
+        const int at = p.pos ? (in ? p.pos[token] : -1) : (int)t;
+        Packed<V> c[SPL], sn[SPL];  // forward: with the weights
 #pragma unroll
         for (int s = 0; s < SPL; ++s) {
             const bool turned = slot[s].a >= 0 && slot[s].angle >= 0 && at >= 0;
+            float co[V], si[V];
 #pragma unroll
-            for (int i = 0; i < V; ++i) { c[s][i] = 1.f; sn[s][i] = 0.f; }
+            for (int i = 0; i < V; ++i) {
+                co[i] = turned ? NAN : 1.f;  // (a position beyond the table)
+                si[i] = 0.f;
+            }
             if (turned && at < p.table) {
-                load_vec<float, V>(c[s], p.cos + (long)at * half + slot[s].angle);
-                load_vec<float, V>(sn[s], p.sin + (long)at * half + slot[s].angle);
-            } else if (turned) {
-#pragma unroll
-                for (int i = 0; i < V; ++i) c[s][i] = NAN;
+                load_vec<float, V>(co, p.cos + (long)at * half + slot[s].angle);
+                load_vec<float, V>(si, p.sin + (long)at * half + slot[s].angle);
             }
             if (BACKWARD)
 #pragma unroll
-                for (int i = 0; i < V; ++i) sn[s][i] = -sn[s][i];
+                for (int i = 0; i < V; ++i) si[i] = -si[i];
+            angles<V>(c[s], sn[s], co, si, INTER);
+            if constexpr (!BACKWARD) {
+                Packed<V> ws;
+#pragma unroll
+                for (int i = 0; i < N; ++i) ws.v[i] = mul2(sn[s].v[i], partner<V>(w[s], i, INTER));
+#pragma unroll
+                for (int i = 0; i < N; ++i) {
+                    sn[s].v[i] = ws.v[i];
+                    c[s].v[i] = mul2(c[s].v[i], w[s].v[i]);
+                }
+            }
         }
 #pragma unroll
         for (int h = 0; h < HEADS; ++h) {
-            float sq = 0.f;
+            Packed<V> xv[SPL], gv[SPL];
+            f32x2 sq2 = 0ull;
 #pragma unroll
-            for (int s = 0; s < SPL; ++s)
+            for (int s = 0; s < SPL; ++s) {
+                widen<T, V>(xv[s], raw[h][s][0], raw[h][s][1]);
+                if constexpr (BACKWARD) widen<T, V>(gv[s], raw[h][s][2], raw[h][s][3]);
 #pragma unroll
-                for (int i = 0; i < V; ++i) sq += xa[h][s][i] * xa[h][s][i] + xb[h][s][i] * xb[h][s][i];
+                for (int i = 0; i < N; ++i) sq2 = fma2(xv[s].v[i], xv[s].v[i], sq2);
+            }
+            float sq = both(sq2);
             for (int d = p.lanes / 2; d; d >>= 1) sq += __shfl_xor_sync(0xffffffffu, sq, d);
             const float r = rsqrtf(sq * inv_d + p.eps);
-            const bool row = in && h0 + h < sd.heads;
-            if (!BACKWARD) {
+            const f32x2 r2 = pack2(r, r);
+            if constexpr (!BACKWARD) {
 #pragma unroll
                 for (int s = 0; s < SPL; ++s) {
+                    Packed<V> o;
 #pragma unroll
-                    for (int i = 0; i < V; ++i) { xa[h][s][i] *= r * wa[s][i]; xb[h][s][i] *= r * wb[s][i]; }
-                    turn<V>(xa[h][s], xb[h][s], c[s], sn[s], p.interleaved);
-                    if (row && slot[s].a >= 0) {
-                        store_vec<T, V>(y + h * p.D + slot[s].a, xa[h][s]);
-                        store_vec<T, V>(y + h * p.D + slot[s].b, xb[h][s]);
-                    }
+                    for (int i = 0; i < N; ++i) xv[s].v[i] = mul2(xv[s].v[i], r2);
+#pragma unroll
+                    for (int i = 0; i < N; ++i) o.v[i] = fma2(partner<V>(xv[s], i, INTER), sn[s].v[i], mul2(xv[s].v[i], c[s].v[i]));
+                    if (h < heads && slot[s].a >= 0) store_slot<T, V>(y + h * p.D, slot[s].a, slot[s].b, o);
                 }
             } else {
-                float dot = 0.f;
+                f32x2 dot2 = 0ull;
 #pragma unroll
                 for (int s = 0; s < SPL; ++s) {
-                    turn<V>(ga[h][s], gb[h][s], c[s], sn[s], p.interleaved);
+                    Packed<V> o;
 #pragma unroll
-                    for (int i = 0; i < V; ++i) {
-                        xa[h][s][i] *= r;
-                        xb[h][s][i] *= r;
-                        da[s][i] += row ? ga[h][s][i] * xa[h][s][i] : 0.f;
-                        db[s][i] += row ? gb[h][s][i] * xb[h][s][i] : 0.f;
-                        ga[h][s][i] *= wa[s][i];
-                        gb[h][s][i] *= wb[s][i];
-                        dot += ga[h][s][i] * xa[h][s][i] + gb[h][s][i] * xb[h][s][i];
+                    for (int i = 0; i < N; ++i) o.v[i] = fma2(partner<V>(gv[s], i, INTER), sn[s].v[i], mul2(gv[s].v[i], c[s].v[i]));
+#pragma unroll
+                    for (int i = 0; i < N; ++i) {
+                        xv[s].v[i] = mul2(xv[s].v[i], r2);
+                        dw[s].v[i] = fma2(o.v[i], xv[s].v[i], dw[s].v[i]);  // (rows that are not there are zeros)
+                        gv[s].v[i] = mul2(o.v[i], w[s].v[i]);
+                        dot2 = fma2(gv[s].v[i], xv[s].v[i], dot2);
                     }
                 }
+                float dot = both(dot2);
                 for (int d = p.lanes / 2; d; d >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, d);
-                dot *= inv_d;
+                dot *= -inv_d;
+                const f32x2 d2 = pack2(dot, dot);
 #pragma unroll
                 for (int s = 0; s < SPL; ++s) {
 #pragma unroll
-                    for (int i = 0; i < V; ++i) {
-                        ga[h][s][i] = r * (ga[h][s][i] - xa[h][s][i] * dot);
-                        gb[h][s][i] = r * (gb[h][s][i] - xb[h][s][i] * dot);
-                    }
-                    if (row && slot[s].a >= 0) {
-                        store_vec<T, V>(y + h * p.D + slot[s].a, ga[h][s]);
-                        store_vec<T, V>(y + h * p.D + slot[s].b, gb[h][s]);
-                    }
+                    for (int i = 0; i < N; ++i) gv[s].v[i] = mul2(r2, fma2(xv[s].v[i], d2, gv[s].v[i]));
+                    if (h < heads && slot[s].a >= 0) store_slot<T, V>(y + h * p.D, slot[s].a, slot[s].b, gv[s]);
                 }
             }
         }
     }
-    if (!BACKWARD || !sd.part) return;
+    if constexpr (BACKWARD) {
+        if (!sd.part) return;
 #pragma unroll
-    for (int s = 0; s < SPL; ++s)
-        if (slot[s].a >= 0)
-#pragma unroll
-            for (int i = 0; i < V; ++i) {
-                sums[group * p.D + slot[s].a + i] = da[s][i];
-                sums[group * p.D + slot[s].b + i] = db[s][i];
-            }
-    __syncthreads();
-    for (int d = threadIdx.x; d < p.D; d += kBlock) {
-        float t = 0.f;
-        for (int k = 0; k < groups; ++k) t += sums[k * p.D + d];
-        sd.part[(size_t)block * p.D + d] = t;
+        for (int s = 0; s < SPL; ++s)
+            if (slot[s].a >= 0) store_slot<float, V>(sums + group * p.D, slot[s].a, slot[s].b, dw[s]);
+        __syncthreads();
+        for (int d = threadIdx.x; d < p.D; d += kBlock) {
+            float t = 0.f;
+            for (int k = 0; k < groups; ++k) t += sums[k * p.D + d];
+            sd.part[(size_t)block * p.D + d] = t;
+        }
     }
 }
 
@@ -267,7 +342,7 @@ __global__ void __launch_bounds__(1024) norm_weight_sums_kernel(const NormArgs p
 
 template <typename T, int V, int SPL, bool BACKWARD>
 int launch(NormArgs &p, int sms, cudaStream_t stream) {
-    constexpr int kMany = SPL > 1 || BACKWARD ? 2 : 4;
+    constexpr int kMany = SPL > 1 ? 1 : BACKWARD ? 2 : 4;  // (as many as leave two blocks to an SM by their registers)
     const int groups = kBlock / p.lanes;
     const long rows = (long)p.B * p.T * (p.side[0].heads + p.side[1].heads);
     const bool many = rows >= 8L * sms * groups;  // four blocks an SM with two heads to a group
@@ -278,15 +353,17 @@ int launch(NormArgs &p, int sms, cudaStream_t stream) {
         const long most = norm_rotate_blocks(sms) * (long)p.side[i].heads / (p.side[0].heads + p.side[1].heads);
         blocks[i] = (units + groups - 1) / groups;
         if (blocks[i] > most) blocks[i] = most > 0 ? most : 1;
-        if (p.side[i].heads == 0) blocks[i] = 0;
         p.side[i].blocks = (int)blocks[i];
     }
     if (BACKWARD && p.side[1].part) p.side[1].part = p.side[1].part + (size_t)blocks[0] * p.D;
     const size_t smem = BACKWARD ? sizeof(float) * groups * p.D : 0;
+    const int grid = (int)(blocks[0] + blocks[1]);
     if (many)
-        norm_rotate_kernel<T, V, SPL, kMany, BACKWARD><<<(int)(blocks[0] + blocks[1]), kBlock, smem, stream>>>(p);
+        (p.interleaved ? norm_rotate_kernel<T, V, SPL, kMany, true, BACKWARD> : norm_rotate_kernel<T, V, SPL, kMany, false, BACKWARD>)
+            <<<grid, kBlock, smem, stream>>>(p);
     else
-        norm_rotate_kernel<T, V, SPL, 1, BACKWARD><<<(int)(blocks[0] + blocks[1]), kBlock, smem, stream>>>(p);
+        (p.interleaved ? norm_rotate_kernel<T, V, SPL, 1, true, BACKWARD> : norm_rotate_kernel<T, V, SPL, 1, false, BACKWARD>)
+            <<<grid, kBlock, smem, stream>>>(p);
     int rc = launch_status();
     if (rc == LUTGEMM_OK && BACKWARD && (p.side[0].part || p.side[1].part)) {
         norm_weight_sums_kernel<<<dim3((p.D + 31) / 32, 2), 1024, 0, stream>>>(p);
@@ -315,7 +392,6 @@ int vector_width(const NormArgs &p, int size, bool backward) {
         bool ok = ((reinterpret_cast<uintptr_t>(p.cos) | reinterpret_cast<uintptr_t>(p.sin)) & (4 * v - 1)) == 0 && p.rot / 2 % v == 0;
         for (int i = 0; i < 2 && ok; ++i) {
             const Side &s = p.side[i];
-            if (s.heads == 0) continue;
             ok = ((reinterpret_cast<uintptr_t>(s.x) | reinterpret_cast<uintptr_t>(s.y)) & (bytes - 1)) == 0 && s.sb % v == 0 &&
                  s.st % v == 0 && s.sh % v == 0;
             if (backward)
