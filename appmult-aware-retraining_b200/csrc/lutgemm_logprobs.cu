@@ -461,19 +461,26 @@ __global__ void __launch_bounds__(256) token_logprobs_grad_kernel(const GradArgs
 #pragma unroll
     for (int k = 0; k < 4; ++k)
         if ((int)threadIdx.x + k * 256 < vecs) w[k].raw = v[threadIdx.x + k * 256];
-    const float m = p.stats[row * 3], L = p.stats[row * 3 + 1], U = p.stats[row * 3 + 2];
+    // (a row without any probability: p = 0 everywhere)
+    const bool none = p.stats[row * 3] == -INFINITY && p.stats[row * 3 + 1] == 0.f;
+    const float m = none ? 0.f : p.stats[row * 3], L = none ? INFINITY : p.stats[row * 3 + 1], U = p.stats[row * 3 + 2];
     const long long t = p.target[row];
-    const bool none = m == -INFINITY && L == 0.f;
-    const float gl = t != p.ignore && p.g_logp ? p.g_logp[row] : 0.f, ge = p.g_entropy ? p.g_entropy[row] : 0.f;
     const bool bad = t != p.ignore && (t < 0 || t >= p.C);
     const int given = bad || t == p.ignore ? -1 : (int)t;
-    const float gu = gl + ge * U;
-    // -p (gl + ge (U - d)), and gl more for the given class: without the difference of near values for it
-    auto grad = [&](int j, float x) {
+    const float gl = bad ? NAN : t != p.ignore && p.g_logp ? p.g_logp[row] : 0.f, ge = p.g_entropy ? p.g_entropy[row] : 0.f;
+    // -p (gl + ge (U - d)), and for the given class gl more, without the difference of near values
+    const f32x2 from2 = pack2(-m, -m), log2e2 = pack2(kLog2e, kLog2e), less2 = pack2(-L * kLog2e, -L * kLog2e),
+                ge2 = pack2(-ge, -ge), gu2 = pack2(-(gl + ge * U), -(gl + ge * U));
+    const auto grads = [&](f32x2 x) {
+        const f32x2 t = add2(x, from2);
+        const float2 z = unpack2(fma2(t, log2e2, less2)), d = unpack2(t);
+        // (-inf: p is 0, and 0 * inf must not reach the product; a NaN reaches it through p)
+        return unpack2(mul2(pack2(exp2_approx(z.x), exp2_approx(z.y)), fma2(ge2, pack2(fmaxf(d.x, -1e30f), fmaxf(d.y, -1e30f)), gu2)));
+    };
+    const auto grad = [&](int j, float x) {
+        if (j != given) return grads(pack2(x, x)).x;
         const float t = x - m, pr = __expf(t - L);
-        float g = pr != 0.f ? -pr * (gu + ge * t) : 0.f;  // (-inf: no probability, no gradient)
-        if (j == given) g = -gl * expm1f(t - L) - (pr != 0.f ? ge * pr * (t + U) : 0.f);
-        return none ? 0.f : bad ? NAN : g;
+        return none ? 0.f : -gl * expm1f(t - L) - (pr != 0.f ? ge * pr * (t + U) : 0.f);
     };
     for (int j = threadIdx.x; j < head; j += 256) gx[first + j] = from_f32<T>(grad(first + j, to_f32<T>(x[first + j])));
     if (tail + (int)threadIdx.x < end) gx[tail + threadIdx.x] = from_f32<T>(grad(tail + threadIdx.x, to_f32<T>(x[tail + threadIdx.x])));
@@ -490,8 +497,14 @@ __global__ void __launch_bounds__(256) token_logprobs_grad_kernel(const GradArgs
                 T v[n];
             } r;
 #pragma unroll
-            for (int e = 0; e < n; ++e) r.v[e] = from_f32<T>(grad(first + head + (i + k * 256) * n + e, w[k].get(e)));
+            for (int e = 0; e < n / 2; ++e) {
+                const float2 g = grads(w[k].pair(e));
+                r.v[2 * e] = from_f32<T>(g.x);
+                r.v[2 * e + 1] = from_f32<T>(g.y);
+            }
             o[i + k * 256] = r.raw;
+            const int base = first + head + (i + k * 256) * n;
+            if ((unsigned)(given - base) < (unsigned)n) gx[given] = from_f32<T>(grad(given, to_f32<T>(x[given])));
         }
     }
 }
