@@ -46,7 +46,7 @@ __global__ void __launch_bounds__(kThreads, Layout<T, DP>::kPerSm)
     volatile int *abort_word = reinterpret_cast<int *>(smem + L::kBars + 72);
     uint32_t *slot = reinterpret_cast<uint32_t *>(smem + L::kBars + 76);
     volatile int *tiles = reinterpret_cast<int *>(smem + L::kBars + 80);  // of the last four rounds begun
-    const int tid = threadIdx.x, warp = tid >> 5;
+    const int tid = threadIdx.x, warp = warp_index();
     // blocks in order of falling work: the last rows see the most keys
     int bid = blockIdx.x;
     const int split = bid % splits;
@@ -88,11 +88,11 @@ __global__ void __launch_bounds__(kThreads, Layout<T, DP>::kPerSm)
             queue[i] = more ? walk.next(docs) : kEnd;
         };
         auto bring_k = [&](int i, int stage) {
-            if (queue[i] >= 0 && (tid & 31) == 0)
+            if (queue[i] >= 0 && elect_one())
                 load_keys<L::kBlocks>(base + L::kK + stage * L::kTile, &map_k, b, g, (queue[i] >> 1) * kKeyTile, bar_k + 8 * stage);
         };
         auto bring_v = [&](int i, int stage) {
-            if (queue[i] >= 0 && (tid & 31) == 0)
+            if (queue[i] >= 0 && elect_one())
                 load_keys<L::kBlocks>(base + L::kV + stage * L::kTile, &map_v, b, g, (queue[i] >> 1) * kKeyTile, bar_v + 8 * stage);
         };
 #pragma unroll
@@ -123,7 +123,7 @@ __global__ void __launch_bounds__(kThreads, Layout<T, DP>::kPerSm)
 #pragma unroll
         for (int i = 0; i < L::kStages; ++i) {
             if (queue[i] >= 0) mbar_wait(bar_k + 8 * i, 0, 206, abort_word, error_word);
-            if ((tid & 31) == 0 && (i == 0 || queue[i - 1] >= 0)) issue_scores(i, queue[i]);
+            if ((i == 0 || queue[i - 1] >= 0) && elect_one()) issue_scores(i, queue[i]);
         }
         __syncwarp();
         for (int n = 0; queue[0] >= 0; ++n) {
@@ -141,7 +141,7 @@ __global__ void __launch_bounds__(kThreads, Layout<T, DP>::kPerSm)
             mbar_wait(bar_p, n & 1, 201, abort_word, error_word);
             tmem_after_sync();
             __syncwarp();
-            if ((tid & 31) == 0) {
+            if (elect_one()) {
                 const uint64_t v = smem_descriptor(base + L::kV + (n & 1) * L::kTile, Op::kPlanes ? 0 : kKeyTile * 128);
                 const uint32_t a = tmem + (n % L::kStages) * L::kS;
                 if constexpr (Op::kPlanes) {

@@ -106,7 +106,7 @@ __global__ void __launch_bounds__(GradLayout<T, DP, KEYS>::kThreads, GradLayout<
     uint32_t *slot = reinterpret_cast<uint32_t *>(smem + L::kBars + 76);
     volatile int *tiles = reinterpret_cast<int *>(smem + L::kBars + 80);  // of the last eight rounds begun
     float *tops = reinterpret_cast<float *>(smem + L::kBars + 128);       // of the warps
-    const int tid = threadIdx.x, warp = tid >> 5;
+    const int tid = threadIdx.x, warp = warp_index();
     int bid = blockIdx.x;
     const int g = bid % p.G;
     bid /= p.G;
@@ -243,7 +243,7 @@ __global__ void __launch_bounds__(GradLayout<T, DP, KEYS>::kThreads, GradLayout<
                     }
                 }
             }
-            if (lane == 0) {
+            if (elect_one()) {
                 tma_expect_bytes(bar, 2 * L::kBlocks * (KEYS ? size : 64) * 128);
 #pragma unroll
                 for (int k = 0; k < L::kBlocks; ++k) {
@@ -308,7 +308,7 @@ __global__ void __launch_bounds__(GradLayout<T, DP, KEYS>::kThreads, GradLayout<
             arrived(i, i);
             __syncwarp();
             // (every group hears of the end in its own round)
-            if (lane == 0) issue_scores(i, queue[i]);
+            if (elect_one()) issue_scores(i, queue[i]);
         }
         __syncwarp();
         int n = 0;
@@ -322,7 +322,7 @@ __global__ void __launch_bounds__(GradLayout<T, DP, KEYS>::kThreads, GradLayout<
             if (!Op::kPlanes && n > 0) mbar_wait(bar_acc, (n - 1) & 1, 213, abort_word, error_word);
             tmem_after_sync();
             __syncwarp();
-            if (lane == 0) {
+            if (elect_one()) {
                 const uint32_t d = tmem + n % G * L::kGroup;
                 const uint64_t x = smem_descriptor(base + L::kRing + n % L::kStages * 2 * L::kTile, Op::kPlanes ? 0 : 64 * 128);
 #pragma unroll

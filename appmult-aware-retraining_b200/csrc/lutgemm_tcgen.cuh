@@ -11,6 +11,17 @@
 
 namespace lutgemm {
 
+// One lane of a whole warp.  Products are issued from `if (elect_one())` in code that the warp enters together, with the operand sizes as
+// constants: the compiler then keeps their operands in uniform registers.  128 x 64 x 16 products take 33 clocks (first operand
+// from tensor memory) and 49 (from shared memory) that way, 94 from `if (lane == 0)`.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+    return p != 0;
+}
+// this thread's warp, the same register for all its lanes
+__device__ __forceinline__ int warp_index() { return __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0); }
+
 // ---- tensor memory ----------------------------------------------------------------------------------------------------
 // by one warp; the address of `columns` (a power of two from 32 on) goes to *slot in shared memory
 __device__ __forceinline__ void tmem_alloc(uint32_t slot, uint32_t columns) {
