@@ -19,6 +19,7 @@ from __future__ import annotations
 
 import contextlib
 import ctypes
+import functools
 import os
 
 import torch
@@ -229,6 +230,13 @@ def _guard(device: torch.device):
 def _stream_ptr(device: torch.device) -> int:
     # (the handle itself: a stream object takes four microseconds to make)
     return torch._C._cuda_getCurrentRawStream(device.index)
+
+
+@functools.lru_cache(maxsize=4096)
+def _scratch_bytes(name: str, index: int, *sizes) -> int:
+    """Scratch bytes of an entry point for a problem of these sizes on CUDA device `index`, which is current: they depend on nothing
+    else, and asking the library takes a call."""
+    return getattr(_load(), name)(*sizes)
 
 
 def _backward_scratch(query, args, codes_t, dev):

@@ -120,24 +120,34 @@ __global__ void __launch_bounds__(kThreads, Layout<T, DP>::kPerSm)
             }
             mbar_arrive(bar);
         };
+        // what padding holds: a probability of zero would not hide it in V, and in K it would have a say in how caps are computed
+        auto clear_padding = [&](int tile, uint32_t at) {
+            if (!docs || Op::kPlanes) return;
+            const unsigned long long mask = key_mask(p, b, (tile >> 1) * kKeyTile);
+            if (~mask) {
+                clear_rows<L::kBlocks>(smem + at, mask);
+                writes_to_tensor_cores();
+            }
+        };
 #pragma unroll
         for (int i = 0; i < L::kStages; ++i) {
-            if (queue[i] >= 0) mbar_wait(bar_k + 8 * i, 0, 206, abort_word, error_word);
+            if (queue[i] >= 0) {
+                mbar_wait(bar_k + 8 * i, 0, 206, abort_word, error_word);
+                clear_padding(queue[i], L::kK + i * L::kTile);
+                __syncwarp();
+            }
             if ((i == 0 || queue[i - 1] >= 0) && elect_one()) issue_scores(i, queue[i]);
         }
         __syncwarp();
         for (int n = 0; queue[0] >= 0; ++n) {
             bring(L::kStages + 1);
             mbar_wait(bar_v + 8 * (n & 1), n >> 1 & 1, 207, abort_word, error_word);
-            if (docs && !Op::kPlanes) {  // a probability of zero does not hide what padding may hold
-                const unsigned long long mask = key_mask(p, b, (queue[0] >> 1) * kKeyTile);
-                if (~mask) {
-                    clear_rows<L::kBlocks>(smem + L::kV + (n & 1) * L::kTile, mask);
-                    writes_to_tensor_cores();
-                }
+            clear_padding(queue[0], L::kV + (n & 1) * L::kTile);
+            if (queue[L::kStages] >= 0 && queue[L::kStages - 1] >= 0) {
+                const int stage = (n + L::kStages) % L::kKStages;
+                mbar_wait(bar_k + 8 * stage, (n + L::kStages) / L::kKStages & 1, 208, abort_word, error_word);
+                clear_padding(queue[L::kStages], L::kK + stage * L::kTile);
             }
-            if (queue[L::kStages] >= 0 && queue[L::kStages - 1] >= 0)
-                mbar_wait(bar_k + 8 * ((n + L::kStages) % L::kKStages), (n + L::kStages) / L::kKStages & 1, 208, abort_word, error_word);
             mbar_wait(bar_p, n & 1, 201, abort_word, error_word);
             tmem_after_sync();
             __syncwarp();
@@ -213,12 +223,23 @@ __global__ void __launch_bounds__(kThreads, Layout<T, DP>::kPerSm)
             if (BENT) {
                 if (p.cap > 0.f) {
 #pragma unroll
-                    for (int h = 0; h < 2; ++h)
+                    for (int h = 0; h < 2; ++h) {
+                        if (bend.all_small(s[h])) {
 #pragma unroll
-                        for (int j = 0; j < 32; ++j) {
-                            float unused;
-                            s[h][j] = bend.capped<Op::kPlanes>(s[h][j], &unused);
+                            for (int j = 0; j < 32; j += 2) {
+                                f32x2 unused;
+                                const float2 x = unpack2(bend.capped_small(pack2(s[h][j], s[h][j + 1]), &unused));
+                                s[h][j] = x.x;
+                                s[h][j + 1] = x.y;
+                            }
+                        } else {
+#pragma unroll
+                            for (int j = 0; j < 32; ++j) {
+                                float unused;
+                                s[h][j] = bend.template capped<Op::kPlanes>(s[h][j], &unused);
+                            }
                         }
+                    }
                 } else {
 #pragma unroll
                     for (int h = 0; h < 2; ++h)

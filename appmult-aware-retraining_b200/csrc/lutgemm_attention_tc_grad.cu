@@ -443,6 +443,7 @@ __global__ void __launch_bounds__(GradLayout<T, DP, KEYS>::kThreads, GradLayout<
                         seen &= same;
                     }
                 }
+                const bool small = BENT && p.cap > 0.f && bend.all_small(s);
                 uint32_t wp[Op::kPlanes ? 3 : 1][16], ws[Op::kPlanes ? 3 : 1][16];
 #pragma unroll
                 for (int j = 0; j < 32; j += 2) {
@@ -455,33 +456,42 @@ __global__ void __launch_bounds__(GradLayout<T, DP, KEYS>::kThreads, GradLayout<
                         d2 = pack2(less_delta, less_delta);
                     }
                     float2 x;
-                    float2 b2 = make_float2(1.f, 1.f);
+                    f32x2 b2 = pack2(1.f, 1.f);
                     if (BENT) {
-                        float y[2] = {s[j], s[j + 1]};
-#pragma unroll
-                        for (int e = 0; e < 2; ++e) {
-                            if (p.cap > 0.f) {
-                                y[e] = bend.capped<Op::kPlanes>(y[e], e ? &b2.y : &b2.x);
+                        f32x2 y;
+                        if (p.cap > 0.f) {
+                            if (small) {
+                                y = bend.capped_small(pack2(s[j], s[j + 1]), &b2);
                             } else {
-                                y[e] *= bend.scale2;
+                                float da, dc;
+                                const float ya = bend.template capped<Op::kPlanes>(s[j], &da), yc = bend.template capped<Op::kPlanes>(s[j + 1], &dc);
+                                y = pack2(ya, yc);
+                                b2 = pack2(da, dc);
                             }
-                            if (p.slopes) {
-                                if (KEYS) {
-                                    const int c = 32 * h + j + e;
-                                    y[e] -= cols[192 + c] * fabsf(cols[256 + c] - (float)key);
-                                } else {
-                                    y[e] -= row.slope * fabsf((float)(row.place - t0) - (float)(32 * h + j + e));
-                                }
-                            }
+                        } else {
+                            y = mul2(pack2(s[j], s[j + 1]), scale2);
                         }
-                        x = unpack2(add2(pack2(y[0], y[1]), l2));
+                        if (p.slopes) {
+                            float2 away, less;  // distances, and what they take from the scores
+                            if (KEYS) {
+                                const int c = 32 * h + j;
+                                away = make_float2(fabsf(cols[256 + c] - (float)key), fabsf(cols[257 + c] - (float)key));
+                                less = make_float2(-cols[192 + c], -cols[193 + c]);
+                            } else {
+                                const float first = (float)(row.place - t0) - (float)(32 * h + j);
+                                away = make_float2(fabsf(first), fabsf(first - 1.f));
+                                less = make_float2(-row.slope, -row.slope);
+                            }
+                            y = fma2(pack2(less.x, less.y), pack2(away.x, away.y), y);
+                        }
+                        x = unpack2(add2(y, l2));
                     } else {
                         x = unpack2(fma2(pack2(s[j], s[j + 1]), scale2, l2));
                     }
                     float a = fast_exp2(x.x), c = fast_exp2(x.y);
                     f32x2 u = add2(pack2(gp[j], gp[j + 1]), d2);
                     if (!kBf16) u = mul2(u, unit2);
-                    if (BENT) u = mul2(u, pack2(b2.x, b2.y));
+                    if (BENT) u = mul2(u, b2);
                     float2 ds = unpack2(mul2(pack2(a, c), u));
                     if (masked) {  // (by choice, not by a factor: what is masked may be anything)
                         const bool sa = seen >> j & 1, sc = seen >> (j + 1) & 1;

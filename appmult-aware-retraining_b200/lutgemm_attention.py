@@ -84,24 +84,28 @@ def rotary_tables_2d(height: int, width: int, rot: int, base: float = 100.0, dev
     return angles.cos().float().to(device), angles.sin().float().to(device)
 
 
+def _norm_rotate_forward(q, k, qw, kw, cos, sin, positions, interleaved, eps):
+    B, T, H, D = q.shape
+    G, dev = k.shape[2], q.device
+    qo = torch.empty((B, T, H, D), dtype=q.dtype, device=dev)
+    ko = torch.empty((B, T, G, D), dtype=q.dtype, device=dev)
+    if B * T:
+        with approx_ops._guard(dev):
+            rc = approx_ops.library().lutgemm_norm_rotate(
+                *_at(q), *_at(k), qw.data_ptr() if qw is not None else None, kw.data_ptr() if kw is not None else None, cos.data_ptr(),
+                sin.data_ptr(), cos.shape[0], positions.data_ptr() if positions is not None else None, qo.data_ptr(), ko.data_ptr(),
+                _DTYPES[q.dtype], B, T, H, G, D, 2 * cos.shape[1], interleaved, eps, approx_ops._stream_ptr(dev))
+        approx_ops._check(rc, "norm_rotate")
+    return qo, ko
+
+
 class _NormRotate(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, qw, kw, cos, sin, positions, interleaved, eps):
         B, T, H, D = q.shape
-        G, rot, table = k.shape[2], 2 * cos.shape[1], cos.shape[0]
-        qo = torch.empty((B, T, H, D), dtype=q.dtype, device=q.device)
-        ko = torch.empty((B, T, G, D), dtype=q.dtype, device=q.device)
-        ctx.cfg = (B, T, H, G, D, rot, interleaved, eps)
+        ctx.cfg = (B, T, H, k.shape[2], D, 2 * cos.shape[1], interleaved, eps)
         ctx.save_for_backward(q, k, qw, kw, cos, sin, positions)
-        if B * T:
-            lib = approx_ops.library()
-            with approx_ops._guard(q.device):
-                rc = lib.lutgemm_norm_rotate(*_at(q), *_at(k), qw.data_ptr() if qw is not None else None,
-                                             kw.data_ptr() if kw is not None else None, cos.data_ptr(), sin.data_ptr(), table,
-                                             positions.data_ptr() if positions is not None else None, qo.data_ptr(), ko.data_ptr(),
-                                             _DTYPES[q.dtype], B, T, H, G, D, rot, interleaved, eps, approx_ops._stream_ptr(q.device))
-            approx_ops._check(rc, "norm_rotate")
-        return qo, ko
+        return _norm_rotate_forward(q, k, qw, kw, cos, sin, positions, interleaved, eps)
 
     @staticmethod
     @once_differentiable
@@ -117,7 +121,9 @@ class _NormRotate(torch.autograd.Function):
         gq, gk = _rows(gq), _rows(gk)
         lib = approx_ops.library()
         with approx_ops._guard(q.device):
-            nbytes = lib.lutgemm_norm_rotate_backward_scratch_bytes(D) if dqw is not None or dkw is not None else 0
+            nbytes = 0
+            if dqw is not None or dkw is not None:
+                nbytes = approx_ops._scratch_bytes("lutgemm_norm_rotate_backward_scratch_bytes", q.get_device(), D)
             scratch = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
             rc = lib.lutgemm_norm_rotate_backward(
                 *_at(gq), *_at(gk), *_at(q), *_at(k), qw.data_ptr() if qw is not None else None,
@@ -172,30 +178,41 @@ def norm_rotate(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor = None,
             _check_side(w, name, w.dtype if w.dtype in _DTYPES else torch.float32, (D,), q)
             w = w.float().contiguous()
         weights.append(w)
-    return _NormRotate.apply(_rows(q), _rows(k), weights[0], weights[1], cos.contiguous(), sin.contiguous(), positions,
-                             layout == "interleaved", float(eps))
+    args = (_rows(q), _rows(k), weights[0], weights[1], cos.contiguous(), sin.contiguous(), positions, layout == "interleaved", float(eps))
+    # (without a backward pass the call through autograd would be a fifth of its time)
+    wanted = torch.is_grad_enabled() and any(x is not None and x.requires_grad for x in args[:4])
+    return _NormRotate.apply(*args) if wanted else _norm_rotate_forward(*args)
+
+
+def _masks(scale, cap, slopes, causal, prefix, doc_q, doc_k):
+    """The arguments of the library's calls that say who sees whom."""
+    return (scale, cap, slopes.data_ptr() if slopes is not None else None, causal, prefix.data_ptr() if prefix is not None else None,
+            *((doc_q.data_ptr(), doc_q.stride(0), doc_k.data_ptr(), doc_k.stride(0)) if doc_q is not None else (None, 0, None, 0)))
+
+
+def _attention_forward(training, q, k, v, scale, cap, slopes, causal, prefix, doc_q, doc_k):
+    """(out, rest, lse); rest, which the backward pass of 16-bit operands wants: what the rounding of out leaves."""
+    B, Tq, H, D = q.shape
+    Tk, G, dev = k.shape[1], k.shape[2], q.device
+    out = torch.empty((B, Tq, H, D), dtype=q.dtype, device=dev)
+    lse = torch.empty((B, G, Tq * H // G), dtype=torch.float32, device=dev)
+    rest = torch.empty_like(out) if training and q.dtype is not torch.float32 else None
+    dtype = _DTYPES[q.dtype]
+    with approx_ops._guard(dev):
+        nbytes = approx_ops._scratch_bytes("lutgemm_attention_scratch_bytes", dev.index, dtype, B, Tq, Tk, H, G, D, doc_k is not None)
+        scratch = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+        rc = approx_ops.library().lutgemm_attention(
+            *_at(q), *_at(k), *_at(v), out.data_ptr(), rest.data_ptr() if rest is not None else None, lse.data_ptr(), dtype, B, Tq, Tk,
+            H, G, D, *_masks(scale, cap, slopes, causal, prefix, doc_q, doc_k), scratch.data_ptr() if nbytes else None, nbytes,
+            approx_ops._stream_ptr(dev))
+    approx_ops._check(rc, "attention")
+    return out, rest, lse
 
 
 class _Attention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, scale, cap, slopes, causal, prefix, doc_q, doc_k):
-        B, Tq, H, D = q.shape
-        Tk, G = k.shape[1], k.shape[2]
-        masks = (scale, cap, slopes.data_ptr() if slopes is not None else None, causal,
-                 prefix.data_ptr() if prefix is not None else None,
-                 *((doc_q.data_ptr(), doc_q.stride(0), doc_k.data_ptr(), doc_k.stride(0)) if doc_q is not None else (None, 0, None, 0)))
-        out = torch.empty((B, Tq, H, D), dtype=q.dtype, device=q.device)
-        lse = torch.empty((B, G, Tq * H // G), dtype=torch.float32, device=q.device)
-        # (the backward pass of 16-bit operands wants what the rounding of out leaves, too)
-        rest = torch.empty_like(out) if q.dtype is not torch.float32 and any(ctx.needs_input_grad[:3]) else None
-        lib, dtype = approx_ops.library(), _DTYPES[q.dtype]
-        with approx_ops._guard(q.device):
-            nbytes = lib.lutgemm_attention_scratch_bytes(dtype, B, Tq, Tk, H, G, D, doc_k is not None)
-            scratch = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
-            rc = lib.lutgemm_attention(*_at(q), *_at(k), *_at(v), out.data_ptr(),
-                                       rest.data_ptr() if rest is not None else None, lse.data_ptr(), dtype, B, Tq, Tk, H, G, D, *masks,
-                                       scratch.data_ptr() if nbytes else None, nbytes, approx_ops._stream_ptr(q.device))
-        approx_ops._check(rc, "attention")
+        out, rest, lse = _attention_forward(True, q, k, v, scale, cap, slopes, causal, prefix, doc_q, doc_k)
         ctx.save_for_backward(q, k, v, out, rest, lse, slopes, prefix, doc_q, doc_k)
         ctx.cfg = (scale, cap, causal)
         return out
@@ -207,20 +224,19 @@ class _Attention(torch.autograd.Function):
         scale, cap, causal = ctx.cfg
         B, Tq, H, D = q.shape
         Tk, G = k.shape[1], k.shape[2]
-        masks = (scale, cap, slopes.data_ptr() if slopes is not None else None, causal,
-                 prefix.data_ptr() if prefix is not None else None,
-                 *((doc_q.data_ptr(), doc_q.stride(0), doc_k.data_ptr(), doc_k.stride(0)) if doc_q is not None else (None, 0, None, 0)))
         go = _vectors(go)
         dq = torch.empty((B, Tq, H, D), dtype=q.dtype, device=q.device)
         dk = torch.empty((B, Tk, G, D), dtype=q.dtype, device=q.device)
         dv = torch.empty((B, Tk, G, D), dtype=q.dtype, device=q.device)
         lib, dtype = approx_ops.library(), _DTYPES[q.dtype]
         with approx_ops._guard(q.device):
-            nbytes = lib.lutgemm_attention_backward_scratch_bytes(dtype, B, Tq, Tk, H, G, D, doc_k is not None)
+            nbytes = approx_ops._scratch_bytes("lutgemm_attention_backward_scratch_bytes", q.get_device(), dtype, B, Tq, Tk, H, G, D,
+                                               doc_k is not None)
             scratch = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
             rc = lib.lutgemm_attention_backward(*_at(go), *_at(q), *_at(k), *_at(v), out.data_ptr(),
                                                 rest.data_ptr() if rest is not None else None, lse.data_ptr(), dq.data_ptr(),
-                                                dk.data_ptr(), dv.data_ptr(), dtype, B, Tq, Tk, H, G, D, *masks, scratch.data_ptr(), nbytes,
+                                                dk.data_ptr(), dv.data_ptr(), dtype, B, Tq, Tk, H, G, D,
+                                                *_masks(scale, cap, slopes, causal, prefix, doc_q, doc_k), scratch.data_ptr(), nbytes,
                                                 approx_ops._stream_ptr(q.device))
         approx_ops._check(rc, "attention (backward)")
         return dq, dk, dv, None, None, None, None, None, None, None
@@ -294,4 +310,7 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: float = 
             query_documents = query_documents if query_documents.stride(1) == 1 or Tq <= 1 else query_documents.contiguous()
     if B * Tq == 0 or Tk == 0:  # nothing to see: zeros, whose gradients are zeros
         return _Empty.apply(q, k, v)
-    return _Attention.apply(_vectors(q), _vectors(k), _vectors(v), scale, cap, slopes, bool(causal), prefix, query_documents, documents)
+    args = (_vectors(q), _vectors(k), _vectors(v), scale, cap, slopes, bool(causal), prefix, query_documents, documents)
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+        return _Attention.apply(*args)
+    return _attention_forward(False, *args)[0]

@@ -10,30 +10,35 @@ import approx_ops
 from lutgemm_attention import _DTYPES
 
 
+def _logprobs_forward(logits, targets, top, ignore_index):
+    """(logp, entropy, top_logp, top_index, stats); stats are for the backward pass."""
+    N, C = logits.shape
+    dev = logits.device
+    logp = torch.empty(N, dtype=torch.float32, device=dev)
+    entropy = torch.empty(N, dtype=torch.float32, device=dev)
+    stats = torch.empty((N, 3), dtype=torch.float32, device=dev)
+    top_logp = torch.empty((N, top), dtype=torch.float32, device=dev)
+    top_index = torch.empty((N, top), dtype=torch.int64, device=dev)
+    if N:
+        with approx_ops._guard(dev):
+            nbytes = approx_ops._scratch_bytes("lutgemm_token_logprobs_scratch_bytes", dev.index, N, C, top)
+            scratch = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+            rc = approx_ops.library().lutgemm_token_logprobs(
+                logits.data_ptr(), _DTYPES[logits.dtype], logits.stride(0), N, C, targets.data_ptr(), ignore_index, top, logp.data_ptr(),
+                entropy.data_ptr(), stats.data_ptr(), top_logp.data_ptr(), top_index.data_ptr(), scratch.data_ptr() if nbytes else None,
+                nbytes, approx_ops._stream_ptr(dev))
+        approx_ops._check(rc, "token_logprobs")
+    return logp, entropy, top_logp, top_index, stats
+
+
 class _TokenLogprobs(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, targets, top, ignore_index):
-        N, C = logits.shape
-        dev = logits.device
-        logp = torch.empty(N, dtype=torch.float32, device=dev)
-        entropy = torch.empty(N, dtype=torch.float32, device=dev)
-        stats = torch.empty((N, 3), dtype=torch.float32, device=dev)  # for the backward pass
-        top_logp = torch.empty((N, top), dtype=torch.float32, device=dev)
-        top_index = torch.empty((N, top), dtype=torch.int64, device=dev)
+        logp, entropy, top_logp, top_index, stats = _logprobs_forward(logits, targets, top, ignore_index)
         ctx.set_materialize_grads(False)
         ctx.mark_non_differentiable(top_logp, top_index)
         ctx.save_for_backward(logits, targets, stats)
         ctx.ignore_index = ignore_index
-        if N:
-            lib = approx_ops.library()
-            with approx_ops._guard(dev):
-                nbytes = lib.lutgemm_token_logprobs_scratch_bytes(N, C, top)
-                scratch = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-                rc = lib.lutgemm_token_logprobs(logits.data_ptr(), _DTYPES[logits.dtype], logits.stride(0), N, C, targets.data_ptr(),
-                                                ignore_index, top, logp.data_ptr(), entropy.data_ptr(), stats.data_ptr(),
-                                                top_logp.data_ptr(), top_index.data_ptr(), scratch.data_ptr() if nbytes else None,
-                                                nbytes, approx_ops._stream_ptr(dev))
-            approx_ops._check(rc, "token_logprobs")
         return logp, entropy, top_logp, top_index
 
     @staticmethod
@@ -86,7 +91,11 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, top: int = 0, ig
     x = logits if logits.dim() == 2 else logits.reshape(-1, C)
     if x.stride(1) != 1 and C > 1:
         x = x.contiguous()
-    out = _TokenLogprobs.apply(x, targets.reshape(-1).contiguous(), top, int(ignore_index))
+    t = targets.reshape(-1).contiguous()
+    if x.requires_grad and torch.is_grad_enabled():
+        out = _TokenLogprobs.apply(x, t, top, int(ignore_index))
+    else:
+        out = _logprobs_forward(x, t, top, int(ignore_index))[:4]
     if logits.dim() == 2:
         return out
     return out[0].view(lead), out[1].view(lead), out[2].view(*lead, top), out[3].view(*lead, top)
