@@ -151,6 +151,11 @@ __global__ void __launch_bounds__(kThreads, Layout<T, DP>::kPerSm)
             mbar_wait(bar_p, n & 1, 201, abort_word, error_word);
             tmem_after_sync();
             __syncwarp();
+            // every row has waited for the products of round n - 1 and S of round n: those buffers are free.  (Copies first: the queue
+            // of the tensor cores lets products go one by one)
+            bring_v(1, (n + 1) & 1);
+            bring_k(L::kStages + 1, n % L::kKStages);
+            __syncwarp();
             if (elect_one()) {
                 const uint64_t v = smem_descriptor(base + L::kV + (n & 1) * L::kTile, Op::kPlanes ? 0 : kKeyTile * 128);
                 const uint32_t a = tmem + (n % L::kStages) * L::kS;
@@ -168,9 +173,6 @@ __global__ void __launch_bounds__(kThreads, Layout<T, DP>::kPerSm)
                 if (queue[L::kStages - 1] >= 0) issue_scores(n + L::kStages, queue[L::kStages]);
             }
             __syncwarp();
-            // every row has waited for the products of round n - 1 and S of round n: those buffers are free
-            bring_v(1, (n + 1) & 1);
-            bring_k(L::kStages + 1, n % L::kKStages);
 #pragma unroll
             for (int i = 0; i <= L::kStages; ++i) queue[i] = queue[i + 1];
         }

@@ -68,19 +68,21 @@ __global__ void __launch_bounds__(256) attention_delta_kernel(const AttnProblem 
 //     S = X x^T, gP = Y y^T (tcgen05) -> a row to a thread: P, dS in registers -> P and dS in 16 bits to tensor memory, over S and gP ->
 //     KEYS: grad_v += P y;   grad_k or grad_q += dS x     (tcgen05, first operand from tensor memory; x and y, in shared memory as
 //     they were copied, serve as row and as column operands)
-// Eight warps share a round, four with the first 32 columns and four with the others; a further warp brings the tiles and issues the
-// products.  Heads of up to 64 values leave room for two blocks on an SM; with larger ones the accumulators fill the tensor
-// memory of an SM, and the block has two groups of eight warps that take rounds in turn, each with its own S and gP.
+// Eight warps share a round, four with the first 32 columns and four with the others; one further warp issues the products and one
+// brings the tiles (when one warp did both, copies were asked for only behind the products of a round, which the queue of the
+// tensor cores lets go one by one: a round of 128-value heads took 3200 clocks for 1300 of products).  Heads of up to 64 values
+// leave room for two blocks on an SM; with larger ones the accumulators fill the tensor memory of an SM, and the block has two
+// groups of eight warps that take rounds in turn, each with its own S and gP.
 // fp16: P is kept 2^10 larger, and grad_o is taken in units of its largest value in this key head (a power of two), so that dS stays
 // out of fp16's subnormal range whatever the scale of the loss.
 // fp32: P and dS are split into planes as the operands were, and have tensor memory of their own; each round's sums start from zero and
 // are added up in registers while the next scores are formed (in the accumulators, what additions cut off came to 2e-5 of
-// the gradients of 4096 rows).  Its ring has one stage less, which is brought when the round's products are done.
+// the gradients of 4096 rows).  Its ring has one stage less.
 template <typename T, int DP, bool KEYS>
 struct GradLayout {
     using Op = Operand<T, DP>;
     static constexpr int kBlocks = Op::kBlocks, kGroups = DP / 64, kStages = kGroups + (Op::kPlanes ? 1 : 2), kPerSm = DP == 64 && !Op::kPlanes ? 2 : 1;
-    static constexpr int kWorkers = 256 * kGroups, kThreads = kWorkers + 32, kSums = KEYS ? 2 : 1;
+    static constexpr int kWorkers = 256 * kGroups, kThreads = kWorkers + 64, kSums = KEYS ? 2 : 1;
     static constexpr uint32_t kTile = 64 * kBlocks * 128, kX = 0, kY = 2 * kTile, kRing = 4 * kTile;  // a stage of the ring: x, y
     static constexpr uint32_t kCols = kRing + kStages * 2 * kTile;  // KEYS: for each stage -lse, -delta, documents, slopes and places of 64 rows
     static constexpr uint32_t kBars = kCols + (KEYS ? kStages * 64 * 20 : 0), kBytes = kBars + 256;
@@ -101,11 +103,12 @@ __global__ void __launch_bounds__(GradLayout<T, DP, KEYS>::kThreads, GradLayout<
     constexpr float kShift = kBf16 ? 0.f : 10.f;
     extern __shared__ __align__(1024) uint8_t smem[];
     const uint32_t base = smem_u32(smem), bars = base + L::kBars;
-    const uint32_t bar_s = bars, bar_p = bars + 16, bar_acc = bars + 32, bar_full = bars + 40;  // (full: up to four stages)
-    volatile int *abort_word = reinterpret_cast<int *>(smem + L::kBars + 72);
-    uint32_t *slot = reinterpret_cast<uint32_t *>(smem + L::kBars + 76);
-    volatile int *tiles = reinterpret_cast<int *>(smem + L::kBars + 80);  // of the last eight rounds begun
-    float *tops = reinterpret_cast<float *>(smem + L::kBars + 128);       // of the warps
+    const uint32_t bar_s = bars, bar_p = bars + 16, bar_acc = bars + 32, bar_full = bars + 40, bar_empty = bars + 72;  // (four stages)
+    volatile int *abort_word = reinterpret_cast<int *>(smem + L::kBars + 104);
+    uint32_t *slot = reinterpret_cast<uint32_t *>(smem + L::kBars + 108);
+    volatile int *tiles = reinterpret_cast<int *>(smem + L::kBars + 112);  // of the last eight rounds begun; then how many there were
+    volatile int *brought = reinterpret_cast<int *>(smem + L::kBars + 148);  // of the stages
+    float *tops = reinterpret_cast<float *>(smem + L::kBars + 164);       // of the warps
     const int tid = threadIdx.x, warp = warp_index();
     int bid = blockIdx.x;
     const int g = bid % p.G;
@@ -124,7 +127,10 @@ __global__ void __launch_bounds__(GradLayout<T, DP, KEYS>::kThreads, GradLayout<
             mbar_init(bar_p + 8 * i, 256);
         }
         mbar_init(bar_acc, 1);
-        for (int i = 0; i < L::kStages; ++i) mbar_init(bar_full + 8 * i, 1);
+        for (int i = 0; i < L::kStages; ++i) {
+            mbar_init(bar_full + 8 * i, 1);
+            mbar_init(bar_empty + 8 * i, 1);
+        }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     // fp16: the unit of grad_o, 2^unit >= its largest value
@@ -166,7 +172,7 @@ __global__ void __launch_bounds__(GradLayout<T, DP, KEYS>::kThreads, GradLayout<
     if (!kBf16) {
         float top = 0.f;
 #pragma unroll
-        for (int w = 0; w < 8 * G + 1; ++w) top = fmaxf(top, tops[w]);
+        for (int w = 0; w < L::kThreads / 32; ++w) top = fmaxf(top, tops[w]);
         // (an infinite or NaN gradient, or none at all: as it is)
         const int e = (int)(__float_as_uint(top) >> 23);
         if (e > 0 && e < 254) unit = __uint_as_float((uint32_t)(e + 1) << 23);
@@ -175,7 +181,7 @@ __global__ void __launch_bounds__(GradLayout<T, DP, KEYS>::kThreads, GradLayout<
     // of the workers: the round group, the half of a round's columns, the row
     const int group = warp >> 3, h = warp >> 2 & 1, r = tid & 127;
     f32x2 sums[Op::kPlanes ? 16 * L::kSums : 1] = {};  // fp32: the worker's half of its row's sums
-    if (warp == 8 * G) {
+    if (warp == 8 * G + 1) {  // brings the tiles
         const int lane = tid & 31;
         TileWalk walk;
         if (KEYS) {
@@ -199,37 +205,29 @@ __global__ void __launch_bounds__(GradLayout<T, DP, KEYS>::kThreads, GradLayout<
                 walk.own = own_range(row_ranges + (long)b * ((p.M + size - 1) / size), o0, last + 1, size);
             }
         }
-        int queue[L::kStages + 1] = {};  // this round's tile and those behind it
-        auto next = [&](int i) {
-            const bool more = i == 0 || queue[i - 1] >= 0;
-            queue[i] = more ? walk.next(docs) : -1;
-        };
-        // KEYS: what a round needs of its rows, two to a lane; asked for ahead of `bring`, which hands it on
-        float row_stat[2], row_delta[2], row_slope[2], row_place[2];
-        int row_doc[2];
-        auto ask = [&](int i) {
-            if (!KEYS || queue[i] < 0) return;
+        for (int n = 0;; ++n) {
+            const int tile = walk.next(docs), t = tile >> 1, stage = n % L::kStages;
+            // KEYS: what a round needs of its rows, two to a lane
+            float row_stat[2], row_delta[2], row_slope[2], row_place[2];
+            int row_doc[2];
+            if (KEYS && tile >= 0)
 #pragma unroll
-            for (int k = 0; k < 2; ++k) {
-                const int c = lane + 32 * k, m = (queue[i] >> 1) * size + c;
-                const bool in = c < size && m < p.M;
-                row_stat[k] = in ? lse[stat0 + m] : INFINITY;
-                row_delta[k] = in ? delta[stat0 + m] : 0.f;
-                if (docs || (BENT && p.slopes)) {
-                    const int t = in ? m / p.R : 0;
-                    if (docs) row_doc[k] = in ? p.doc_q[b * p.doc_q_sb + t] : -1;
-                    if (BENT && p.slopes) {
-                        row_slope[k] = in ? p.slopes[g * p.R + m - t * p.R] * kLog2e : 0.f;
-                        row_place[k] = (float)(t + p.shift);
+                for (int k = 0; k < 2; ++k) {
+                    const int c = lane + 32 * k, m = t * size + c;
+                    const bool in = c < size && m < p.M;
+                    row_stat[k] = in ? lse[stat0 + m] : INFINITY;
+                    row_delta[k] = in ? delta[stat0 + m] : 0.f;
+                    if (docs || (BENT && p.slopes)) {
+                        const int i = in ? m / p.R : 0;
+                        if (docs) row_doc[k] = in ? p.doc_q[b * p.doc_q_sb + i] : -1;
+                        if (BENT && p.slopes) {
+                            row_slope[k] = in ? p.slopes[g * p.R + m - i * p.R] * kLog2e : 0.f;
+                            row_place[k] = (float)(i + p.shift);
+                        }
                     }
                 }
-            }
-        };
-        auto bring = [&](int i, int n) {  // queue[i], which is round n's
-            if (queue[i] < 0) return;
-            const int t = queue[i] >> 1, stage = n % L::kStages;
-            const uint32_t at = base + L::kRing + stage * 2 * L::kTile, bar = bar_full + 8 * stage;
-            if (KEYS) {
+            if (n >= L::kStages) mbar_wait(bar_empty + 8 * stage, (n / L::kStages - 1) & 1, 211, abort_word, error_word);
+            if (KEYS && tile >= 0) {
                 float *cols = reinterpret_cast<float *>(smem + L::kCols + stage * 64 * 20);
 #pragma unroll
                 for (int k = 0; k < 2; ++k) {
@@ -243,83 +241,91 @@ __global__ void __launch_bounds__(GradLayout<T, DP, KEYS>::kThreads, GradLayout<
                     }
                 }
             }
+            __syncwarp();
             if (elect_one()) {
-                tma_expect_bytes(bar, 2 * L::kBlocks * (KEYS ? size : 64) * 128);
+                const uint32_t at = base + L::kRing + stage * 2 * L::kTile, bar = bar_full + 8 * stage;
+                brought[stage] = tile;
+                if (tile >= 0) {
+                    tma_expect_bytes(bar, 2 * L::kBlocks * (KEYS ? size : 64) * 128);
 #pragma unroll
-                for (int k = 0; k < L::kBlocks; ++k) {
-                    const int i0 = KEYS ? t * (size / p.R) : t * 64;
-                    tma_load_5d(at + k * 64 * 128, &map_x, 64 * k, 0, i0, g, b, bar);
-                    tma_load_5d(at + L::kTile + k * 64 * 128, &map_y, 64 * k, 0, i0, g, b, bar);
+                    for (int k = 0; k < L::kBlocks; ++k) {
+                        const int i0 = KEYS ? t * (size / p.R) : t * 64;
+                        tma_load_5d(at + k * 64 * 128, &map_x, 64 * k, 0, i0, g, b, bar);
+                        tma_load_5d(at + L::kTile + k * 64 * 128, &map_y, 64 * k, 0, i0, g, b, bar);
+                    }
+                } else {
+                    mbar_arrive(bar);
                 }
             }
-        };
-        // the tile of round n has come; what padding holds must not meet a probability of zero
-        auto arrived = [&](int i, int n) {
-            if (queue[i] < 0) return;
-            mbar_wait(bar_full + 8 * (n % L::kStages), n / L::kStages & 1, 211, abort_word, error_word);
-            if (!docs || Op::kPlanes) return;  // (planes of padding are zeros)
-            uint8_t *at = smem + L::kRing + n % L::kStages * 2 * L::kTile;
-            if (KEYS) {
-                const int *ids = reinterpret_cast<const int *>(smem + L::kCols + n % L::kStages * 64 * 20) + 128;
-                const unsigned long long mask = __ballot_sync(0xffffffffu, ids[lane] >= 0) |
-                                                (unsigned long long)__ballot_sync(0xffffffffu, ids[lane + 32] >= 0) << 32;
-                if (~mask) {
-                    clear_rows<L::kBlocks>(at, mask);
-                    clear_rows<L::kBlocks>(at + L::kTile, mask);
-                    writes_to_tensor_cores();
-                }
-            } else {
-                const unsigned long long mask = key_mask(p, b, (queue[i] >> 1) * kKeyTile);
-                if (~mask) {
-                    clear_rows<L::kBlocks>(at, mask);
-                    writes_to_tensor_cores();
-                }
-            }
-        };
+            __syncwarp();
+            if (tile < 0 || *abort_word) break;
+        }
+    } else if (warp == 8 * G) {  // issues the products
+        const int lane = tid & 31;
         constexpr uint32_t desc_s = mma_descriptor(kBf16, 64, false), desc_acc = mma_descriptor(kBf16, DP, true);
-        auto issue_scores = [&](int n, int tile) {  // S and gP of round n, or word that there is none; one lane
+        // the tile of round n when it has come; -1: there is none
+        auto arrived = [&](int n, bool more) {
+            int tile = -1;
+            if (more) {
+                const int stage = n % L::kStages;
+                mbar_wait(bar_full + 8 * stage, n / L::kStages & 1, 212, abort_word, error_word);
+                tile = *abort_word ? -1 : brought[stage];
+                if (docs && !Op::kPlanes && tile >= 0) {
+                    // what padding holds must not meet a probability of zero (planes of padding are zeros)
+                    uint8_t *at = smem + L::kRing + stage * 2 * L::kTile;
+                    if (KEYS) {
+                        const int *ids = reinterpret_cast<const int *>(smem + L::kCols + stage * 64 * 20) + 128;
+                        const unsigned long long mask = __ballot_sync(0xffffffffu, ids[lane] >= 0) |
+                                                        (unsigned long long)__ballot_sync(0xffffffffu, ids[lane + 32] >= 0) << 32;
+                        if (~mask) {
+                            clear_rows<L::kBlocks>(at, mask);
+                            clear_rows<L::kBlocks>(at + L::kTile, mask);
+                            writes_to_tensor_cores();
+                        }
+                    } else {
+                        const unsigned long long mask = key_mask(p, b, (tile >> 1) * kKeyTile);
+                        if (~mask) {
+                            clear_rows<L::kBlocks>(at, mask);
+                            writes_to_tensor_cores();
+                        }
+                    }
+                }
+            }
+            return tile;
+        };
+        // S and gP of round n, or word that there is none; one lane
+        auto issue_scores = [&](int n, int tile) {
             const uint32_t bar = bar_s + 8 * (n % G);
-            tiles[n & 7] = tile;
-            if (tile >= 0) {
-                const uint32_t d = tmem + n % G * L::kGroup;
-                const uint64_t own = smem_descriptor(base + L::kX, 0), x = smem_descriptor(base + L::kRing + n % L::kStages * 2 * L::kTile, 0);
+            {
+                tiles[n & 7] = tile;
+                if (tile >= 0) {
+                    const uint32_t d = tmem + n % G * L::kGroup;
+                    const uint64_t own = smem_descriptor(base + L::kX, 0), x = smem_descriptor(base + L::kRing + n % L::kStages * 2 * L::kTile, 0);
 #pragma unroll
-                for (int e = 0; e < 2; ++e)
+                    for (int e = 0; e < 2; ++e)
 #pragma unroll
-                    for (int i = 0; i < 4 * Op::kProducts; ++i)
-                        mma_ss(d + 64 * e, descriptor_at(own, (e ? L::kY : L::kX) + Op::a(i >> 2) * 128 * 128 + (i & 3) * 32),
-                               descriptor_at(x, e * L::kTile + Op::b(i >> 2) * 64 * 128 + (i & 3) * 32), desc_s, i > 0);
-                mma_commit(bar);
-            } else {
+                        for (int i = 0; i < 4 * Op::kProducts; ++i)
+                            mma_ss(d + 64 * e, descriptor_at(own, (e ? L::kY : L::kX) + Op::a(i >> 2) * 128 * 128 + (i & 3) * 32),
+                                   descriptor_at(x, e * L::kTile + Op::b(i >> 2) * 64 * 128 + (i & 3) * 32), desc_s, i > 0);
+                    mma_commit(bar);
+                } else {
+                    mbar_arrive(bar);
+                }
                 mbar_arrive(bar);
             }
-            mbar_arrive(bar);
         };
-#pragma unroll
-        for (int i = 0; i < L::kStages; ++i) next(i);
-#pragma unroll
-        for (int i = 0; i < L::kStages - (Op::kPlanes ? 0 : 1); ++i) {
-            ask(i);
-            bring(i, i);
-        }
-        __syncwarp();
+        int ahead[G];  // tiles of the rounds that have begun
 #pragma unroll
         for (int i = 0; i < G; ++i) {
-            arrived(i, i);
+            ahead[i] = arrived(i, i == 0 || ahead[i > 0 ? i - 1 : 0] >= 0);
             __syncwarp();
-            // (every group hears of the end in its own round)
-            if (elect_one()) issue_scores(i, queue[i]);
+            if (elect_one()) issue_scores(i, ahead[i]);
+            __syncwarp();
         }
-        __syncwarp();
         int n = 0;
-        for (; queue[0] >= 0; ++n) {
-            next(L::kStages);
-            ask(L::kStages - (Op::kPlanes ? 0 : 1));
-            arrived(G, n + G);
-            mbar_wait(bar_p + 8 * (n % G), n / G & 1, 212, abort_word, error_word);
-            // the products of the round before are done, and with them its stage (before this round's commit: the barrier's parity
-            // tells two phases apart, not three)
-            if (!Op::kPlanes && n > 0) mbar_wait(bar_acc, (n - 1) & 1, 213, abort_word, error_word);
+        for (; ahead[0] >= 0; ++n) {
+            const int tile = arrived(n + G, ahead[G - 1] >= 0);
+            mbar_wait(bar_p + 8 * (n % G), n / G & 1, 213, abort_word, error_word);
             tmem_after_sync();
             __syncwarp();
             if (elect_one()) {
@@ -342,21 +348,20 @@ __global__ void __launch_bounds__(GradLayout<T, DP, KEYS>::kThreads, GradLayout<
                                    descriptor_at(with, i * 16 * 128), desc_acc, n > 0 || i > 0);
                     }
                 }
-                mma_commit(bar_acc);
-                issue_scores(n + G, queue[G]);
-            }
-            __syncwarp();
-            if (Op::kPlanes) {
-                mbar_wait(bar_acc, n & 1, 214, abort_word, error_word);
-                bring(L::kStages, n + L::kStages);
-            } else {
-                bring(L::kStages - 1, n + L::kStages - 1);
+                mma_commit(bar_empty + 8 * (n % L::kStages));
+                if (Op::kPlanes) mma_commit(bar_acc);
+                issue_scores(n + G, tile);
             }
             __syncwarp();
 #pragma unroll
-            for (int i = 0; i < L::kStages; ++i) queue[i] = queue[i + 1];
+            for (int i = 0; i + 1 < G; ++i) ahead[i] = ahead[i + 1];
+            ahead[G - 1] = tile;
         }
-        if (!Op::kPlanes && n > 0) mbar_wait(bar_acc, (n - 1) & 1, 216, abort_word, error_word);
+        if (n > 0) {  // (fp32: the workers have waited for all rounds but the last)
+            if (!Op::kPlanes && elect_one()) mma_commit(bar_acc);
+            __syncwarp();
+            mbar_wait(bar_acc, Op::kPlanes ? (n - 1) & 1 : 0, 214, abort_word, error_word);
+        }
         if (lane == 0) tiles[8] = n;  // rounds done
     } else {
         const uint32_t mine = tmem + ((uint32_t)((warp & 3) * 32) << 16);
