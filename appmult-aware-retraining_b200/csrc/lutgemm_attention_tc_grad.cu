@@ -296,23 +296,21 @@ __global__ void __launch_bounds__(GradLayout<T, DP, KEYS>::kThreads, GradLayout<
         // S and gP of round n, or word that there is none; one lane
         auto issue_scores = [&](int n, int tile) {
             const uint32_t bar = bar_s + 8 * (n % G);
-            {
-                tiles[n & 7] = tile;
-                if (tile >= 0) {
-                    const uint32_t d = tmem + n % G * L::kGroup;
-                    const uint64_t own = smem_descriptor(base + L::kX, 0), x = smem_descriptor(base + L::kRing + n % L::kStages * 2 * L::kTile, 0);
+            tiles[n & 7] = tile;
+            if (tile >= 0) {
+                const uint32_t d = tmem + n % G * L::kGroup;
+                const uint64_t own = smem_descriptor(base + L::kX, 0), x = smem_descriptor(base + L::kRing + n % L::kStages * 2 * L::kTile, 0);
 #pragma unroll
-                    for (int e = 0; e < 2; ++e)
+                for (int e = 0; e < 2; ++e)
 #pragma unroll
-                        for (int i = 0; i < 4 * Op::kProducts; ++i)
-                            mma_ss(d + 64 * e, descriptor_at(own, (e ? L::kY : L::kX) + Op::a(i >> 2) * 128 * 128 + (i & 3) * 32),
-                                   descriptor_at(x, e * L::kTile + Op::b(i >> 2) * 64 * 128 + (i & 3) * 32), desc_s, i > 0);
-                    mma_commit(bar);
-                } else {
-                    mbar_arrive(bar);
-                }
+                    for (int i = 0; i < 4 * Op::kProducts; ++i)
+                        mma_ss(d + 64 * e, descriptor_at(own, (e ? L::kY : L::kX) + Op::a(i >> 2) * 128 * 128 + (i & 3) * 32),
+                               descriptor_at(x, e * L::kTile + Op::b(i >> 2) * 64 * 128 + (i & 3) * 32), desc_s, i > 0);
+                mma_commit(bar);
+            } else {
                 mbar_arrive(bar);
             }
+            mbar_arrive(bar);
         };
         int ahead[G];  // tiles of the rounds that have begun
 #pragma unroll
@@ -414,107 +412,105 @@ __global__ void __launch_bounds__(GradLayout<T, DP, KEYS>::kThreads, GradLayout<
             const int t0 = (tile >> 1) * (KEYS ? size : 64);
             const bool masked = !(tile & 1);
             const f32x2 scale2 = pack2(bend.scale2, bend.scale2), unit2 = pack2(per_unit, per_unit);
-            {
-                float s[32], gp[32];
-                tmem_load32(at + 32 * h, s);
-                tmem_load32(at + 64 + 32 * h, gp);
-                tmem_loads_done();
-                // which of the 32 are seen
-                uint32_t seen = 0xffffffffu;
-                if (masked) {
+            float s[32], gp[32];
+            tmem_load32(at + 32 * h, s);
+            tmem_load32(at + 64 + 32 * h, gp);
+            tmem_loads_done();
+            // which of the 32 are seen
+            uint32_t seen = 0xffffffffu;
+            if (masked) {
+                if (KEYS) {
+                    const long skip = (long)from - t0 - 32 * h;
+                    seen = skip <= 0 ? 0xffffffffu : skip >= 32 ? 0u : 0xffffffffu << skip;
+                } else {
+                    const int reach = row.limit - t0 - 32 * h;
+                    seen = reach >= 31 ? 0xffffffffu : reach < 0 ? 0u : 0xffffffffu >> (31 - reach);
+                }
+                if (docs) {
+                    uint32_t same = 0;
                     if (KEYS) {
-                        const long skip = (long)from - t0 - 32 * h;
-                        seen = skip <= 0 ? 0xffffffffu : skip >= 32 ? 0u : 0xffffffffu << skip;
+                        const int4 *ids = reinterpret_cast<const int4 *>(cols + 128 + 32 * h);
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) {
+                            const int4 d = ids[j];
+                            same |= (uint32_t)(d.x == row.doc) << (4 * j) | (uint32_t)(d.y == row.doc) << (4 * j + 1) |
+                                    (uint32_t)(d.z == row.doc) << (4 * j + 2) | (uint32_t)(d.w == row.doc) << (4 * j + 3);
+                        }
                     } else {
-                        const int reach = row.limit - t0 - 32 * h;
-                        seen = reach >= 31 ? 0xffffffffu : reach < 0 ? 0u : 0xffffffffu >> (31 - reach);
+                        const int *ids = p.doc_k + b * p.doc_k_sb + t0 + 32 * h;
+                        const int have = p.Tk - t0 - 32 * h;
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) if (j < have && ids[j] == row.doc) same |= 1u << j;
                     }
-                    if (docs) {
-                        uint32_t same = 0;
+                    seen &= same;
+                }
+            }
+            const bool small = BENT && p.cap > 0.f && bend.all_small(s);
+            uint32_t wp[Op::kPlanes ? 3 : 1][16], ws[Op::kPlanes ? 3 : 1][16];
+#pragma unroll
+            for (int j = 0; j < 32; j += 2) {
+                f32x2 l2, d2;
+                if (KEYS) {
+                    l2 = *reinterpret_cast<const f32x2 *>(cols + 32 * h + j);
+                    d2 = *reinterpret_cast<const f32x2 *>(cols + 64 + 32 * h + j);
+                } else {
+                    l2 = pack2(less, less);
+                    d2 = pack2(less_delta, less_delta);
+                }
+                float2 x;
+                f32x2 b2 = pack2(1.f, 1.f);
+                if (BENT) {
+                    f32x2 y;
+                    if (p.cap > 0.f) {
+                        if (small) {
+                            y = bend.capped_small(pack2(s[j], s[j + 1]), &b2);
+                        } else {
+                            float da, dc;
+                            const float ya = bend.template capped<Op::kPlanes>(s[j], &da), yc = bend.template capped<Op::kPlanes>(s[j + 1], &dc);
+                            y = pack2(ya, yc);
+                            b2 = pack2(da, dc);
+                        }
+                    } else {
+                        y = mul2(pack2(s[j], s[j + 1]), scale2);
+                    }
+                    if (p.slopes) {
+                        float2 away, less;  // distances, and what they take from the scores
                         if (KEYS) {
-                            const int4 *ids = reinterpret_cast<const int4 *>(cols + 128 + 32 * h);
-#pragma unroll
-                            for (int j = 0; j < 8; ++j) {
-                                const int4 d = ids[j];
-                                same |= (uint32_t)(d.x == row.doc) << (4 * j) | (uint32_t)(d.y == row.doc) << (4 * j + 1) |
-                                        (uint32_t)(d.z == row.doc) << (4 * j + 2) | (uint32_t)(d.w == row.doc) << (4 * j + 3);
-                            }
+                            const int c = 32 * h + j;
+                            away = make_float2(fabsf(cols[256 + c] - (float)key), fabsf(cols[257 + c] - (float)key));
+                            less = make_float2(-cols[192 + c], -cols[193 + c]);
                         } else {
-                            const int *ids = p.doc_k + b * p.doc_k_sb + t0 + 32 * h;
-                            const int have = p.Tk - t0 - 32 * h;
-#pragma unroll
-                            for (int j = 0; j < 32; ++j) if (j < have && ids[j] == row.doc) same |= 1u << j;
+                            const float first = (float)(row.place - t0) - (float)(32 * h + j);
+                            away = make_float2(fabsf(first), fabsf(first - 1.f));
+                            less = make_float2(-row.slope, -row.slope);
                         }
-                        seen &= same;
+                        y = fma2(pack2(less.x, less.y), pack2(away.x, away.y), y);
                     }
+                    x = unpack2(add2(y, l2));
+                } else {
+                    x = unpack2(fma2(pack2(s[j], s[j + 1]), scale2, l2));
                 }
-                const bool small = BENT && p.cap > 0.f && bend.all_small(s);
-                uint32_t wp[Op::kPlanes ? 3 : 1][16], ws[Op::kPlanes ? 3 : 1][16];
+                float a = fast_exp2(x.x), c = fast_exp2(x.y);
+                f32x2 u = add2(pack2(gp[j], gp[j + 1]), d2);
+                if (!kBf16) u = mul2(u, unit2);
+                if (BENT) u = mul2(u, b2);
+                float2 ds = unpack2(mul2(pack2(a, c), u));
+                if (masked) {  // (by choice, not by a factor: what is masked may be anything)
+                    const bool sa = seen >> j & 1, sc = seen >> (j + 1) & 1;
+                    a = sa ? a : 0.f;
+                    c = sc ? c : 0.f;
+                    ds.x = sa ? ds.x : 0.f;
+                    ds.y = sc ? ds.y : 0.f;
+                }
+                if (KEYS) plane_words<T>(wp, j / 2, a, c);
+                plane_words<T>(ws, j / 2, ds.x, ds.y);
+            }
 #pragma unroll
-                for (int j = 0; j < 32; j += 2) {
-                    f32x2 l2, d2;
-                    if (KEYS) {
-                        l2 = *reinterpret_cast<const f32x2 *>(cols + 32 * h + j);
-                        d2 = *reinterpret_cast<const f32x2 *>(cols + 64 + 32 * h + j);
-                    } else {
-                        l2 = pack2(less, less);
-                        d2 = pack2(less_delta, less_delta);
-                    }
-                    float2 x;
-                    f32x2 b2 = pack2(1.f, 1.f);
-                    if (BENT) {
-                        f32x2 y;
-                        if (p.cap > 0.f) {
-                            if (small) {
-                                y = bend.capped_small(pack2(s[j], s[j + 1]), &b2);
-                            } else {
-                                float da, dc;
-                                const float ya = bend.template capped<Op::kPlanes>(s[j], &da), yc = bend.template capped<Op::kPlanes>(s[j + 1], &dc);
-                                y = pack2(ya, yc);
-                                b2 = pack2(da, dc);
-                            }
-                        } else {
-                            y = mul2(pack2(s[j], s[j + 1]), scale2);
-                        }
-                        if (p.slopes) {
-                            float2 away, less;  // distances, and what they take from the scores
-                            if (KEYS) {
-                                const int c = 32 * h + j;
-                                away = make_float2(fabsf(cols[256 + c] - (float)key), fabsf(cols[257 + c] - (float)key));
-                                less = make_float2(-cols[192 + c], -cols[193 + c]);
-                            } else {
-                                const float first = (float)(row.place - t0) - (float)(32 * h + j);
-                                away = make_float2(fabsf(first), fabsf(first - 1.f));
-                                less = make_float2(-row.slope, -row.slope);
-                            }
-                            y = fma2(pack2(less.x, less.y), pack2(away.x, away.y), y);
-                        }
-                        x = unpack2(add2(y, l2));
-                    } else {
-                        x = unpack2(fma2(pack2(s[j], s[j + 1]), scale2, l2));
-                    }
-                    float a = fast_exp2(x.x), c = fast_exp2(x.y);
-                    f32x2 u = add2(pack2(gp[j], gp[j + 1]), d2);
-                    if (!kBf16) u = mul2(u, unit2);
-                    if (BENT) u = mul2(u, b2);
-                    float2 ds = unpack2(mul2(pack2(a, c), u));
-                    if (masked) {  // (by choice, not by a factor: what is masked may be anything)
-                        const bool sa = seen >> j & 1, sc = seen >> (j + 1) & 1;
-                        a = sa ? a : 0.f;
-                        c = sc ? c : 0.f;
-                        ds.x = sa ? ds.x : 0.f;
-                        ds.y = sc ? ds.y : 0.f;
-                    }
-                    if (KEYS) plane_words<T>(wp, j / 2, a, c);
-                    plane_words<T>(ws, j / 2, ds.x, ds.y);
-                }
-#pragma unroll
-                for (int e = 0; e < (Op::kPlanes ? 3 : 1); ++e) {
-                    // (16-bit: over what these warps alone have read)
-                    const uint32_t half = Op::kPlanes ? 32 * e + 16 * h : 32 * h;
-                    if constexpr (KEYS) tmem_store16(at + L::kP + half, wp[e]);
-                    tmem_store16(at + L::kDS + half, ws[e]);
-                }
+            for (int e = 0; e < (Op::kPlanes ? 3 : 1); ++e) {
+                // (16-bit: over what these warps alone have read)
+                const uint32_t half = Op::kPlanes ? 32 * e + 16 * h : 32 * h;
+                if constexpr (KEYS) tmem_store16(at + L::kP + half, wp[e]);
+                tmem_store16(at + L::kDS + half, ws[e]);
             }
             tmem_stores_done();
             tmem_before_sync();

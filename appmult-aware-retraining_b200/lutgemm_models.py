@@ -6,12 +6,17 @@ widths 64/128/256/512, global average pool, linear classifier; cf. micronet+/mod
 `resnet50_imagenet` (7x7 stride-2 stem, max pool, bottleneck stages [3,4,6,3], 1000-way classifier) and
 `vit_small_16` (patch 16, 12 blocks, width 384, 6 heads, MLP 1536; attention scores and softmax stay exact
 fp32, the QKV / projection / MLP linears and the patch embedding are swapped) are the two larger
-configurations."""
+configurations.  With `attention="fused"` the exact part between the linears runs on this package's own kernels
+(`lutgemm_attention`), which also know what networks that are to be retrained with approximate linears are built with: norms of
+queries and keys per head (they bound the logits that the multipliers' errors reach), positions as rotations, capped logits, packed
+images, and a last block for the class token alone."""
 from __future__ import annotations
 
 import torch
 import torch.nn as nn
 import torch.nn.functional as F
+
+from lutgemm_attention import attention, norm_rotate, rotary_tables_2d
 
 
 class BasicBlock(nn.Module):
@@ -103,37 +108,88 @@ def resnet50_imagenet(num_classes: int = 1000, base: int = 64, blocks=(3, 4, 6, 
 
 
 class ViTBlock(nn.Module):
-    def __init__(self, dim: int, heads: int, mlp: int):
+    """`attention`: "library" (PyTorch's scaled_dot_product_attention) or "fused" (`lutgemm_attention`).  Fused only: `qk_norm`
+    gives queries and keys of every head a root-mean-square norm with weights, `logit_cap` caps the logits by a tanh,
+    `class_query` makes the block return its first token alone, the only one that a classifier's last block needs."""
+
+    def __init__(self, dim: int, heads: int, mlp: int, attention: str = "library", qk_norm: bool = False, logit_cap: float = 0.0,
+                 class_query: bool = False):
         super().__init__()
-        self.heads = heads
+        if attention not in ("library", "fused"):
+            raise ValueError(f"attention must be 'library' or 'fused', got {attention!r}")
+        if attention == "library" and (qk_norm or logit_cap or class_query):
+            raise ValueError("qk_norm, logit_cap and class_query belong to attention='fused'")
+        self.heads, self.attention, self.logit_cap, self.class_query = heads, attention, logit_cap, class_query
         self.norm1, self.norm2 = nn.LayerNorm(dim), nn.LayerNorm(dim)
         self.qkv, self.proj = nn.Linear(dim, 3 * dim), nn.Linear(dim, dim)
         self.fc1, self.fc2 = nn.Linear(dim, mlp), nn.Linear(mlp, dim)
+        self.q_norm = nn.Parameter(torch.ones(dim // heads)) if qk_norm else None
+        self.k_norm = nn.Parameter(torch.ones(dim // heads)) if qk_norm else None
 
-    def forward(self, x):
+    def forward(self, x, cos=None, sin=None, positions=None, documents=None):
+        """cos, sin, positions: rotation of queries and keys (with `qk_norm`); documents: int32 [B, T], see
+        `lutgemm_attention.attention`.  Both belong to the fused attention."""
         B, T, D = x.shape
-        q, k, v = self.qkv(self.norm1(x)).view(B, T, 3, self.heads, D // self.heads).permute(2, 0, 3, 1, 4)
-        a = F.scaled_dot_product_attention(q, k, v)  # exact fp32 scores and softmax
-        x = x + self.proj(a.transpose(1, 2).reshape(B, T, D))
+        if self.attention == "library":
+            if cos is not None or documents is not None:
+                raise ValueError("rotations and documents belong to attention='fused'")
+            q, k, v = self.qkv(self.norm1(x)).view(B, T, 3, self.heads, D // self.heads).permute(2, 0, 3, 1, 4)
+            a = F.scaled_dot_product_attention(q, k, v)  # exact fp32 scores and softmax
+            x = x + self.proj(a.transpose(1, 2).reshape(B, T, D))
+            return x + self.fc2(F.gelu(self.fc1(self.norm2(x))))
+        q, k, v = self.qkv(self.norm1(x)).view(B, T, 3, self.heads, D // self.heads).unbind(2)
+        if self.q_norm is not None:
+            q, k = norm_rotate(q, k, self.q_norm, self.k_norm, cos, sin, positions)
+        elif cos is not None:
+            raise ValueError("rotations belong to qk_norm")
+        asked = None
+        if self.class_query:
+            q, x = q[:, :1], x[:, :1]
+            asked = documents[:, :1] if documents is not None else None
+        a = attention(q, k, v, cap=self.logit_cap, documents=documents, query_documents=asked)
+        x = x + self.proj(a.reshape(B, -1, D))
         return x + self.fc2(F.gelu(self.fc1(self.norm2(x))))
 
 
 class ViT(nn.Module):
+    """`attention`, `qk_norm`, `logit_cap` as in `ViTBlock`; `rotary` (with `qk_norm`) turns queries and keys by their patch's row and
+    column, the class token not at all; `class_query` lets the last block work for the class token alone, whose linears and
+    their observers then see one row per image."""
+
     def __init__(self, image: int = 224, patch: int = 16, dim: int = 384, depth: int = 12, heads: int = 6,
-                 mlp: int = 1536, num_classes: int = 1000):
+                 mlp: int = 1536, num_classes: int = 1000, attention: str = "library", qk_norm: bool = False, rotary: bool = False,
+                 logit_cap: float = 0.0, class_query: bool = False):
         super().__init__()
+        if rotary and not qk_norm:
+            raise ValueError("rotary belongs to qk_norm")
         self.patch_embed = nn.Conv2d(3, dim, patch, patch, 0)
-        tokens = (image // patch) ** 2 + 1
+        side = image // patch
+        tokens = side ** 2 + 1
         self.cls = nn.Parameter(torch.zeros(1, 1, dim))
         self.pos = nn.Parameter(torch.randn(1, tokens, dim) * 0.02)
-        self.blocks = nn.Sequential(*[ViTBlock(dim, heads, mlp) for _ in range(depth)])
+        self.blocks = nn.Sequential(*[ViTBlock(dim, heads, mlp, attention, qk_norm, logit_cap, class_query and i == depth - 1)
+                                      for i in range(depth)])
         self.norm = nn.LayerNorm(dim)
         self.head = nn.Linear(dim, num_classes)
+        self.rotary = rotary
+        if rotary:
+            cos, sin = rotary_tables_2d(side, side, dim // heads)
+            self.register_buffer("cos", cos, persistent=False)
+            self.register_buffer("sin", sin, persistent=False)
+            self.register_buffer("place", torch.arange(tokens, dtype=torch.int32) - 1, persistent=False)
 
-    def forward(self, x):
+    def forward(self, x, documents=None):
+        """documents (fused attention): int32 [B, tokens], the class token first: a token attends to those of its own id, and none to
+        ids below zero (patches that are masked or lie beyond a smaller image)."""
         x = self.patch_embed(x).flatten(2).transpose(1, 2)
         x = torch.cat([self.cls.expand(x.shape[0], -1, -1), x], dim=1) + self.pos
-        return self.head(self.norm(self.blocks(x))[:, 0])
+        if not self.rotary and documents is None:
+            x = self.blocks(x)
+        else:
+            turn = (self.cos, self.sin, self.place.expand(x.shape[0], -1)) if self.rotary else (None, None, None)
+            for block in self.blocks:
+                x = block(x, *turn, documents)
+        return self.head(self.norm(x)[:, 0])
 
 
 def vit_small_16(num_classes: int = 1000, **kw) -> ViT:
