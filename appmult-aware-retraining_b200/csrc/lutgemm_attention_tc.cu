@@ -534,7 +534,7 @@ int attention_tc_forward(const AttnProblem &problem, int dtype, void *out, void 
     const bool bf16 = dtype != LUTGEMM_F16;
     const int width = dtype == LUTGEMM_F32 ? kPlaneWidth : p.D;
     if (!attention_map(&map_k, bf16, p.k, p.B, p.Tk, p.G, 1, width) || !attention_map(&map_v, bf16, p.v, p.B, p.Tk, p.G, 1, width))
-        return LUTGEMM_E_BADARG;
+        return LUTGEMM_E_CUDA;  // (no tensor maps on this driver)
     const int splits = key_splits(p, dtype, sms), dp = p.D <= 64 ? 64 : 128;
     const DocRange *kr, *rr;
     rc = doc_ranges(p, at, &kr, &rr, stream);

@@ -601,7 +601,7 @@ int gradients(const AttnProblem &p, const AttnTensor &go, const float *lse, cons
     CUtensorMap map_q, map_go, map_k, map_v;
     if (!attention_map(&map_q, Op::kBf16, p.q, p.B, p.Tq, p.G, p.R, width) || !attention_map(&map_go, Op::kBf16, go, p.B, p.Tq, p.G, p.R, width) ||
         !attention_map(&map_k, Op::kBf16, p.k, p.B, p.Tk, p.G, 1, width) || !attention_map(&map_v, Op::kBf16, p.v, p.B, p.Tk, p.G, 1, width))
-        return LUTGEMM_E_BADARG;
+        return LUTGEMM_E_CUDA;  // (no tensor maps on this driver)
     const bool bent = p.cap > 0.f || p.slopes;
     const int rc = bent ? launch<T, DP, true, true>(p, go, map_q, map_go, kr, rr, lse, delta, most, parts, gk, gv, error_word, stream)
                         : launch<T, DP, false, true>(p, go, map_q, map_go, kr, rr, lse, delta, most, parts, gk, gv, error_word, stream);
