@@ -19,7 +19,7 @@ from __future__ import annotations
 
 import contextlib
 import ctypes
-import functools
+import importlib.util
 import os
 
 import torch
@@ -114,27 +114,6 @@ def _load():
     lib.lutgemm_backward_f32lut_scratch_bytes.argtypes = [ci, ci, ci, ci]
     lib.lutgemm_backward_f32lut.restype = ci
     lib.lutgemm_backward_f32lut.argtypes = [vp, vp, vp, vp, vp, vp, vp, ci, ci, ci, ci, vp, sz, vp]
-    lib.lutgemm_norm_rotate.restype = ci
-    lib.lutgemm_norm_rotate.argtypes = [vp, cl, cl, cl] * 2 + [vp] * 4 + [ci] + [vp] * 3 + [ci] * 8 + [cf, vp]
-    lib.lutgemm_norm_rotate_backward_scratch_bytes.restype = sz
-    lib.lutgemm_norm_rotate_backward_scratch_bytes.argtypes = [ci]
-    lib.lutgemm_norm_rotate_backward.restype = ci
-    lib.lutgemm_norm_rotate_backward.argtypes = [vp, cl, cl, cl] * 4 + [vp] * 4 + [ci] + [vp] * 5 + [ci] * 8 + [cf, vp, sz, vp]
-    masks = [cf, cf, vp, ci, vp, vp, cl, vp, cl]
-    lib.lutgemm_attention.restype = ci
-    lib.lutgemm_attention.argtypes = [vp, cl, cl, cl] * 3 + [vp] * 3 + [ci] * 7 + masks + [vp, sz, vp]
-    lib.lutgemm_attention_scratch_bytes.restype = sz
-    lib.lutgemm_attention_scratch_bytes.argtypes = [ci] * 8
-    lib.lutgemm_attention_backward.restype = ci
-    lib.lutgemm_attention_backward.argtypes = [vp, cl, cl, cl] * 4 + [vp] * 6 + [ci] * 7 + masks + [vp, sz, vp]
-    lib.lutgemm_attention_backward_scratch_bytes.restype = sz
-    lib.lutgemm_attention_backward_scratch_bytes.argtypes = [ci] * 8
-    lib.lutgemm_token_logprobs_scratch_bytes.restype = sz
-    lib.lutgemm_token_logprobs_scratch_bytes.argtypes = [cl, ci, ci]
-    lib.lutgemm_token_logprobs.restype = ci
-    lib.lutgemm_token_logprobs.argtypes = [vp, ci, cl, cl, ci, vp, ctypes.c_longlong, ci] + [vp] * 6 + [sz, vp]
-    lib.lutgemm_token_logprobs_backward.restype = ci
-    lib.lutgemm_token_logprobs_backward.argtypes = [vp, ci, cl, cl, ci, vp, ctypes.c_longlong] + [vp] * 5
     lib.lutgemm_set_tma.restype = ci
     lib.lutgemm_set_tma.argtypes = [ci]
     lib.lutgemm_set_handover.restype = ci
@@ -147,6 +126,24 @@ def _load():
     lib.lutgemm_selftest_bounded_wait.argtypes = [vp]
     _lib = lib
     return lib
+
+
+def torch_operators():
+    """The extension module `lutgemm_torch` (raises if it has not been built)."""
+    global _torch_operators
+    if _torch_operators is None:
+        path = os.path.join(_HERE, "lutgemm_torch.so")
+        if not os.path.exists(path):
+            raise RuntimeError(f"{path} is missing: build it with `python {os.path.join(_HERE, 'build_ext.py')}` "
+                               "(there is no fallback path for these operators)")
+        spec = importlib.util.spec_from_file_location("lutgemm_torch", path)
+        module = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(module)
+        _torch_operators = module
+    return _torch_operators
+
+
+_torch_operators = None
 
 
 def library():
@@ -230,13 +227,6 @@ def _guard(device: torch.device):
 def _stream_ptr(device: torch.device) -> int:
     # (the handle itself: a stream object takes four microseconds to make)
     return torch._C._cuda_getCurrentRawStream(device.index)
-
-
-@functools.lru_cache(maxsize=4096)
-def _scratch_bytes(name: str, index: int, *sizes) -> int:
-    """Scratch bytes of an entry point for a problem of these sizes on CUDA device `index`, which is current: they depend on nothing
-    else, and asking the library takes a call."""
-    return getattr(_load(), name)(*sizes)
 
 
 def _backward_scratch(query, args, codes_t, dev):

@@ -1,15 +1,16 @@
-"""In-tree build of liblutgemm_b200.so (sm_100a only).
+"""In-tree build of liblutgemm_b200.so (sm_100a only) and of lutgemm_torch.so, the PyTorch operators over it.
 
     python appmult-aware-retraining_b200/build_ext.py [--force] [--verbose]
 
 Each .cu under csrc/ is compiled with nvcc for compute_100a/sm_100a and linked into one shared
-library next to this file.  nvcc cross-compiles without a GPU, so this also runs on a CPU-only box.
+library next to this file; lutgemm_torch.cpp is compiled against the installed PyTorch and linked to that library.  nvcc cross-compiles without a GPU, so this also runs on a CPU-only box.
 """
 from __future__ import annotations
 
 import os
 import subprocess
 import sys
+import threading
 from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
@@ -17,6 +18,8 @@ CSRC = os.path.join(HERE, "csrc")
 INCLUDE = os.path.join(os.path.dirname(HERE), "include")
 OBJ_DIR = os.path.join(HERE, "build")
 LIB = os.path.join(HERE, "liblutgemm_b200.so")
+TORCH_SRC = os.path.join(CSRC, "lutgemm_torch.cpp")
+TORCH_LIB = os.path.join(HERE, "lutgemm_torch.so")
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
@@ -50,16 +53,46 @@ def _compile(src: str, verbose: bool) -> str:
     return obj
 
 
+def _compile_torch(lib_ready) -> None:
+    """The extension module: compiled while the library's sources are, linked when it is there (`lib_ready`: waits for that)."""
+    import sysconfig
+
+    import torch
+    from torch.utils.cpp_extension import include_paths, library_paths
+
+    obj = os.path.join(OBJ_DIR, "torch_module.obj")  # (not .o: it is no part of the library)
+    cuda = os.environ.get("CUDA_HOME", "/usr/local/cuda")
+    includes = [INCLUDE, sysconfig.get_paths()["include"], os.path.join(cuda, "include"), *include_paths()]
+    flags = ["-O2", "-std=c++17", "-fPIC", "-DTORCH_EXTENSION_NAME=lutgemm_torch", "-DTORCH_API_INCLUDE_EXTENSION_H",
+             f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"]
+    res = subprocess.run(["g++", *flags, *(x for i in includes for x in ("-isystem", i)), "-c", TORCH_SRC, "-o", obj], capture_output=True,
+                         text=True)
+    if res.returncode != 0:
+        sys.stderr.write(res.stdout + res.stderr)
+        raise RuntimeError("g++ failed on lutgemm_torch.cpp")
+    lib_ready()
+    dirs = [HERE, *library_paths()]
+    subprocess.run(["g++", "-shared", "-o", TORCH_LIB + ".tmp", obj, *(f"-L{d}" for d in dirs), "-l:liblutgemm_b200.so", "-lc10", "-lc10_cuda",
+                    "-ltorch_cpu", "-ltorch", "-ltorch_python", "-Wl,-rpath,$ORIGIN"], check=True)
+    os.replace(TORCH_LIB + ".tmp", TORCH_LIB)
+
+
 def build(force: bool = False, verbose: bool = False) -> str:
     os.makedirs(OBJ_DIR, exist_ok=True)
-    if not force and os.path.exists(LIB) and os.path.getmtime(LIB) >= _deps_mtime():
+    newest = _deps_mtime()
+    if not force and all(os.path.exists(x) and os.path.getmtime(x) >= newest for x in (LIB, TORCH_LIB)):
         return LIB
     srcs = _sources()
-    with ThreadPoolExecutor(max_workers=min(8, len(srcs))) as ex:
-        objs = list(ex.map(lambda s: _compile(s, verbose), srcs))
-    cmd = ["nvcc", "-shared", "-o", LIB + ".tmp", *objs, "-lcudart"]
-    subprocess.run(cmd, check=True)
-    os.replace(LIB + ".tmp", LIB)
+    linked = threading.Event()
+    with ThreadPoolExecutor(max_workers=min(8, len(srcs)) + 1) as ex:
+        module = ex.submit(_compile_torch, linked.wait)
+        try:
+            objs = list(ex.map(lambda s: _compile(s, verbose), srcs))
+            subprocess.run(["nvcc", "-shared", "-o", LIB + ".tmp", *objs, "-lcudart"], check=True)
+            os.replace(LIB + ".tmp", LIB)
+        finally:
+            linked.set()
+        module.result()
     return LIB
 
 
