@@ -125,7 +125,7 @@ __device__ __forceinline__ void copy_row_tile(uint32_t dst, const AttnProblem &p
     const int c = thread & 7;
 #pragma unroll 4
     for (int n = 0; n < kRowTile / 16; ++n) {
-        const int r = (thread >> 3) + 16 * n, m = m0 + r, i = m / p.R;
+        const int r = (thread >> 3) + 16 * n, m = m0 + r, i = p.R == 1 ? m : m / p.R;
         const bool in = m < p.M && (!p.doc_q || p.doc_q[b * p.doc_q_sb + i] >= 0);
         const char *src = base + 2 * (i * t.st + (m - i * p.R) * t.sh) + 16 * c;
 #pragma unroll

@@ -70,29 +70,34 @@ __global__ void __launch_bounds__(256) attention_delta_kernel(const AttnProblem 
 //     they were copied, serve as row and as column operands)
 // Eight warps share a round, four with the first 32 columns and four with the others; one further warp issues the products and one
 // brings the tiles (when one warp did both, copies were asked for only behind the products of a round, which the queue of the
-// tensor cores lets go one by one: a round of 128-value heads took 3200 clocks for 1300 of products).  Heads of up to 64 values
-// leave room for two blocks on an SM; with larger ones the accumulators fill the tensor memory of an SM, and the block has two
-// groups of eight warps that take rounds in turn, each with its own S and gP.
+// tensor cores lets go one by one: a round of 128-value heads took 3200 clocks for 1300 of products).  There are two groups of
+// eight warps that take rounds in turn, each with its own S and gP, so that the products of one round run beside the exponentials
+// of another.  Heads of up to 64 values leave room for P and dS beside S and gP; the scores of a group's next round are then
+// formed as soon as it has this round's in registers.  Larger ones keep P over S and dS over gP.
 // fp16: P is kept 2^10 larger, and grad_o is taken in units of its largest value in this key head (a power of two), so that dS stays
 // out of fp16's subnormal range whatever the scale of the loss.
-// fp32: P and dS are split into planes as the operands were, and have tensor memory of their own; each round's sums start from zero and
-// are added up in registers while the next scores are formed (in the accumulators, what additions cut off came to 2e-5 of
-// the gradients of 4096 rows).  Its ring has one stage less.
+// fp32: P and dS are split into planes as the operands were; there is one group, and each round's sums start from zero and are added up
+// in registers (in the accumulators, what additions cut off came to 2e-5 of the gradients of 4096 rows).
 template <typename T, int DP, bool KEYS>
 struct GradLayout {
     using Op = Operand<T, DP>;
-    static constexpr int kBlocks = Op::kBlocks, kGroups = DP / 64, kStages = kGroups + (Op::kPlanes ? 1 : 2), kPerSm = DP == 64 && !Op::kPlanes ? 2 : 1;
+    static constexpr int kBlocks = Op::kBlocks, kGroups = Op::kPlanes ? 1 : 2, kStages = Op::kPlanes ? 2 : DP == 64 ? 6 : 4;
+    static constexpr bool kEarly = DP == 64;  // P and dS have room of their own
     static constexpr int kWorkers = 256 * kGroups, kThreads = kWorkers + 64, kSums = KEYS ? 2 : 1;
     static constexpr uint32_t kTile = 64 * kBlocks * 128, kX = 0, kY = 2 * kTile, kRing = 4 * kTile;  // a stage of the ring: x, y
     static constexpr uint32_t kCols = kRing + kStages * 2 * kTile;  // KEYS: for each stage -lse, -delta, documents, slopes and places of 64 rows
-    static constexpr uint32_t kBars = kCols + (KEYS ? kStages * 64 * 20 : 0), kBytes = kBars + 256;
-    // tensor memory of a group: S, gP and, over them or behind them, P and dS; then the sums
-    static constexpr uint32_t kP = Op::kPlanes ? 128 : 0, kDS = Op::kPlanes ? 224 : 64, kGroup = Op::kPlanes ? 320 : 128;
-    static constexpr uint32_t kAcc = kGroups * kGroup, kColumns = kAcc + kSums * DP <= 256 ? 256 : 512;
+    static constexpr uint32_t kBars = kCols + (KEYS ? kStages * 64 * 20 : 0), kBytes = kBars + 384;
+    // tensor memory of a group: S, gP and, behind them or over them, P and dS (64 values of 16 bits: 32 columns); then the sums
+    static constexpr uint32_t kP = kEarly ? 128 : 0, kDS = Op::kPlanes ? 224 : kEarly ? 160 : 64, kGroup = Op::kPlanes ? 320 : kEarly ? 192 : 128;
+    static constexpr uint32_t kAcc = kGroups * kGroup, kColumns = 512;
+    static_assert(kAcc + kSums * DP <= kColumns, "tensor memory");
+    // where a half of the columns of P or dS lies, and the operand of the i-th sixteen of them
+    __device__ static constexpr uint32_t half(int h) { return kEarly ? 16 * h : 32 * h; }
+    __device__ static constexpr uint32_t sixteen(int i) { return half(i >> 1) + 8 * (i & 1); }
 };
 
 template <typename T, int DP, bool BENT, bool KEYS>
-__global__ void __launch_bounds__(GradLayout<T, DP, KEYS>::kThreads, GradLayout<T, DP, KEYS>::kPerSm)
+__global__ void __launch_bounds__(GradLayout<T, DP, KEYS>::kThreads, 1)
     attention_tc_grad_kernel(const AttnProblem p, const AttnTensor go, const __grid_constant__ CUtensorMap map_x,
                              const __grid_constant__ CUtensorMap map_y, const DocRange *key_ranges, const DocRange *row_ranges,
                              const float *lse, const float *delta, const float *most, int most_parts, T *g1, T *g2, int *error_word) {
@@ -103,12 +108,14 @@ __global__ void __launch_bounds__(GradLayout<T, DP, KEYS>::kThreads, GradLayout<
     constexpr float kShift = kBf16 ? 0.f : 10.f;
     extern __shared__ __align__(1024) uint8_t smem[];
     const uint32_t base = smem_u32(smem), bars = base + L::kBars;
-    const uint32_t bar_s = bars, bar_p = bars + 16, bar_acc = bars + 32, bar_full = bars + 40, bar_empty = bars + 72;  // (four stages)
-    volatile int *abort_word = reinterpret_cast<int *>(smem + L::kBars + 104);
-    uint32_t *slot = reinterpret_cast<uint32_t *>(smem + L::kBars + 108);
-    volatile int *tiles = reinterpret_cast<int *>(smem + L::kBars + 112);  // of the last eight rounds begun; then how many there were
-    volatile int *brought = reinterpret_cast<int *>(smem + L::kBars + 148);  // of the stages
-    float *tops = reinterpret_cast<float *>(smem + L::kBars + 164);       // of the warps
+    // S and gP of a group are formed, are in registers (early), P and dS stand, their products are done (early); the ring
+    const uint32_t bar_s = bars, bar_l = bars + 16, bar_p = bars + 32, bar_acc = bars + 48, bar_full = bars + 64, bar_empty = bars + 112,
+                   bar_end = bars + 160;
+    volatile int *abort_word = reinterpret_cast<int *>(smem + L::kBars + 168);
+    uint32_t *slot = reinterpret_cast<uint32_t *>(smem + L::kBars + 172);
+    volatile int *tiles = reinterpret_cast<int *>(smem + L::kBars + 176);    // of the last eight rounds begun; then how many there were
+    volatile int *brought = reinterpret_cast<int *>(smem + L::kBars + 212);  // of the stages
+    float *tops = reinterpret_cast<float *>(smem + L::kBars + 236);          // of the workers' warps
     const int tid = threadIdx.x, warp = warp_index();
     int bid = blockIdx.x;
     const int g = bid % p.G;
@@ -122,66 +129,73 @@ __global__ void __launch_bounds__(GradLayout<T, DP, KEYS>::kThreads, GradLayout<
     const long stat0 = ((long)b * p.G + g) * p.M;
     if (tid == 0) {
         *abort_word = 0;
-        for (int i = 0; i < 2; ++i) {
+        for (int i = 0; i < G; ++i) {
             mbar_init(bar_s + 8 * i, 2);  // the products' arrival and the issuing lane's own, which orders what it wrote
+            mbar_init(bar_l + 8 * i, 256);
             mbar_init(bar_p + 8 * i, 256);
+            mbar_init(bar_acc + 8 * i, 1);
         }
-        mbar_init(bar_acc, 1);
         for (int i = 0; i < L::kStages; ++i) {
             mbar_init(bar_full + 8 * i, 1);
             mbar_init(bar_empty + 8 * i, 1);
         }
+        mbar_init(bar_end, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    // fp16: the unit of grad_o, 2^unit >= its largest value
-    float unit = 1.f;
-    if (!kBf16) {
-        float top = 0.f;
-        for (int i = tid; i < most_parts; i += L::kThreads) top = fmaxf(top, most[((long)b * p.G + g) * most_parts + i]);
-#pragma unroll
-        for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-        if ((tid & 31) == 0) tops[warp] = top;
-    }
-    if (warp == 8 * G) tmem_alloc(smem_u32(slot), L::kColumns);
     if (KEYS && size < 64) {  // rows of a tile that bulk copies never write
         for (int i = tid; i < (int)(L::kStages * 2 * L::kTile / 16); i += L::kThreads)
             *reinterpret_cast<uint4 *>(smem + L::kRing + 16 * i) = make_uint4(0, 0, 0, 0);
         writes_to_tensor_cores();
     }
-    if (warp < 8) {  // X by four warps, Y by four
-        const bool y = warp >= 4;
-        const uint32_t to = base + (y ? L::kY : L::kX);
-        if (KEYS) {
-            // (like rows of one head)
-            AttnProblem keys = p;
-            keys.M = p.Tk;
-            keys.R = 1;
-            keys.doc_q = p.doc_k;
-            keys.doc_q_sb = p.doc_k_sb;
-            copy_row_tile<L::kBlocks>(to, keys, y ? p.v : p.k, width, b, g, o0, tid & 127);
-        } else {
-            copy_row_tile<L::kBlocks>(to, p, y ? go : p.q, width, b, g, o0, tid & 127);
-        }
-        copies_end_group();
-        copies_wait<0>();
-        writes_to_tensor_cores();
-    }
     __syncthreads();
-    tmem_after_sync();
-    const uint32_t tmem = *slot;
-    if (!kBf16) {
-        float top = 0.f;
+    // (the warp that brings tiles begins at once; the others meet again when X and Y have come)
+    float unit = 1.f;  // fp16: the unit of grad_o, a power of two above its largest value
+    uint32_t tmem = 0;
+    if (warp <= L::kWorkers / 32) {
+        if (warp == L::kWorkers / 32) tmem_alloc(smem_u32(slot), L::kColumns);
+        if (!kBf16 && warp < L::kWorkers / 32) {
+            float top = 0.f;
+            for (int i = tid; i < most_parts; i += L::kWorkers) top = fmaxf(top, most[((long)b * p.G + g) * most_parts + i]);
 #pragma unroll
-        for (int w = 0; w < L::kThreads / 32; ++w) top = fmaxf(top, tops[w]);
-        // (an infinite or NaN gradient, or none at all: as it is)
-        const int e = (int)(__float_as_uint(top) >> 23);
-        if (e > 0 && e < 254) unit = __uint_as_float((uint32_t)(e + 1) << 23);
+            for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+            if ((tid & 31) == 0) tops[warp] = top;
+        }
+        if (warp < 8) {  // X by four warps, Y by four
+            const bool y = warp >= 4;
+            const uint32_t to = base + (y ? L::kY : L::kX);
+            if (KEYS) {
+                // (like rows of one head)
+                AttnProblem keys = p;
+                keys.M = p.Tk;
+                keys.R = 1;
+                keys.doc_q = p.doc_k;
+                keys.doc_q_sb = p.doc_k_sb;
+                copy_row_tile<L::kBlocks>(to, keys, y ? p.v : p.k, width, b, g, o0, tid & 127);
+            } else {
+                copy_row_tile<L::kBlocks>(to, p, y ? go : p.q, width, b, g, o0, tid & 127);
+            }
+            copies_end_group();
+            copies_wait<0>();
+            writes_to_tensor_cores();
+        }
+        tmem_before_sync();
+        asm volatile("bar.sync 1, %0;" ::"n"(L::kWorkers + 32) : "memory");
+        tmem_after_sync();
+        tmem = *slot;
+        if (!kBf16) {
+            float top = 0.f;
+#pragma unroll
+            for (int w = 0; w < L::kWorkers / 32; ++w) top = fmaxf(top, tops[w]);
+            // (an infinite or NaN gradient, or none at all: as it is)
+            const int e = (int)(__float_as_uint(top) >> 23);
+            if (e > 0 && e < 254) unit = __uint_as_float((uint32_t)(e + 1) << 23);
+        }
     }
 
     // of the workers: the round group, the half of a round's columns, the row
     const int group = warp >> 3, h = warp >> 2 & 1, r = tid & 127;
     f32x2 sums[Op::kPlanes ? 16 * L::kSums : 1] = {};  // fp32: the worker's half of its row's sums
-    if (warp == 8 * G + 1) {  // brings the tiles
+    if (warp == L::kWorkers / 32 + 1) {  // brings the tiles
         const int lane = tid & 31;
         TileWalk walk;
         if (KEYS) {
@@ -260,7 +274,7 @@ __global__ void __launch_bounds__(GradLayout<T, DP, KEYS>::kThreads, GradLayout<
             __syncwarp();
             if (tile < 0 || *abort_word) break;
         }
-    } else if (warp == 8 * G) {  // issues the products
+    } else if (warp == L::kWorkers / 32) {  // issues the products
         const int lane = tid & 31;
         constexpr uint32_t desc_s = mma_descriptor(kBf16, 64, false), desc_acc = mma_descriptor(kBf16, DP, true);
         // the tile of round n when it has come; -1: there is none
@@ -320,45 +334,87 @@ __global__ void __launch_bounds__(GradLayout<T, DP, KEYS>::kThreads, GradLayout<
             if (elect_one()) issue_scores(i, ahead[i]);
             __syncwarp();
         }
-        int n = 0;
-        for (; ahead[0] >= 0; ++n) {
+        auto next_scores = [&](int n) {  // those of the round G behind n, where n's are in registers
             const int tile = arrived(n + G, ahead[G - 1] >= 0);
-            mbar_wait(bar_p + 8 * (n % G), n / G & 1, 213, abort_word, error_word);
-            tmem_after_sync();
-            __syncwarp();
-            if (elect_one()) {
-                const uint32_t d = tmem + n % G * L::kGroup;
-                const uint64_t x = smem_descriptor(base + L::kRing + n % L::kStages * 2 * L::kTile, Op::kPlanes ? 0 : 64 * 128);
-#pragma unroll
-                for (int e = 0; e < L::kSums; ++e) {  // grad_v with KEYS, then grad_k or grad_q
-                    const bool first = KEYS && e == 0;
-                    const uint32_t from = d + (first ? L::kP : L::kDS);
-                    const uint64_t with = descriptor_at(x, first ? L::kTile : 0);
-                    if constexpr (Op::kPlanes) {
-#pragma unroll
-                        for (int i = 0; i < 4 * Op::kProducts; ++i)
-                            mma_ts(tmem + L::kAcc + e * DP, from + 32 * Op::a(i >> 2) + 8 * (i & 3),
-                                   descriptor_at(with, Op::b(i >> 2) * 64 * 128 + (i & 3) * 16 * 128), desc_acc, i > 0);
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                            mma_ts(tmem + L::kAcc + e * DP, from + 32 * (i >> 1) + 8 * (i & 1),
-                                   descriptor_at(with, i * 16 * 128), desc_acc, n > 0 || i > 0);
-                    }
-                }
-                mma_commit(bar_empty + 8 * (n % L::kStages));
-                if (Op::kPlanes) mma_commit(bar_acc);
-                issue_scores(n + G, tile);
-            }
-            __syncwarp();
+            if (L::kEarly && ahead[0] >= 0) mbar_wait(bar_l + 8 * (n % G), n / G & 1, 217, abort_word, error_word);
+            return tile;
+        };
+        auto advance = [&](int tile) {
 #pragma unroll
             for (int i = 0; i + 1 < G; ++i) ahead[i] = ahead[i + 1];
             ahead[G - 1] = tile;
-        }
-        if (n > 0) {  // (fp32: the workers have waited for all rounds but the last)
-            if (!Op::kPlanes && elect_one()) mma_commit(bar_acc);
+        };
+        auto issue_sums = [&](int n) {
+            const uint32_t d = tmem + n % G * L::kGroup;
+            const uint64_t x = smem_descriptor(base + L::kRing + n % L::kStages * 2 * L::kTile, Op::kPlanes ? 0 : 64 * 128);
+#pragma unroll
+            for (int e = 0; e < L::kSums; ++e) {  // grad_v with KEYS, then grad_k or grad_q
+                const bool first = KEYS && e == 0;
+                const uint32_t from = d + (first ? L::kP : L::kDS);
+                const uint64_t with = descriptor_at(x, first ? L::kTile : 0);
+                if constexpr (Op::kPlanes) {
+#pragma unroll
+                    for (int i = 0; i < 4 * Op::kProducts; ++i)
+                        mma_ts(tmem + L::kAcc + e * DP, from + 32 * Op::a(i >> 2) + L::sixteen(i & 3),
+                               descriptor_at(with, Op::b(i >> 2) * 64 * 128 + (i & 3) * 16 * 128), desc_acc, i > 0);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        mma_ts(tmem + L::kAcc + e * DP, from + L::sixteen(i), descriptor_at(with, i * 16 * 128), desc_acc, n > 0 || i > 0);
+                }
+            }
+            mma_commit(bar_empty + 8 * (n % L::kStages));
+            if (L::kEarly) mma_commit(bar_acc + 8 * (n % G));
+        };
+        int n = 0;
+        if constexpr (L::kEarly && G == 2) {
+            // scores of round n + 3 before the sums of round n: the other group has had its scores in registers for long
+            int now = ahead[0], tile = next_scores(0);
+            tmem_after_sync();
             __syncwarp();
-            mbar_wait(bar_acc, Op::kPlanes ? (n - 1) & 1 : 0, 214, abort_word, error_word);
+            if (now >= 0 && elect_one()) issue_scores(G, tile);
+            __syncwarp();
+            for (; now >= 0; ++n) {
+                const int then = ahead[1];  // round n + 1
+                advance(tile);
+                if (then >= 0) {
+                    tile = next_scores(n + 1);
+                    tmem_after_sync();
+                    __syncwarp();
+                    if (elect_one()) issue_scores(n + 1 + G, tile);
+                    __syncwarp();
+                }
+                mbar_wait(bar_p + 8 * (n % G), n / G & 1, 213, abort_word, error_word);
+                tmem_after_sync();
+                __syncwarp();
+                if (elect_one()) issue_sums(n);
+                __syncwarp();
+                now = then;
+            }
+        } else {
+            for (; ahead[0] >= 0; ++n) {
+                const int tile = next_scores(n);
+                if (L::kEarly) {
+                    tmem_after_sync();
+                    __syncwarp();
+                    if (elect_one()) issue_scores(n + G, tile);
+                    __syncwarp();
+                }
+                mbar_wait(bar_p + 8 * (n % G), n / G & 1, 213, abort_word, error_word);
+                tmem_after_sync();
+                __syncwarp();
+                if (elect_one()) {
+                    issue_sums(n);
+                    if (!L::kEarly) issue_scores(n + G, tile);
+                }
+                __syncwarp();
+                advance(tile);
+            }
+        }
+        if (n > 0) {  // every product is done
+            if (elect_one()) mma_commit(bar_end);
+            __syncwarp();
+            mbar_wait(bar_end, 0, 214, abort_word, error_word);
         }
         if (lane == 0) tiles[8] = n;  // rounds done
     } else {
@@ -383,28 +439,32 @@ __global__ void __launch_bounds__(GradLayout<T, DP, KEYS>::kThreads, GradLayout<
             less_delta = o0 + r < p.M ? -delta[stat0 + o0 + r] : 0.f;
         }
         const bool idle = __all_sync(0xffffffffu, KEYS ? from == 0x7fffffff : row.limit < 0);
-        for (int n = group;; n += G) {
-            if constexpr (Op::kPlanes) {
-                if (n > 0) {
-                    mbar_wait(bar_acc, (n - 1) & 1, 217, abort_word, error_word);
-                    tmem_after_sync();
+        // fp32: the sums of a round, which are done
+        auto add_sums = [&](int n) {
+            mbar_wait(bar_acc, n & 1, 218, abort_word, error_word);
+            tmem_after_sync();
 #pragma unroll
-                    for (int c = 0; c < L::kSums; ++c) {
-                        float v[32];
-                        tmem_load32(mine + L::kAcc + 32 * (L::kSums * h + c), v);
-                        tmem_loads_done();
+            for (int c = 0; c < L::kSums; ++c) {
+                float v[32];
+                tmem_load32(mine + L::kAcc + 32 * (L::kSums * h + c), v);
+                tmem_loads_done();
 #pragma unroll
-                        for (int j = 0; j < 16; ++j) sums[16 * c + j] = add2(sums[16 * c + j], pack2(v[2 * j], v[2 * j + 1]));
-                    }
-                    tmem_before_sync();
-                }
+                for (int j = 0; j < 16; ++j) sums[Op::kPlanes ? 16 * c + j : 0] = add2(sums[Op::kPlanes ? 16 * c + j : 0], pack2(v[2 * j], v[2 * j + 1]));
             }
+        };
+        int n = group;
+        for (;; n += G) {
             mbar_wait(bar_s + 8 * group, n / G & 1, 215, abort_word, error_word);
             const int tile = tiles[n & 7];
             if (tile < 0 || *abort_word) break;
             tmem_after_sync();
             const uint32_t at = mine + group * L::kGroup;
             if (idle) {
+                if (L::kEarly) {
+                    mbar_arrive(bar_l + 8 * group);
+                    // (not ahead of the others: an arrival before their last round's would be taken for that)
+                    if (n >= G) mbar_wait(bar_acc + 8 * group, (n / G - 1) & 1, 220, abort_word, error_word);
+                }
                 mbar_arrive(bar_p + 8 * group);
                 continue;
             }
@@ -416,6 +476,11 @@ __global__ void __launch_bounds__(GradLayout<T, DP, KEYS>::kThreads, GradLayout<
             tmem_load32(at + 32 * h, s);
             tmem_load32(at + 64 + 32 * h, gp);
             tmem_loads_done();
+            if (L::kEarly) {
+                tmem_before_sync();
+                mbar_arrive(bar_l + 8 * group);
+            }
+            if (Op::kPlanes && n > 0) add_sums(n - 1);
             // which of the 32 are seen
             uint32_t seen = 0xffffffffu;
             if (masked) {
@@ -505,23 +570,24 @@ __global__ void __launch_bounds__(GradLayout<T, DP, KEYS>::kThreads, GradLayout<
                 if (KEYS) plane_words<T>(wp, j / 2, a, c);
                 plane_words<T>(ws, j / 2, ds.x, ds.y);
             }
+            // the products of this group's last round are done (fp32: have been waited for)
+            if (L::kEarly && !Op::kPlanes && n >= G) mbar_wait(bar_acc + 8 * group, (n / G - 1) & 1, 219, abort_word, error_word);
 #pragma unroll
             for (int e = 0; e < (Op::kPlanes ? 3 : 1); ++e) {
-                // (16-bit: over what these warps alone have read)
-                const uint32_t half = Op::kPlanes ? 32 * e + 16 * h : 32 * h;
-                if constexpr (KEYS) tmem_store16(at + L::kP + half, wp[e]);
-                tmem_store16(at + L::kDS + half, ws[e]);
+                if constexpr (KEYS) tmem_store16(at + L::kP + 32 * e + L::half(h), wp[e]);
+                tmem_store16(at + L::kDS + 32 * e + L::half(h), ws[e]);
             }
             tmem_stores_done();
             tmem_before_sync();
             mbar_arrive(bar_p + 8 * group);
         }
+        if (Op::kPlanes && n > 0) add_sums(n - 1);
     }
     settle(abort_word);
     tmem_before_sync();
     __syncthreads();
     tmem_after_sync();
-    if (warp < 8 * G) {
+    if (warp < L::kWorkers / 32) {
         const int rounds = tiles[8], o = o0 + r;
         const bool in = o < (KEYS ? p.Tk : p.M);
         bool real = in && rounds > 0;
@@ -573,7 +639,7 @@ __global__ void __launch_bounds__(GradLayout<T, DP, KEYS>::kThreads, GradLayout<
         tmem_before_sync();
     }
     __syncthreads();
-    if (warp == 8 * G) {
+    if (warp == L::kWorkers / 32) {
         tmem_after_sync();
         tmem_free(tmem, L::kColumns);
     }
