@@ -73,7 +73,10 @@ __global__ void __launch_bounds__(256) attention_delta_kernel(const AttnProblem 
 // tensor cores lets go one by one: a round of 128-value heads took 3200 clocks for 1300 of products).  There are two groups of
 // eight warps that take rounds in turn, each with its own S and gP, so that the products of one round run beside the exponentials
 // of another.  Heads of up to 64 values leave room for P and dS beside S and gP; the scores of a group's next round are then
-// formed as soon as it has this round's in registers.  Larger ones keep P over S and dS over gP.
+// formed as soon as it has this round's in registers, and another warp issues the sums (one warp for both spent half of its
+// rounds on waits that had long been over).  Larger ones keep P over S and dS over gP.
+// Results go through shared memory, which the ring has left, so that whole rows are written (a row to a thread took 6000 clocks of
+// a block of 16000 where there are 197 keys).
 // fp16: P is kept 2^10 larger, and grad_o is taken in units of its largest value in this key head (a power of two), so that dS stays
 // out of fp16's subnormal range whatever the scale of the loss.
 // fp32: P and dS are split into planes as the operands were; there is one group, and each round's sums start from zero and are added up
@@ -82,8 +85,8 @@ template <typename T, int DP, bool KEYS>
 struct GradLayout {
     using Op = Operand<T, DP>;
     static constexpr int kBlocks = Op::kBlocks, kGroups = Op::kPlanes ? 1 : 2, kStages = Op::kPlanes ? 2 : DP == 64 ? 6 : 4;
-    static constexpr bool kEarly = DP == 64;  // P and dS have room of their own
-    static constexpr int kWorkers = 256 * kGroups, kThreads = kWorkers + 64, kSums = KEYS ? 2 : 1;
+    static constexpr bool kEarly = DP == 64;  // P and dS have room of their own; a warp for the scores and one for the sums
+    static constexpr int kWorkers = 256 * kGroups, kThreads = kWorkers + (kEarly ? 96 : 64), kSums = KEYS ? 2 : 1;
     static constexpr uint32_t kTile = 64 * kBlocks * 128, kX = 0, kY = 2 * kTile, kRing = 4 * kTile;  // a stage of the ring: x, y
     static constexpr uint32_t kCols = kRing + kStages * 2 * kTile;  // KEYS: for each stage -lse, -delta, documents, slopes and places of 64 rows
     static constexpr uint32_t kBars = kCols + (KEYS ? kStages * 64 * 20 : 0), kBytes = kBars + 384;
@@ -115,7 +118,8 @@ __global__ void __launch_bounds__(GradLayout<T, DP, KEYS>::kThreads, 1)
     uint32_t *slot = reinterpret_cast<uint32_t *>(smem + L::kBars + 172);
     volatile int *tiles = reinterpret_cast<int *>(smem + L::kBars + 176);    // of the last eight rounds begun; then how many there were
     volatile int *brought = reinterpret_cast<int *>(smem + L::kBars + 212);  // of the stages
-    float *tops = reinterpret_cast<float *>(smem + L::kBars + 236);          // of the workers' warps
+    volatile int *rounds_seen = reinterpret_cast<int *>(smem + L::kBars + 236);  // how many there are, once that is known
+    float *tops = reinterpret_cast<float *>(smem + L::kBars + 240);          // of the workers' warps
     const int tid = threadIdx.x, warp = warp_index();
     int bid = blockIdx.x;
     const int g = bid % p.G;
@@ -129,6 +133,7 @@ __global__ void __launch_bounds__(GradLayout<T, DP, KEYS>::kThreads, 1)
     const long stat0 = ((long)b * p.G + g) * p.M;
     if (tid == 0) {
         *abort_word = 0;
+        *rounds_seen = 0x7fffffff;
         for (int i = 0; i < G; ++i) {
             mbar_init(bar_s + 8 * i, 2);  // the products' arrival and the issuing lane's own, which orders what it wrote
             mbar_init(bar_l + 8 * i, 256);
@@ -151,7 +156,7 @@ __global__ void __launch_bounds__(GradLayout<T, DP, KEYS>::kThreads, 1)
     // (the warp that brings tiles begins at once; the others meet again when X and Y have come)
     float unit = 1.f;  // fp16: the unit of grad_o, a power of two above its largest value
     uint32_t tmem = 0;
-    if (warp <= L::kWorkers / 32) {
+    if (warp != L::kWorkers / 32 + 1) {
         if (warp == L::kWorkers / 32) tmem_alloc(smem_u32(slot), L::kColumns);
         if (!kBf16 && warp < L::kWorkers / 32) {
             float top = 0.f;
@@ -179,7 +184,7 @@ __global__ void __launch_bounds__(GradLayout<T, DP, KEYS>::kThreads, 1)
             writes_to_tensor_cores();
         }
         tmem_before_sync();
-        asm volatile("bar.sync 1, %0;" ::"n"(L::kWorkers + 32) : "memory");
+        asm volatile("bar.sync 1, %0;" ::"n"(L::kThreads - 32) : "memory");
         tmem_after_sync();
         tmem = *slot;
         if (!kBf16) {
@@ -197,6 +202,11 @@ __global__ void __launch_bounds__(GradLayout<T, DP, KEYS>::kThreads, 1)
     f32x2 sums[Op::kPlanes ? 16 * L::kSums : 1] = {};  // fp32: the worker's half of its row's sums
     if (warp == L::kWorkers / 32 + 1) {  // brings the tiles
         const int lane = tid & 31;
+        if (elect_one()) {
+            tma_prefetch_map(&map_x);
+            tma_prefetch_map(&map_y);
+        }
+        __syncwarp();
         TileWalk walk;
         if (KEYS) {
             const int last = min(o0 + 128, p.Tk) - 1;
@@ -274,7 +284,7 @@ __global__ void __launch_bounds__(GradLayout<T, DP, KEYS>::kThreads, 1)
             __syncwarp();
             if (tile < 0 || *abort_word) break;
         }
-    } else if (warp == L::kWorkers / 32) {  // issues the products
+    } else if (warp >= L::kWorkers / 32) {  // issue the products
         const int lane = tid & 31;
         constexpr uint32_t desc_s = mma_descriptor(kBf16, 64, false), desc_acc = mma_descriptor(kBf16, DP, true);
         // the tile of round n when it has come; -1: there is none
@@ -326,24 +336,6 @@ __global__ void __launch_bounds__(GradLayout<T, DP, KEYS>::kThreads, 1)
             }
             mbar_arrive(bar);
         };
-        int ahead[G];  // tiles of the rounds that have begun
-#pragma unroll
-        for (int i = 0; i < G; ++i) {
-            ahead[i] = arrived(i, i == 0 || ahead[i > 0 ? i - 1 : 0] >= 0);
-            __syncwarp();
-            if (elect_one()) issue_scores(i, ahead[i]);
-            __syncwarp();
-        }
-        auto next_scores = [&](int n) {  // those of the round G behind n, where n's are in registers
-            const int tile = arrived(n + G, ahead[G - 1] >= 0);
-            if (L::kEarly && ahead[0] >= 0) mbar_wait(bar_l + 8 * (n % G), n / G & 1, 217, abort_word, error_word);
-            return tile;
-        };
-        auto advance = [&](int tile) {
-#pragma unroll
-            for (int i = 0; i + 1 < G; ++i) ahead[i] = ahead[i + 1];
-            ahead[G - 1] = tile;
-        };
         auto issue_sums = [&](int n) {
             const uint32_t d = tmem + n % G * L::kGroup;
             const uint64_t x = smem_descriptor(base + L::kRing + n % L::kStages * 2 * L::kTile, Op::kPlanes ? 0 : 64 * 128);
@@ -367,48 +359,64 @@ __global__ void __launch_bounds__(GradLayout<T, DP, KEYS>::kThreads, 1)
             if (L::kEarly) mma_commit(bar_acc + 8 * (n % G));
         };
         int n = 0;
-        if constexpr (L::kEarly && G == 2) {
-            // scores of round n + 3 before the sums of round n: the other group has had its scores in registers for long
-            int now = ahead[0], tile = next_scores(0);
-            tmem_after_sync();
-            __syncwarp();
-            if (now >= 0 && elect_one()) issue_scores(G, tile);
-            __syncwarp();
-            for (; now >= 0; ++n) {
-                const int then = ahead[1];  // round n + 1
-                advance(tile);
-                if (then >= 0) {
-                    tile = next_scores(n + 1);
-                    tmem_after_sync();
-                    __syncwarp();
-                    if (elect_one()) issue_scores(n + 1 + G, tile);
-                    __syncwarp();
-                }
-                mbar_wait(bar_p + 8 * (n % G), n / G & 1, 213, abort_word, error_word);
+        if (!L::kEarly) {
+            int ahead[G];  // tiles of the rounds that have begun
+#pragma unroll
+            for (int i = 0; i < G; ++i) {
+                ahead[i] = arrived(i, i == 0 || ahead[i > 0 ? i - 1 : 0] >= 0);
                 tmem_after_sync();
                 __syncwarp();
-                if (elect_one()) issue_sums(n);
+                if (elect_one()) issue_scores(i, ahead[i]);
                 __syncwarp();
-                now = then;
             }
-        } else {
             for (; ahead[0] >= 0; ++n) {
-                const int tile = next_scores(n);
-                if (L::kEarly) {
-                    tmem_after_sync();
-                    __syncwarp();
-                    if (elect_one()) issue_scores(n + G, tile);
-                    __syncwarp();
-                }
+                const int tile = arrived(n + G, ahead[G - 1] >= 0);
                 mbar_wait(bar_p + 8 * (n % G), n / G & 1, 213, abort_word, error_word);
                 tmem_after_sync();
                 __syncwarp();
                 if (elect_one()) {
                     issue_sums(n);
-                    if (!L::kEarly) issue_scores(n + G, tile);
+                    issue_scores(n + G, tile);
                 }
                 __syncwarp();
-                advance(tile);
+#pragma unroll
+                for (int i = 0; i + 1 < G; ++i) ahead[i] = ahead[i + 1];
+                ahead[G - 1] = tile;
+            }
+        } else if (warp == L::kWorkers / 32) {  // the scores
+            constexpr int kUnknown = 1 << 30;  // (there are at most 2^25 tiles)
+            int last = kUnknown;
+            for (int k = 0; k < last + G; ++k) {
+                const int tile = arrived(k, last == kUnknown);
+                if (tile < 0 && last == kUnknown) last = k;
+                if (k >= G && k - G < last) mbar_wait(bar_l + 8 * (k % G), (k / G - 1) & 1, 217, abort_word, error_word);
+                if (k == last && k >= G) {
+                    // Word of the end goes to the sums in place of the workers' arrivals, when those of the group's last round are all
+                    // there and the sums have taken note of them: a barrier's parity tells two phases apart, not three.  (The
+                    // first wait makes the second one sure of its phase.)
+                    mbar_wait(bar_p + 8 * (k % G), (k / G - 1) & 1, 221, abort_word, error_word);
+                    mbar_wait(bar_acc + 8 * (k % G), (k / G - 1) & 1, 222, abort_word, error_word);
+                }
+                tmem_after_sync();
+                __syncwarp();
+                if (elect_one()) {
+                    issue_scores(k, tile);
+                    if (k == last) {
+                        *rounds_seen = k;
+                        mbar_arrive_many(bar_p + 8 * (k % G), 256);
+                    }
+                }
+                __syncwarp();
+                if (*abort_word) break;
+            }
+        } else {  // the sums
+            for (;; ++n) {
+                mbar_wait(bar_p + 8 * (n % G), n / G & 1, 213, abort_word, error_word);
+                if (n >= *rounds_seen || *abort_word) break;
+                tmem_after_sync();
+                __syncwarp();
+                if (elect_one()) issue_sums(n);
+                __syncwarp();
             }
         }
         if (n > 0) {  // every product is done
@@ -416,7 +424,7 @@ __global__ void __launch_bounds__(GradLayout<T, DP, KEYS>::kThreads, 1)
             __syncwarp();
             mbar_wait(bar_end, 0, 214, abort_word, error_word);
         }
-        if (lane == 0) tiles[8] = n;  // rounds done
+        if (lane == 0 && (!L::kEarly || warp != L::kWorkers / 32)) tiles[8] = n;  // rounds done
     } else {
         const uint32_t mine = tmem + ((uint32_t)((warp & 3) * 32) << 16);
         const Bend bend = make_bend<Op::kPlanes>(p);
@@ -593,10 +601,10 @@ __global__ void __launch_bounds__(GradLayout<T, DP, KEYS>::kThreads, 1)
         bool real = in && rounds > 0;
         if (in && docs) real = real && (KEYS ? p.doc_k[b * p.doc_k_sb + o] : p.doc_q[b * p.doc_q_sb + o / p.R]) >= 0;
         if (!KEYS && in && lse[stat0 + o] == INFINITY) real = false;  // a row that sees nothing
-        const int i = KEYS ? o : o / p.R, head = KEYS ? g : g * p.R + o - i * p.R;
-        const long to = (((long)b * (KEYS ? p.Tk : p.Tq) + i) * (KEYS ? p.G : p.H) + head) * p.D;
         const float f1 = kBf16 ? 1.f : 1.f / 1024.f, f2 = kBf16 ? p.scale : p.scale * unit;
         constexpr int kChunks = L::kSums * DP / 32, kOwn = (kChunks + 2 * G - 1) / (2 * G);  // 32 columns each
+        constexpr int kPieces = DP * (int)sizeof(T) / 16;  // of 16 bytes, of a row; piece c of row r lies at c ^ (r & 7)
+        uint8_t *stage = smem + L::kRing;                  // grad_q or grad_k, then grad_v
 #pragma unroll
         for (int k = 0; k < kOwn; ++k) {
             const int c = kOwn * (2 * group + h) + k;
@@ -615,28 +623,31 @@ __global__ void __launch_bounds__(GradLayout<T, DP, KEYS>::kThreads, 1)
             }
             const bool second = KEYS && c < DP / 32;  // grad_v
             const int d0 = (second || !KEYS ? c : c - DP / 32) * 32;
-            T *dst = second ? g2 : g1;
             const float f = second ? f1 : f2;
-            if (in)
+            uint4 *row_out = reinterpret_cast<uint4 *>(stage) + ((second ? 128 : 0) + r) * kPieces;
+            constexpr int kPer = 16 / (int)sizeof(T);  // values of a piece
 #pragma unroll
-                for (int j = 0; j < 32; j += 8) {
-                    if (d0 + j >= p.D) break;
-                    if constexpr (Op::kPlanes) {
+            for (int j = 0; j < 32; j += kPer) {
+                uint4 w;
+                uint32_t *q = &w.x;
 #pragma unroll
-                        for (int e = 0; e < 8; e += 4)
-                            *reinterpret_cast<float4 *>(dst + to + d0 + j + e) =
-                                real ? make_float4(v[j + e] * f, v[j + e + 1] * f, v[j + e + 2] * f, v[j + e + 3] * f) : make_float4(0.f, 0.f, 0.f, 0.f);
-                    } else {
-                        uint4 w;
-                        uint32_t *q = &w.x;
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) q[e] = real ? pack_pair<T>(v[j + 2 * e] * f, v[j + 2 * e + 1] * f) : 0u;
-                        *reinterpret_cast<uint4 *>(dst + to + d0 + j) = w;
-                    }
+                for (int e = 0; e < 4; ++e) {
+                    if constexpr (Op::kPlanes) q[e] = real ? __float_as_uint(v[j + e] * f) : 0u;
+                    else q[e] = real ? pack_pair<T>(v[j + 2 * e] * f, v[j + 2 * e + 1] * f) : 0u;
                 }
+                row_out[((d0 + j) / kPer) ^ (r & 7)] = w;
+            }
             __syncwarp();
         }
         tmem_before_sync();
+        asm volatile("bar.sync 2, %0;" ::"n"(L::kWorkers) : "memory");
+        for (int idx = tid; idx < L::kSums * 128 * kPieces; idx += L::kWorkers) {
+            const int which = idx / (128 * kPieces), at = idx % (128 * kPieces), row_at = at / kPieces, c = at % kPieces, m = o0 + row_at;
+            if (m >= (KEYS ? p.Tk : p.M) || c * (16 / (int)sizeof(T)) >= p.D) continue;
+            const int t = KEYS || p.R == 1 ? m : m / p.R, head = KEYS ? g : g * p.R + m - t * p.R;
+            T *dst = (which ? g2 : g1) + (((long)b * (KEYS ? p.Tk : p.Tq) + t) * (KEYS ? p.G : p.H) + head) * p.D;
+            reinterpret_cast<uint4 *>(dst)[c] = reinterpret_cast<const uint4 *>(stage)[(which * 128 + row_at) * kPieces + (c ^ (row_at & 7))];
+        }
     }
     __syncthreads();
     if (warp == L::kWorkers / 32) {

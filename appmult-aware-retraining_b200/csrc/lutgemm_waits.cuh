@@ -18,6 +18,10 @@ __device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {
 __device__ __forceinline__ void mbar_arrive(uint32_t bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
 }
+// `count` arrivals at once
+__device__ __forceinline__ void mbar_arrive_many(uint32_t bar, uint32_t count) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(count) : "memory");
+}
 // One attempt: returns at once when the phase with this parity is complete, otherwise the hardware suspends the
 // thread until it completes or a short, implementation-defined time has passed (so a waiting warp does not
 // spend issue slots and shared-memory bandwidth on polling).
