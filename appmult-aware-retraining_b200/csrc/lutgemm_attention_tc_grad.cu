@@ -73,8 +73,8 @@ __global__ void __launch_bounds__(256) attention_delta_kernel(const AttnProblem 
 // tensor cores lets go one by one: a round of 128-value heads took 3200 clocks for 1300 of products).  There are two groups of
 // eight warps that take rounds in turn, each with its own S and gP, so that the products of one round run beside the exponentials
 // of another.  Heads of up to 64 values leave room for P and dS beside S and gP; the scores of a group's next round are then
-// formed as soon as it has this round's in registers, and another warp issues the sums (one warp for both spent half of its
-// rounds on waits that had long been over).  Larger ones keep P over S and dS over gP.
+// formed as soon as it has this round's in registers, by a warp for each group, and another warp issues the sums, in order (one warp
+// for all spent half of its rounds on waits that had long been over).  Larger ones keep P over S and dS over gP.
 // Results go through shared memory, which the ring has left, so that whole rows are written (a row to a thread took 6000 clocks of
 // a block of 16000 where there are 197 keys).
 // fp16: P is kept 2^10 larger, and grad_o is taken in units of its largest value in this key head (a power of two), so that dS stays
@@ -85,8 +85,8 @@ template <typename T, int DP, bool KEYS>
 struct GradLayout {
     using Op = Operand<T, DP>;
     static constexpr int kBlocks = Op::kBlocks, kGroups = Op::kPlanes ? 1 : 2, kStages = Op::kPlanes ? 2 : DP == 64 ? 6 : 4;
-    static constexpr bool kEarly = DP == 64;  // P and dS have room of their own; a warp for the scores and one for the sums
-    static constexpr int kWorkers = 256 * kGroups, kThreads = kWorkers + (kEarly ? 96 : 64), kSums = KEYS ? 2 : 1;
+    static constexpr bool kEarly = DP == 64;  // P and dS have room of their own; a warp for each group's scores and one for the sums
+    static constexpr int kWorkers = 256 * kGroups, kThreads = kWorkers + (kEarly ? 64 + 32 * kGroups : 64), kSums = KEYS ? 2 : 1;
     static constexpr uint32_t kTile = 64 * kBlocks * 128, kX = 0, kY = 2 * kTile, kRing = 4 * kTile;  // a stage of the ring: x, y
     static constexpr uint32_t kCols = kRing + kStages * 2 * kTile;  // KEYS: for each stage -lse, -delta, documents, slopes and places of 64 rows
     static constexpr uint32_t kBars = kCols + (KEYS ? kStages * 64 * 20 : 0), kBytes = kBars + 384;
@@ -229,8 +229,9 @@ __global__ void __launch_bounds__(GradLayout<T, DP, KEYS>::kThreads, 1)
                 walk.own = own_range(row_ranges + (long)b * ((p.M + size - 1) / size), o0, last + 1, size);
             }
         }
+        int ends = 0;
         for (int n = 0;; ++n) {
-            const int tile = walk.next(docs), t = tile >> 1, stage = n % L::kStages;
+            const int tile = ends ? -1 : walk.next(docs), t = tile >> 1, stage = n % L::kStages;
             // KEYS: what a round needs of its rows, two to a lane
             float row_stat[2], row_delta[2], row_slope[2], row_place[2];
             int row_doc[2];
@@ -268,7 +269,7 @@ __global__ void __launch_bounds__(GradLayout<T, DP, KEYS>::kThreads, 1)
             __syncwarp();
             if (elect_one()) {
                 const uint32_t at = base + L::kRing + stage * 2 * L::kTile, bar = bar_full + 8 * stage;
-                brought[stage] = tile;
+                brought[stage] = tile - ends;  // (-1: the end; -2: behind it)
                 if (tile >= 0) {
                     tma_expect_bytes(bar, 2 * L::kBlocks * (KEYS ? size : 64) * 128);
 #pragma unroll
@@ -282,7 +283,8 @@ __global__ void __launch_bounds__(GradLayout<T, DP, KEYS>::kThreads, 1)
                 }
             }
             __syncwarp();
-            if (tile < 0 || *abort_word) break;
+            ends += tile < 0;
+            if (ends == G || *abort_word) break;  // (each group hears of the end)
         }
     } else if (warp >= L::kWorkers / 32) {  // issue the products
         const int lane = tid & 31;
@@ -383,14 +385,11 @@ __global__ void __launch_bounds__(GradLayout<T, DP, KEYS>::kThreads, 1)
                 for (int i = 0; i + 1 < G; ++i) ahead[i] = ahead[i + 1];
                 ahead[G - 1] = tile;
             }
-        } else if (warp == L::kWorkers / 32) {  // the scores
-            constexpr int kUnknown = 1 << 30;  // (there are at most 2^25 tiles)
-            int last = kUnknown;
-            for (int k = 0; k < last + G; ++k) {
-                const int tile = arrived(k, last == kUnknown);
-                if (tile < 0 && last == kUnknown) last = k;
-                if (k >= G && k - G < last) mbar_wait(bar_l + 8 * (k % G), (k / G - 1) & 1, 217, abort_word, error_word);
-                if (k == last && k >= G) {
+        } else if (warp != L::kWorkers / 32 + 2) {  // the scores of a group
+            for (int k = warp == L::kWorkers / 32 ? 0 : 1;; k += G) {
+                const int tile = arrived(k, true);
+                if (k >= G) mbar_wait(bar_l + 8 * (k % G), (k / G - 1) & 1, 217, abort_word, error_word);
+                if (tile == -1 && k >= G) {
                     // Word of the end goes to the sums in place of the workers' arrivals, when those of the group's last round are all
                     // there and the sums have taken note of them: a barrier's parity tells two phases apart, not three.  (The
                     // first wait makes the second one sure of its phase.)
@@ -401,13 +400,13 @@ __global__ void __launch_bounds__(GradLayout<T, DP, KEYS>::kThreads, 1)
                 __syncwarp();
                 if (elect_one()) {
                     issue_scores(k, tile);
-                    if (k == last) {
+                    if (tile == -1) {
                         *rounds_seen = k;
                         mbar_arrive_many(bar_p + 8 * (k % G), 256);
                     }
                 }
                 __syncwarp();
-                if (*abort_word) break;
+                if (tile < 0 || *abort_word) break;
             }
         } else {  // the sums
             for (;; ++n) {
@@ -424,7 +423,7 @@ __global__ void __launch_bounds__(GradLayout<T, DP, KEYS>::kThreads, 1)
             __syncwarp();
             mbar_wait(bar_end, 0, 214, abort_word, error_word);
         }
-        if (lane == 0 && (!L::kEarly || warp != L::kWorkers / 32)) tiles[8] = n;  // rounds done
+        if (lane == 0 && warp == L::kWorkers / 32 + (L::kEarly ? 2 : 0)) tiles[8] = n;  // rounds done
     } else {
         const uint32_t mine = tmem + ((uint32_t)((warp & 3) * 32) << 16);
         const Bend bend = make_bend<Op::kPlanes>(p);
