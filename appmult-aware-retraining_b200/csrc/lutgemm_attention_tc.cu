@@ -23,9 +23,10 @@ constexpr int kThreads = 160;  // four warps with a row to a thread, one that br
 template <typename T, int DP>
 struct Layout {
     using Op = Operand<T, DP>;
-    static constexpr int kBlocks = Op::kBlocks, kStages = DP == 64 && !Op::kPlanes ? 1 : 2, kKStages = kStages + 1;
+    static constexpr int kBlocks = Op::kBlocks, kStages = DP == 64 && !Op::kPlanes ? 1 : 2;  // of S
+    static constexpr int kKStages = 3, kVStages = kStages == 1 ? 3 : 2;                        // of tiles of K and V
     static constexpr int kPerSm = Op::kPlanes ? 1 : DP == 64 ? 3 : 2;
-    static constexpr uint32_t kTile = kKeyTile * kBlocks * 128, kQ = 0, kK = 2 * kTile, kV = kK + kKStages * kTile, kBars = kV + 2 * kTile,
+    static constexpr uint32_t kTile = kKeyTile * kBlocks * 128, kQ = 0, kK = 2 * kTile, kV = kK + kKStages * kTile, kBars = kV + kVStages * kTile,
                               kBytes = kBars + 128;
     static constexpr uint32_t kS = Op::kPlanes ? 96 : 64, kO = kStages * kS;  // tensor memory: S or P of each stage, then O
     static constexpr uint32_t kColumns = kO + DP <= 128 ? 128 : 256;
@@ -42,10 +43,10 @@ __global__ void __launch_bounds__(kThreads, Layout<T, DP>::kPerSm)
     constexpr float kShift = Op::kBf16 ? 0.f : 7.f;
     const int width = Op::kPlanes ? kPlaneWidth : p.D;
     extern __shared__ __align__(1024) uint8_t smem[];
-    const uint32_t base = smem_u32(smem), bar_s = base + L::kBars, bar_o = bar_s + 16, bar_p = bar_s + 24, bar_k = bar_s + 32, bar_v = bar_s + 56;
-    volatile int *abort_word = reinterpret_cast<int *>(smem + L::kBars + 72);
-    uint32_t *slot = reinterpret_cast<uint32_t *>(smem + L::kBars + 76);
-    volatile int *tiles = reinterpret_cast<int *>(smem + L::kBars + 80);  // of the last four rounds begun
+    const uint32_t base = smem_u32(smem), bar_s = base + L::kBars, bar_o = bar_s + 16, bar_p = bar_s + 24, bar_k = bar_s + 32, bar_v = bar_s + 56;  // (three each)
+    volatile int *abort_word = reinterpret_cast<int *>(smem + L::kBars + 80);
+    uint32_t *slot = reinterpret_cast<uint32_t *>(smem + L::kBars + 84);
+    volatile int *tiles = reinterpret_cast<int *>(smem + L::kBars + 88);  // of the last four rounds begun
     const int tid = threadIdx.x, warp = warp_index();
     // blocks in order of falling work: the last rows see the most keys
     int bid = blockIdx.x;
@@ -62,11 +63,17 @@ __global__ void __launch_bounds__(kThreads, Layout<T, DP>::kPerSm)
         mbar_init(bar_s + 8, 2);
         mbar_init(bar_o, 1);
         mbar_init(bar_p, 128);
-        for (int i = 0; i < 5; ++i) mbar_init(bar_k + 8 * i, 1);
+        for (int i = 0; i < L::kKStages; ++i) mbar_init(bar_k + 8 * i, 1);
+        for (int i = 0; i < L::kVStages; ++i) mbar_init(bar_v + 8 * i, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
+    __syncthreads();
     if (warp == 4) {
-        tmem_alloc(smem_u32(slot), L::kColumns);
+        if (elect_one()) {
+            tma_prefetch_map(&map_k);
+            tma_prefetch_map(&map_v);
+        }
+        __syncwarp();
         TileWalk walk;
         const int last = min(m0 + kRowTile, p.M) - 1;
         const int all = max(0, key_limit(p, last / p.R + p.shift, pre) + kKeyTile) / kKeyTile;  // up to the last visible key
@@ -96,11 +103,16 @@ __global__ void __launch_bounds__(kThreads, Layout<T, DP>::kPerSm)
                 load_keys<L::kBlocks>(base + L::kV + stage * L::kTile, &map_v, b, g, (queue[i] >> 1) * kKeyTile, bar_v + 8 * stage);
         };
 #pragma unroll
-        for (int i = 0; i <= L::kStages; ++i) bring(i);
-        __syncthreads();
+        for (int i = 0; i < L::kKStages; ++i) bring(i);
 #pragma unroll
-        for (int i = 0; i <= L::kStages; ++i) bring_k(i, i);
-        bring_v(0, 0);
+        for (int i = 0; i < L::kKStages; ++i) {
+            bring_k(i, i);
+            if (i < L::kVStages - 1) bring_v(i, i);
+        }
+        __syncwarp();
+        tmem_alloc(smem_u32(slot), L::kColumns);
+        tmem_before_sync();
+        __syncthreads();  // Q has come
         tmem_after_sync();
         const uint32_t tmem = *slot;
         constexpr uint32_t desc_s = mma_descriptor(Op::kBf16, kKeyTile, false), desc_o = mma_descriptor(Op::kBf16, DP, true);
@@ -140,9 +152,9 @@ __global__ void __launch_bounds__(kThreads, Layout<T, DP>::kPerSm)
         }
         __syncwarp();
         for (int n = 0; queue[0] >= 0; ++n) {
-            bring(L::kStages + 1);
-            mbar_wait(bar_v + 8 * (n & 1), n >> 1 & 1, 207, abort_word, error_word);
-            clear_padding(queue[0], L::kV + (n & 1) * L::kTile);
+            bring(L::kKStages);
+            mbar_wait(bar_v + 8 * (n % L::kVStages), n / L::kVStages & 1, 207, abort_word, error_word);
+            clear_padding(queue[0], L::kV + n % L::kVStages * L::kTile);
             if (queue[L::kStages] >= 0 && queue[L::kStages - 1] >= 0) {
                 const int stage = (n + L::kStages) % L::kKStages;
                 mbar_wait(bar_k + 8 * stage, (n + L::kStages) / L::kKStages & 1, 208, abort_word, error_word);
@@ -153,11 +165,11 @@ __global__ void __launch_bounds__(kThreads, Layout<T, DP>::kPerSm)
             __syncwarp();
             // every row has waited for the products of round n - 1 and S of round n: those buffers are free.  (Copies first: the queue
             // of the tensor cores lets products go one by one)
-            bring_v(1, (n + 1) & 1);
-            bring_k(L::kStages + 1, n % L::kKStages);
+            bring_v(L::kVStages - 1, (n + L::kVStages - 1) % L::kVStages);
+            bring_k(L::kKStages, n % L::kKStages);
             __syncwarp();
             if (elect_one()) {
-                const uint64_t v = smem_descriptor(base + L::kV + (n & 1) * L::kTile, Op::kPlanes ? 0 : kKeyTile * 128);
+                const uint64_t v = smem_descriptor(base + L::kV + n % L::kVStages * L::kTile, Op::kPlanes ? 0 : kKeyTile * 128);
                 const uint32_t a = tmem + (n % L::kStages) * L::kS;
                 if constexpr (Op::kPlanes) {
 #pragma unroll
@@ -174,7 +186,7 @@ __global__ void __launch_bounds__(kThreads, Layout<T, DP>::kPerSm)
             }
             __syncwarp();
 #pragma unroll
-            for (int i = 0; i <= L::kStages; ++i) queue[i] = queue[i + 1];
+            for (int i = 0; i < L::kKStages; ++i) queue[i] = queue[i + 1];
         }
     } else {
         copy_row_tile<L::kBlocks>(base + L::kQ, p, p.q, width, b, g, m0, tid);
@@ -337,8 +349,11 @@ __global__ void __launch_bounds__(kThreads, Layout<T, DP>::kPerSm)
         }
         const float inv = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : NAN;
         const float stat = sum == 0.f ? INFINITY : most - kShift + log2f(sum);
-        const int i = m < p.M ? m / p.R : 0, h = g * p.R + m - i * p.R;
         const long at = ((long)b * p.G + g) * p.M + m;
+        // Whole rows are stored, through shared memory that Q and K have left (a row to a thread would touch 32 lines with every
+        // store): a row's 16-byte pieces c at c ^ (row & 7), the rest of the rounding behind the rows.
+        constexpr int kPieces = DP * (int)sizeof(T) / 16, kPer = 16 / (int)sizeof(T);
+        uint4 *stage = reinterpret_cast<uint4 *>(smem);
 #pragma unroll
         for (int c = 0; c < DP / 32; ++c) {
             float o[32];
@@ -353,40 +368,53 @@ __global__ void __launch_bounds__(kThreads, Layout<T, DP>::kPerSm)
                 tmem_load32(mine + L::kO + 32 * c, o);
                 tmem_loads_done();
             }
-            if (m < p.M) {
 #pragma unroll
-                for (int j = 0; j < 32; ++j) o[j] = sum == 0.f ? 0.f : o[j] * inv;
-                if (splits > 1) {
+            for (int j = 0; j < 32; ++j) o[j] = sum == 0.f ? 0.f : o[j] * inv;
+            if (splits > 1) {
+                if (m < p.M) {
                     float4 *dst = reinterpret_cast<float4 *>(part + ((long)split * p.B * p.G * p.M + at) * DP + 32 * c);
 #pragma unroll
                     for (int j = 0; j < 8; ++j) dst[j] = make_float4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
-                } else {
-                    const long to = (((long)b * p.Tq + i) * p.H + h) * p.D + 32 * c;
+                }
+            } else {
 #pragma unroll
-                    for (int j = 0; j < 32; j += 8) {
-                        if (32 * c + j >= p.D) break;
-                        if constexpr (Op::kPlanes) {
-                            *reinterpret_cast<float4 *>(out + to + j) = make_float4(o[j], o[j + 1], o[j + 2], o[j + 3]);
-                            *reinterpret_cast<float4 *>(out + to + j + 4) = make_float4(o[j + 4], o[j + 5], o[j + 6], o[j + 7]);
-                        } else {
-                        uint4 v;
-                        uint32_t *r = &v.x;
+                for (int j = 0; j < 32; j += kPer) {
+                    uint4 v;
+                    uint32_t *r = &v.x;
+                    uint4 *to = stage + tid * kPieces + (((32 * c + j) / kPer) ^ (tid & 7));
+                    if constexpr (Op::kPlanes) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) r[e] = __float_as_uint(o[j + e]);
+                        *to = v;
+                    } else {
 #pragma unroll
                         for (int e = 0; e < 4; ++e) r[e] = pack_pair<T>(o[j + 2 * e], o[j + 2 * e + 1]);
-                        *reinterpret_cast<uint4 *>(out + to + j) = v;
+                        *to = v;
                         if (rest) {
 #pragma unroll
                             for (int e = 0; e < 4; ++e) {
                                 const float2 hi = unpack_pair<T>(r[e]);
                                 r[e] = pack_pair<T>(o[j + 2 * e] - hi.x, o[j + 2 * e + 1] - hi.y);
                             }
-                            *reinterpret_cast<uint4 *>(rest + to + j) = v;
-                        }
+                            to[kRowTile * kPieces] = v;
                         }
                     }
                 }
             }
             __syncwarp();
+        }
+        if (splits == 1) {
+            __syncwarp();
+            // (a warp's rows are its own)
+            for (int idx = tid & 31; idx < 32 * kPieces; idx += 32) {
+                const int r = 32 * warp + idx / kPieces, c = idx % kPieces, row_at = m0 + r;
+                if (row_at >= p.M || c * kPer >= p.D) continue;
+                const int t = p.R == 1 ? row_at : row_at / p.R;
+                const long to = (((long)b * p.Tq + t) * p.H + g * p.R + row_at - t * p.R) * p.D;
+                const uint4 *from = stage + r * kPieces + (c ^ (r & 7));
+                reinterpret_cast<uint4 *>(out + to)[c] = *from;
+                if (!Op::kPlanes && rest) reinterpret_cast<uint4 *>(rest + to)[c] = from[kRowTile * kPieces];
+            }
         }
         if (m < p.M) {
             if (splits > 1) part_lse[(long)split * p.B * p.G * p.M + at] = sum == 0.f ? -INFINITY : stat;
