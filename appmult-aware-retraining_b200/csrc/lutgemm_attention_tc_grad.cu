@@ -70,29 +70,34 @@ __global__ void __launch_bounds__(256) attention_delta_kernel(const AttnProblem 
 //     they were copied, serve as row and as column operands)
 // Eight warps share a round, four with the first 32 columns and four with the others; one further warp issues the products and one
 // brings the tiles (when one warp did both, copies were asked for only behind the products of a round, which the queue of the
-// tensor cores lets go one by one: a round of 128-value heads took 3200 clocks for 1300 of products).  There are two groups of
-// eight warps that take rounds in turn, each with its own S and gP, so that the products of one round run beside the exponentials
-// of another.  Heads of up to 64 values leave room for P and dS beside S and gP; the scores of a group's next round are then
-// formed as soon as it has this round's in registers, by a warp for each group, and another warp issues the sums, in order (one warp
-// for all spent half of its rounds on waits that had long been over).  Larger ones keep P over S and dS over gP.
+// tensor cores lets go one by one: a round of 128-value heads took 3200 clocks for 1300 of products).  What overlaps rounds:
+//   heads of more than 64 values    their sums fill the tensor memory of an SM; two groups of eight warps take rounds in turn, each with
+//                                   its own S and gP, and keep P over S and dS over gP
+//   up to 64 values                 one group, P and dS over S and gP, and two blocks on an SM
+//   the same with bent scores       (a cap, a bias) whose exponentials take longer: two groups with P and dS of their own, so that the
+//                                   scores of a group's next round are formed as soon as this round's are in registers, by a warp
+//                                   for each group; another warp issues the sums, in order.  4 x 4096 x 6 x 64 bf16: with a cap
+//                                   950 us for both kernels (as above 1100), without one 600 us (as above 530)
 // Results go through shared memory, which the ring has left, so that whole rows are written (a row to a thread took 6000 clocks of
 // a block of 16000 where there are 197 keys).
 // fp16: P is kept 2^10 larger, and grad_o is taken in units of its largest value in this key head (a power of two), so that dS stays
 // out of fp16's subnormal range whatever the scale of the loss.
 // fp32: P and dS are split into planes as the operands were; there is one group, and each round's sums start from zero and are added up
 // in registers (in the accumulators, what additions cut off came to 2e-5 of the gradients of 4096 rows).
-template <typename T, int DP, bool KEYS>
+template <typename T, int DP, bool BENT, bool KEYS>
 struct GradLayout {
     using Op = Operand<T, DP>;
-    static constexpr int kBlocks = Op::kBlocks, kGroups = Op::kPlanes ? 1 : 2, kStages = Op::kPlanes ? 2 : DP == 64 ? 6 : 4;
-    static constexpr bool kEarly = DP == 64;  // P and dS have room of their own; a warp for each group's scores and one for the sums
+    static constexpr bool kSmall = DP == 64 && !Op::kPlanes && !BENT;  // two blocks on an SM
+    static constexpr bool kEarly = DP == 64 && !kSmall;  // P and dS have room of their own; a warp for each group's scores and one for the sums
+    static constexpr int kBlocks = Op::kBlocks, kGroups = Op::kPlanes || kSmall ? 1 : 2, kPerSm = kSmall ? 2 : 1;
+    static constexpr int kStages = Op::kPlanes ? 2 : kSmall ? 3 : kEarly ? 6 : 4;
     static constexpr int kWorkers = 256 * kGroups, kThreads = kWorkers + (kEarly ? 64 + 32 * kGroups : 64), kSums = KEYS ? 2 : 1;
     static constexpr uint32_t kTile = 64 * kBlocks * 128, kX = 0, kY = 2 * kTile, kRing = 4 * kTile;  // a stage of the ring: x, y
     static constexpr uint32_t kCols = kRing + kStages * 2 * kTile;  // KEYS: for each stage -lse, -delta, documents, slopes and places of 64 rows
     static constexpr uint32_t kBars = kCols + (KEYS ? kStages * 64 * 20 : 0), kBytes = kBars + 384;
     // tensor memory of a group: S, gP and, behind them or over them, P and dS (64 values of 16 bits: 32 columns); then the sums
     static constexpr uint32_t kP = kEarly ? 128 : 0, kDS = Op::kPlanes ? 224 : kEarly ? 160 : 64, kGroup = Op::kPlanes ? 320 : kEarly ? 192 : 128;
-    static constexpr uint32_t kAcc = kGroups * kGroup, kColumns = 512;
+    static constexpr uint32_t kAcc = kGroups * kGroup, kColumns = kSmall ? 256 : 512;
     static_assert(kAcc + kSums * DP <= kColumns, "tensor memory");
     // where a half of the columns of P or dS lies, and the operand of the i-th sixteen of them
     __device__ static constexpr uint32_t half(int h) { return kEarly ? 16 * h : 32 * h; }
@@ -100,11 +105,11 @@ struct GradLayout {
 };
 
 template <typename T, int DP, bool BENT, bool KEYS>
-__global__ void __launch_bounds__(GradLayout<T, DP, KEYS>::kThreads, 1)
+__global__ void __launch_bounds__(GradLayout<T, DP, BENT, KEYS>::kThreads, GradLayout<T, DP, BENT, KEYS>::kPerSm)
     attention_tc_grad_kernel(const AttnProblem p, const AttnTensor go, const __grid_constant__ CUtensorMap map_x,
                              const __grid_constant__ CUtensorMap map_y, const DocRange *key_ranges, const DocRange *row_ranges,
                              const float *lse, const float *delta, const float *most, int most_parts, T *g1, T *g2, int *error_word) {
-    using L = GradLayout<T, DP, KEYS>;
+    using L = GradLayout<T, DP, BENT, KEYS>;
     constexpr int G = L::kGroups;
     using Op = typename L::Op;
     constexpr bool kBf16 = Op::kBf16;
@@ -658,7 +663,7 @@ __global__ void __launch_bounds__(GradLayout<T, DP, KEYS>::kThreads, 1)
 template <typename T, int DP, bool BENT, bool KEYS>
 int launch(const AttnProblem &p, const AttnTensor &go, const CUtensorMap &map_x, const CUtensorMap &map_y, const DocRange *kr, const DocRange *rr,
            const float *lse, const float *delta, const float *most, int most_parts, void *g1, void *g2, int *error_word, cudaStream_t stream) {
-    using L = GradLayout<T, DP, KEYS>;
+    using L = GradLayout<T, DP, BENT, KEYS>;
     if (!cuda_ok(cudaFuncSetAttribute(attention_tc_grad_kernel<T, DP, BENT, KEYS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)L::kBytes)))
         return LUTGEMM_E_CUDA;
     const long blocks = (long)(((KEYS ? p.Tk : p.M) + 127) / 128) * p.B * p.G;
