@@ -1245,7 +1245,7 @@ int lutgemm_token_logprobs(const void *logits, int dtype, long pitch, long N, in
                            size_t scratch_bytes, void *stream) {
     if (!logits || !target || !logp || !entropy || !stats || !dtype_supported(dtype)) return LUTGEMM_E_BADARG;
     if (N <= 0 || C <= 0 || top < 0 || top > C || (top > 0 && (!top_logp || !top_index))) return LUTGEMM_E_BADARG;
-    if (top > 32 || N > 0x7fffffffL) return LUTGEMM_E_TOOLARGE;
+    if (top > 32 || N > 0x7fffffffL || C > 1 << 27) return LUTGEMM_E_TOOLARGE;
     const int sms = current_num_sms();
     if (sms <= 0) return LUTGEMM_E_CUDA;
     const size_t need = lutgemm::logprobs_scratch_bytes(N, C, top, sms);
@@ -1258,7 +1258,7 @@ int lutgemm_token_logprobs(const void *logits, int dtype, long pitch, long N, in
 int lutgemm_token_logprobs_backward(const void *logits, int dtype, long pitch, long N, int C, const long long *target, long long ignore,
                                     const float *stats, const float *g_logp, const float *g_entropy, void *grad, void *stream) {
     if (!logits || !target || !stats || !grad || !dtype_supported(dtype) || N <= 0 || C <= 0) return LUTGEMM_E_BADARG;
-    if (N > 0x7fffffffL) return LUTGEMM_E_TOOLARGE;
+    if (N > 0x7fffffffL || C > 1 << 27) return LUTGEMM_E_TOOLARGE;
     return lutgemm::logprobs_backward(logits, dtype, pitch, N, C, target, ignore, stats, g_logp, g_entropy, grad,
                                       static_cast<cudaStream_t>(stream));
 }

@@ -99,8 +99,8 @@ struct NormRotate : torch::autograd::Function<NormRotate> {
         const Tensor &q = saved[0], &k = saved[1], &cos = saved[4], &sin = saved[5];
         const MaybeTensor qw = maybe(saved[2]), kw = maybe(saved[3]), positions = maybe(saved[6]);
         Tensor dq = at::empty(q.sizes(), q.options()), dk = at::empty(k.sizes(), q.options()), dqw, dkw;
-        if (qw && ctx->needs_input_grad(2)) dqw = at::empty(qw->sizes(), qw->options());
-        if (kw && ctx->needs_input_grad(3)) dkw = at::empty(kw->sizes(), kw->options());
+        if (wants_grad(qw)) dqw = at::empty(qw->sizes(), qw->options());
+        if (wants_grad(kw)) dkw = at::empty(kw->sizes(), kw->options());
         if (q.size(0) * q.size(1) > 0) {
             const Tensor gq = rows(grads[0]), gk = rows(grads[1]);
             const c10::cuda::CUDAGuard guard(q.device());
@@ -141,6 +141,7 @@ std::pair<Tensor, Tensor> norm_rotate(const Tensor &q, const Tensor &k, const Ma
         TORCH_CHECK(cos.dim() == 2 && 2 * cos.size(1) <= D, "cos must be [positions, at most ", D / 2, "], got ", cos.sizes());
         check_side(cos, "cos", at::kFloat, cos.sizes(), q);
         check_side(sin, "sin", at::kFloat, cos.sizes(), q);
+        TORCH_CHECK(!at::GradMode::is_enabled() || !(cos.requires_grad() || sin.requires_grad()), "cos and sin have no gradient");
         TORCH_CHECK(cos.size(0) <= 0x7fffffffLL, "cos and sin have too many positions");
         cos = cos.contiguous();
         sin = sin.contiguous();
@@ -258,7 +259,7 @@ Tensor attention(const Tensor &q, const Tensor &k, const Tensor &v, c10::optiona
                       cap, " and ", scale);
     if (slopes.has_value()) {
         check_side(*slopes, "slopes", at::kFloat, {H}, q);
-        TORCH_CHECK(!slopes->requires_grad(), "slopes have no gradient");
+        TORCH_CHECK(!at::GradMode::is_enabled() || !slopes->requires_grad(), "slopes have no gradient");
         slopes = slopes->contiguous();
     }
     if (prefix.has_value()) {

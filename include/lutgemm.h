@@ -417,7 +417,7 @@ int lutgemm_attention_backward(const void *go, long go_sb, long go_st, long go_s
                                size_t scratch_bytes, void *stream);
 
 /*
- * For each of N rows of C logits, `pitch` elements apart: logp[n] = log softmax(logits[n])[target[n]] (0 where the target is `ignore`,
+ * For each of N rows of C (up to 2^27) logits, `pitch` elements apart: logp[n] = log softmax(logits[n])[target[n]] (0 where the target is `ignore`,
  * NaN where it is no class), entropy[n] of the softmax, and the `top` (0 to 32, at most C) most probable classes in order, the
  * lower class first among equals (NaN logits before all others).  Logits of -inf have no probability; a row of nothing else has
  * logp -inf and entropy 0; a NaN or +inf logit makes its row's results NaN.  `stats` fp32 [N, 3] is for the backward pass:

@@ -164,3 +164,8 @@ def test_rotary_tables():
         lutgemm_attention.rotary_tables(4, 3)
     with pytest.raises(ValueError):
         lutgemm_attention.rotary_tables_2d(4, 4, 6)
+
+
+def test_logprobs_refuse_rows_beyond_their_indices(lib):
+    most = 1 << 27
+    assert logprobs(lib, N=1, C=most)[0] == H.OK and logprobs(lib, N=1, C=most + 1) == (H.E_TOOLARGE, [])
