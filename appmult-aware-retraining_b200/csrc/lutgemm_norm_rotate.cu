@@ -10,11 +10,14 @@
 // that both halves of a pair are in the same lane, so a rotation needs no exchange and a norm one shuffle reduction over the few
 // lanes of a head (4 for 64 bf16 values).  A group of lanes takes HEADS heads of one token at a time: weights and angles
 // are loaded once for them and their loads are in flight together; a grid of few tokens takes one head per group instead, so that
-// it spreads over the GPU.  The blocks are split between queries and keys, in proportion; weights then stay with a block, and
-// so do the sums of their gradients: per lane in registers, per block in shared memory, over the blocks by a second kernel in
-// ascending order, so results do not depend on timing.
+// it spreads over the GPU.  Where groups go round often, the loads of the next two rounds are under way in a ring in shared memory
+// (each thread reads what it asked for itself, so the ring needs no barrier) and the next angles in registers.  The blocks are
+// split between queries and keys, in proportion; weights then stay with a block, and so do the sums of their gradients: per lane
+// in registers, per block in shared memory, over the blocks by a second kernel in ascending order, so results do not depend on
+// timing.  4 x 8192 tokens of 32 + 8 bf16 heads of 128: 304 us for both passes (1.68 GB, 5.5 TB/s).
 #include "lutgemm.h"
 #include "lutgemm_attention.cuh"
+#include "lutgemm_common.cuh"
 #include "lutgemm_f32x2.cuh"
 #include "lutgemm_kernels.h"
 
@@ -61,21 +64,32 @@ __device__ __forceinline__ void store_vec(T *dst, const float (&src)[V]) {
     *reinterpret_cast<Vec<T, V> *>(dst) = x;
 }
 
-// a slot's two vectors: places in the head, and the first angle (-1: not turned)
+// A slot's two vectors: places in the head, and the angles that turn them (-1: none).  Neighbouring lanes take neighbouring vectors, so
+// that every load and store of a warp covers whole sectors: with both vectors of a slot side by side each touched half of every sector
+// and the training pass of 4 x 8192 x 40 heads of 128 bf16 values took 414 us instead of 338.
 struct Slot {
-    int a, b, angle;
+    int a, b, angle, angle_b;
 };
 template <int V>
 __device__ __forceinline__ Slot slot_of(const NormArgs &p, int c) {
     Slot s;
-    if (p.interleaved || c * V >= p.rot / 2) {
-        s.a = p.interleaved ? c * 2 * V : p.rot + (c - p.rot / 2 / V) * 2 * V;
-        s.b = s.a + V;
-        s.angle = p.interleaved && s.a < p.rot ? c * V : -1;
+    if (p.interleaved && V > 1) {  // pairs lie within a vector
+        s.a = c * V;
+        s.b = p.D / 2 + c * V;
+        s.angle = s.a < p.rot ? s.a / 2 : -1;
+        s.angle_b = s.b < p.rot ? s.b / 2 : -1;
+    } else if (p.interleaved) {
+        s.a = 2 * c;
+        s.b = s.a + 1;
+        s.angle = s.angle_b = s.a < p.rot ? c : -1;
+    } else if (c * V >= p.rot / 2) {
+        s.a = p.rot / 2 + c * V;
+        s.b = s.a + (p.D - p.rot) / 2;
+        s.angle = s.angle_b = -1;
     } else {
         s.a = c * V;
         s.b = s.a + p.rot / 2;
-        s.angle = s.a;
+        s.angle = s.angle_b = s.a;
     }
     return s;
 }
@@ -154,11 +168,18 @@ __device__ __forceinline__ float both(f32x2 v) {
     return t.x + t.y;
 }
 
-// V values to a vector, SPL slots to a lane, HEADS heads of a token at a time.  INTER: the interleaved layout
-template <typename T, int V, int SPL, int HEADS, bool INTER, bool BACKWARD>
+constexpr int kStages = 3;  // rounds of vectors that a ring in shared memory holds
+
+// V values to a vector, SPL slots to a lane, HEADS heads of a token at a time.  INTER: the interleaved layout.  RING: vectors of 16
+// bytes are asked for two rounds ahead, angles one
+template <typename T, int V, int SPL, int HEADS, bool INTER, bool RING, bool BACKWARD>
 __global__ void __launch_bounds__(kBlock, 2) norm_rotate_kernel(const NormArgs p) {
     constexpr int N = Packed<V>::n;
-    extern __shared__ float sums[];  // backward: [groups][D]
+    constexpr int kPieces = BACKWARD ? 4 : 2, kRing = RING ? kStages : 0;
+    // the vectors on their way, [stage][head][slot][piece][thread]; backward: then sums [groups][D]
+    extern __shared__ __align__(16) unsigned char shared[];
+    Vec<T, V> *ring = reinterpret_cast<Vec<T, V> *>(shared) + threadIdx.x;
+    float *sums = reinterpret_cast<float *>(shared);
     const bool second = (int)blockIdx.x >= p.side[0].blocks;
     const Side &sd = p.side[second];
     const int block = blockIdx.x - (second ? p.side[0].blocks : 0);
@@ -196,53 +217,119 @@ __global__ void __launch_bounds__(kBlock, 2) norm_rotate_kernel(const NormArgs p
 #pragma unroll
             for (int i = 0; i < N; ++i) dw[s].v[i] = 0ull;
     }
-    // (whole warps go round together: the shuffles below are over groups of lanes of one warp)
-    for (unsigned u0 = (unsigned)block * groups; u0 < units; u0 += (unsigned)sd.blocks * groups) {
-        const unsigned u = u0 + group;
-        const bool in = u < units;
-        const unsigned token = in ? u / chunks : 0u, b = token / (unsigned)p.T, t = token - b * (unsigned)p.T;
-        const int h0 = in ? (int)(u - token * chunks) * HEADS : 0, heads = in ? min(HEADS, sd.heads - h0) : 0;
-        const T *x = static_cast<const T *>(sd.x) + (long)b * sd.sb + (long)t * sd.st + h0 * sd.sh;
-        const T *g = BACKWARD ? static_cast<const T *>(sd.g) + (long)b * sd.gb + (long)t * sd.gt + h0 * sd.gh : nullptr;
-        T *y = static_cast<T *>(sd.y) + ((long)token * sd.heads + h0) * p.D;
-        // as they lie in memory, all heads' loads in flight together
-        Vec<T, V> raw[HEADS][SPL][BACKWARD ? 4 : 2];
+    struct Unit {
+        bool in;
+        unsigned token, b, t;
+        int h0, heads;
+    };
+    const auto unit = [&](unsigned u) {
+        Unit r;
+        r.in = u < units;
+        r.token = r.in ? u / chunks : 0u;
+        r.b = r.token / (unsigned)p.T;
+        r.t = r.token - r.b * (unsigned)p.T;
+        r.h0 = r.in ? (int)(u - r.token * chunks) * HEADS : 0;
+        r.heads = r.in ? min(HEADS, sd.heads - r.h0) : 0;
+        return r;
+    };
+    // load(where, piece, address, is there) for the vectors of a unit: a and b of x, of g
+    const auto vectors = [&](const Unit &r, auto load) {
+        const T *x = static_cast<const T *>(sd.x) + (long)r.b * sd.sb + (long)r.t * sd.st + r.h0 * sd.sh;
+        [[maybe_unused]] const T *g = BACKWARD ? static_cast<const T *>(sd.g) + (long)r.b * sd.gb + (long)r.t * sd.gt + r.h0 * sd.gh : nullptr;
 #pragma unroll
         for (int h = 0; h < HEADS; ++h)
 #pragma unroll
             for (int s = 0; s < SPL; ++s) {
-#pragma unroll
-                for (int k = 0; k < (BACKWARD ? 4 : 2); ++k)
-#pragma unroll
-                    for (int i = 0; i < V; ++i) raw[h][s][k].v[i] = from_f32<T>(0.f);
-                if (h < heads && slot[s].a >= 0) {
-                    raw[h][s][0] = *reinterpret_cast<const Vec<T, V> *>(x + h * sd.sh + slot[s].a);
-                    raw[h][s][1] = *reinterpret_cast<const Vec<T, V> *>(x + h * sd.sh + slot[s].b);
-                    if constexpr (BACKWARD) {
-                        raw[h][s][2] = *reinterpret_cast<const Vec<T, V> *>(g + h * sd.gh + slot[s].a);
-                        raw[h][s][3] = *reinterpret_cast<const Vec<T, V> *>(g + h * sd.gh + slot[s].b);
-                    }
+                const bool there = h < r.heads && slot[s].a >= 0;
+                load(h * SPL + s, 0, x + h * sd.sh + slot[s].a, there);
+                load(h * SPL + s, 1, x + h * sd.sh + slot[s].b, there);
+                if constexpr (BACKWARD) {
+                    load(h * SPL + s, 2, g + h * sd.gh + slot[s].a, there);
+                    load(h * SPL + s, 3, g + h * sd.gh + slot[s].b, there);
                 }
             }
-        const int at = p.pos ? (in ? p.pos[token] : -1) : (int)t;
+    };
+    const auto fetch = [&](unsigned u, int stage) {
+        vectors(unit(u), [&](int at, int piece, const T *from, bool there) {
+            cp_async16_zfill(ring + (((size_t)stage * HEADS * SPL + at) * kPieces + piece) * kBlock, there ? from : static_cast<const T *>(sd.x), there);
+        });
+    };
+    const auto place = [&](const Unit &r) { return p.pos ? (r.in ? p.pos[r.token] : -1) : (int)r.t; };
+    const auto turns = [&](int at, float (&co)[SPL][V], float (&si)[SPL][V]) {
+#pragma unroll
+        for (int s = 0; s < SPL; ++s) {
+            // (interleaved: the first half of the angles turns a, the second b)
+            constexpr int P = INTER && V > 1 ? 2 : 1, W = V / P;
+#pragma unroll
+            for (int k = 0; k < P; ++k) {
+                const int angle = k ? slot[s].angle_b : slot[s].angle;
+                const bool turned = slot[s].a >= 0 && angle >= 0 && at >= 0;
+                float x[W], y[W];
+#pragma unroll
+                for (int i = 0; i < W; ++i) {
+                    x[i] = turned ? NAN : 1.f;  // (a position beyond the table)
+                    y[i] = 0.f;
+                }
+                if (turned && at < p.table) {
+                    load_vec<float, W>(x, p.cos + (long)at * half + angle);
+                    load_vec<float, W>(y, p.sin + (long)at * half + angle);
+                }
+#pragma unroll
+                for (int i = 0; i < W; ++i) {
+                    co[s][k * W + i] = x[i];
+                    si[s][k * W + i] = y[i];
+                }
+            }
+        }
+    };
+    float co[SPL][V], si[SPL][V];
+    int ahead = 0;  // the place of the next unit
+    // (whole warps go round together: the shuffles below are over groups of lanes of one warp)
+    const unsigned u1 = (unsigned)block * groups, step = (unsigned)sd.blocks * groups;
+    if constexpr (kRing > 0)
+#pragma unroll
+        for (int i = 0; i < kRing - 1; ++i) {
+            fetch(u1 + i * step + group, i);
+            cp_async_commit();
+        }
+    if constexpr (kRing > 0) {
+        turns(place(unit(u1 + group)), co, si);
+        ahead = place(unit(u1 + step + group));
+    }
+    int stage = 0;
+    for (unsigned u0 = u1; u0 < units; u0 += step) {
+        const Unit r = unit(u0 + group);
+        const unsigned token = r.token;
+        const int h0 = r.h0, heads = r.heads;
+        T *y = static_cast<T *>(sd.y) + ((long)token * sd.heads + h0) * p.D;
+        // as they lie in memory, all heads' loads in flight together
+        Vec<T, V> raw[HEADS * SPL][kPieces];
+        if constexpr (kRing > 0) {
+            // a thread reads what it fetched itself, and fetches where it read a round ago
+            cp_async_wait<kRing - 2>();
+            const int next = stage == 0 ? kRing - 1 : stage - 1;
+            fetch(u0 + (kRing - 1) * step + group, next);
+            cp_async_commit();
+#pragma unroll
+            for (int i = 0; i < HEADS * SPL; ++i)
+#pragma unroll
+                for (int k = 0; k < kPieces; ++k) raw[i][k] = ring[(((size_t)stage * HEADS * SPL + i) * kPieces + k) * kBlock];
+            stage = stage == kRing - 1 ? 0 : stage + 1;
+        } else {
+            vectors(r, [&](int at, int piece, const T *from, bool there) {
+#pragma unroll
+                for (int i = 0; i < V; ++i) raw[at][piece].v[i] = from_f32<T>(0.f);
+                if (there) raw[at][piece] = *reinterpret_cast<const Vec<T, V> *>(from);
+            });
+        }
+        if constexpr (kRing == 0) turns(place(r), co, si);
         Packed<V> c[SPL], sn[SPL];  // forward: with the weights
 #pragma unroll
         for (int s = 0; s < SPL; ++s) {
-            const bool turned = slot[s].a >= 0 && slot[s].angle >= 0 && at >= 0;
-            float co[V], si[V];
-#pragma unroll
-            for (int i = 0; i < V; ++i) {
-                co[i] = turned ? NAN : 1.f;  // (a position beyond the table)
-                si[i] = 0.f;
-            }
-            if (turned && at < p.table) {
-                load_vec<float, V>(co, p.cos + (long)at * half + slot[s].angle);
-                load_vec<float, V>(si, p.sin + (long)at * half + slot[s].angle);
-            }
             if (BACKWARD)
 #pragma unroll
-                for (int i = 0; i < V; ++i) si[i] = -si[i];
-            angles<V>(c[s], sn[s], co, si, INTER);
+                for (int i = 0; i < V; ++i) si[s][i] = -si[s][i];
+            angles<V>(c[s], sn[s], co[s], si[s], INTER);
             if constexpr (!BACKWARD) {
                 Packed<V> ws;
 #pragma unroll
@@ -254,14 +341,18 @@ __global__ void __launch_bounds__(kBlock, 2) norm_rotate_kernel(const NormArgs p
                 }
             }
         }
+        if constexpr (kRing > 0) {
+            turns(ahead, co, si);
+            ahead = place(unit(u0 + 2 * step + group));
+        }
 #pragma unroll
         for (int h = 0; h < HEADS; ++h) {
             Packed<V> xv[SPL], gv[SPL];
             f32x2 sq2 = 0ull;
 #pragma unroll
             for (int s = 0; s < SPL; ++s) {
-                widen<T, V>(xv[s], raw[h][s][0], raw[h][s][1]);
-                if constexpr (BACKWARD) widen<T, V>(gv[s], raw[h][s][2], raw[h][s][3]);
+                widen<T, V>(xv[s], raw[h * SPL + s][0], raw[h * SPL + s][1]);
+                if constexpr (BACKWARD) widen<T, V>(gv[s], raw[h * SPL + s][2], raw[h * SPL + s][3]);
 #pragma unroll
                 for (int i = 0; i < N; ++i) sq2 = fma2(xv[s].v[i], xv[s].v[i], sq2);
             }
@@ -307,6 +398,10 @@ __global__ void __launch_bounds__(kBlock, 2) norm_rotate_kernel(const NormArgs p
             }
         }
     }
+    if constexpr (kRing > 0) {
+        cp_async_wait<0>();
+        __syncthreads();  // (the sums below lie where the ring did)
+    }
     if constexpr (BACKWARD) {
         if (!sd.part) return;
 #pragma unroll
@@ -346,25 +441,39 @@ int launch(NormArgs &p, int sms, cudaStream_t stream) {
     const int groups = kBlock / p.lanes;
     const long rows = (long)p.B * p.T * (p.side[0].heads + p.side[1].heads);
     const bool many = rows >= 8L * sms * groups;  // four blocks an SM with two heads to a group
+    // two blocks an SM with a ring, where each goes round at least eight times: 4 x 8192 tokens of 32 + 8 bf16 heads of 128 take 305 us
+    // for both passes, 338 without it; 64 x 197 tokens of 6 + 6 fp32 heads of 64, which go round twice, 59 with it and 55 without
+    const bool ring = sizeof(T) * V == 16 && rows >= 8L * 2 * sms * groups * kMany;
     long blocks[2];
     for (int i = 0; i < 2; ++i) {
         const int hc = many ? kMany : 1;
         const long units = (long)p.B * p.T * ((p.side[i].heads + hc - 1) / hc);
-        const long most = norm_rotate_blocks(sms) * (long)p.side[i].heads / (p.side[0].heads + p.side[1].heads);
+        const long most = (ring ? 2L * sms : norm_rotate_blocks(sms)) * (long)p.side[i].heads / (p.side[0].heads + p.side[1].heads);
         blocks[i] = (units + groups - 1) / groups;
         if (blocks[i] > most) blocks[i] = most > 0 ? most : 1;
         p.side[i].blocks = (int)blocks[i];
     }
     if (BACKWARD && p.side[1].part) p.side[1].part = p.side[1].part + (size_t)blocks[0] * p.D;
-    const size_t smem = BACKWARD ? sizeof(float) * groups * p.D : 0;
     const int grid = (int)(blocks[0] + blocks[1]);
-    if (many)
-        (p.interleaved ? norm_rotate_kernel<T, V, SPL, kMany, true, BACKWARD> : norm_rotate_kernel<T, V, SPL, kMany, false, BACKWARD>)
-            <<<grid, kBlock, smem, stream>>>(p);
-    else
-        (p.interleaved ? norm_rotate_kernel<T, V, SPL, 1, true, BACKWARD> : norm_rotate_kernel<T, V, SPL, 1, false, BACKWARD>)
-            <<<grid, kBlock, smem, stream>>>(p);
-    int rc = launch_status();
+    const auto run = [&](auto kernel, size_t ring_bytes) {
+        const size_t sums = BACKWARD ? sizeof(float) * groups * p.D : 0, smem = ring_bytes > sums ? ring_bytes : sums;
+        if (smem > 48 * 1024 && !cuda_ok(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem))) return LUTGEMM_E_CUDA;
+        kernel<<<grid, kBlock, smem, stream>>>(p);
+        return launch_status();
+    };
+    int rc = LUTGEMM_OK;
+    if constexpr (sizeof(T) * V == 16) {
+        constexpr size_t kBytes = (size_t)kStages * kMany * SPL * (BACKWARD ? 4 : 2) * kBlock * 16;
+        if (ring)
+            rc = p.interleaved ? run(norm_rotate_kernel<T, V, SPL, kMany, true, true, BACKWARD>, kBytes)
+                               : run(norm_rotate_kernel<T, V, SPL, kMany, false, true, BACKWARD>, kBytes);
+    }
+    if (!ring && many)
+        rc = p.interleaved ? run(norm_rotate_kernel<T, V, SPL, kMany, true, false, BACKWARD>, 0)
+                           : run(norm_rotate_kernel<T, V, SPL, kMany, false, false, BACKWARD>, 0);
+    else if (!ring)
+        rc = p.interleaved ? run(norm_rotate_kernel<T, V, SPL, 1, true, false, BACKWARD>, 0)
+                           : run(norm_rotate_kernel<T, V, SPL, 1, false, false, BACKWARD>, 0);
     if (rc == LUTGEMM_OK && BACKWARD && (p.side[0].part || p.side[1].part)) {
         norm_weight_sums_kernel<<<dim3((p.D + 31) / 32, 2), 1024, 0, stream>>>(p);
         rc = launch_status();
