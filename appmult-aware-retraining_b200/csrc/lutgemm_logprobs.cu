@@ -9,14 +9,16 @@
 // sums over all classes; where 1 + s comes out below 2, the one thread that has m sums those around it again without it.
 //     grad_j = g_logp (1[j is given] - p_j) - g_entropy p_j (log p_j + entropy);   1 - p = -expm1(log p) for the given class
 //
-// DRAM bounds both directions: logits once in, in the backward pass once more, and the gradient once out.  A block has a row, or
-// a part of one where there are few rows; every thread keeps (m, 1 + s, u) of its own values, four vectors at a time, so that the
-// maximum is looked at once for 32 values of 16 bits, and the block joins them.  It also keeps which four vectors hold its
-// largest value and how large the others get: a second look at values (below, and above) is then one more load, not a pass.
-// The most probable classes come from the same pass at little cost: the k-th largest of the thread groups' largest logits is a
-// bound that at least k values reach, so only threads whose own largest value reaches it look at their values once more, and the
-// candidates are ranked by counting.  Ties go to the lower class.  Rows with so many
-// ties that the candidates do not fit are gone through once per answer instead.
+// DRAM bounds the gradient (logits in, gradient out), issued instructions the forward pass.  A block has a row, or a part of one where
+// there are few rows; every thread keeps (m, 1 + s, u) of its own values, four vectors at a time, so that the maximum is looked at
+// once for 32 values of 16 bits, and the block joins them.  It also keeps which four vectors hold its largest value and how large
+// the others get: a second look at values (below, and above) is then one more load, not a pass.  The most probable classes come
+// from the same pass: the k-th largest of the thread groups' largest logits is a bound that at least k values reach, so only
+// threads whose own largest value reaches it look at their values once more, and the candidates are ranked by counting.  Ties go
+// to the lower class.  Rows with so many ties that the candidates do not fit are gone through once per answer instead.
+//
+// 8192 rows of 32001 bf16 classes with 5 answers: 128 us (4.1 TB/s, 74 % of the issue slots; 178 before states were joined maximum first
+// and offers were made from bits), gradient 214 us (1.05 GB, 4.7 TB/s).
 #include "lutgemm.h"
 #include "lutgemm_attention.cuh"
 #include "lutgemm_f32x2.cuh"
@@ -130,8 +132,10 @@ struct Share {
         for (int k = 0; k < 4; ++k)
             if (k < have)
 #pragma unroll
-                for (int i = 0; i < n; ++i) one(first + head + (threadIdx.x + (r * 4 + k) * THREADS) * n + i, w[k].get(i));
+                for (int i = 0; i < n; ++i) one(place(r, k) + i, w[k].get(i));
     }
+    // of this thread's k-th vector of a round
+    __device__ __forceinline__ int place(int r, int k) const { return first + head + (threadIdx.x + (r * 4 + k) * THREADS) * n; }
     template <typename One>
     __device__ __forceinline__ void every(One one) const {
         for (int r = -1; r < rounds(); ++r) round(r, one);
@@ -169,16 +173,52 @@ __device__ __forceinline__ void block_sync() {
     if (THREADS == 32) __syncwarp(); else __syncthreads();
 }
 
-// the states of a block's threads joined, for all of them
+// the states of a block's threads joined, for all of them: the largest value first, then the sums relative to it (a join of two states
+// at every step of the exchange would take an exponential and the same sums each time)
 template <int THREADS>
-__device__ __forceinline__ RowState join_block(RowState all, RowState *shared) {
+__device__ __forceinline__ RowState join_block(const ThreadState &st, float (*shared)[3]) {
+    float m = st.m;
+#pragma unroll
+    for (int d = 16; d; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
+    if (THREADS > 32) {
+        if (threadIdx.x % 32 == 0) shared[threadIdx.x / 32][0] = m;
+        __syncthreads();
+        m = shared[0][0];
+#pragma unroll
+        for (int w = 1; w < THREADS / 32; ++w) m = fmaxf(m, shared[w][0]);
+    }
+    // (nothing but -inf: no sums of its own; a NaN among them stays in s)
+    const float e = st.m == m ? 1.f : __expf(st.m - m), all = st.all();
+    float s = all * e, u = st.m == -INFINITY ? 0.f : st.m == m ? st.u : e * (st.u + (m - st.m) * all);
+#pragma unroll
+    for (int d = 16; d; d >>= 1) {
+        s += __shfl_xor_sync(0xffffffffu, s, d);
+        u += __shfl_xor_sync(0xffffffffu, u, d);
+    }
+    if (THREADS > 32) {
+        if (threadIdx.x % 32 == 0) {
+            shared[threadIdx.x / 32][1] = s;
+            shared[threadIdx.x / 32][2] = u;
+        }
+        __syncthreads();
+        s = u = 0.f;
+#pragma unroll
+        for (int w = 0; w < THREADS / 32; ++w) {
+            s += shared[w][1];
+            u += shared[w][2];
+        }
+    }
+    return {m, m == -INFINITY && s == 0.f ? -1.f : m == -INFINITY ? s : s - 1.f, u};
+}
+// the states of parts joined one by one, so that s of the part with the largest value keeps its bits; for all threads of a block
+template <int THREADS>
+__device__ __forceinline__ RowState join_states(RowState all, RowState *shared) {
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
         const RowState other{__shfl_xor_sync(0xffffffffu, all.m, d), __shfl_xor_sync(0xffffffffu, all.s, d), __shfl_xor_sync(0xffffffffu, all.u, d)};
         // (both lanes join in the same order, so that they agree)
         all = threadIdx.x & d ? join(other, all) : join(all, other);
     }
-    if (THREADS == 32) return all;
     if (threadIdx.x % 32 == 0) shared[threadIdx.x / 32] = all;
     __syncthreads();
     all = shared[0];
@@ -226,11 +266,11 @@ __device__ __forceinline__ float logp_of(float x, float m, float L) { return m =
 template <typename T, int THREADS, bool TOP>
 __global__ void __launch_bounds__(THREADS) token_logprobs_kernel(const LogpArgs p) {
     constexpr int kGroup = THREADS >= 64 ? THREADS / 64 : 1, kGroups = THREADS / kGroup, kWarps = THREADS / 32;
-    __shared__ RowState states[kWarps];
-    __shared__ float group_top[TOP ? kGroups : 1];
+    __shared__ float states[kWarps][3];
+    __shared__ __align__(16) float group_top[TOP ? kGroups : 4];
     __shared__ unsigned long long cand[TOP ? kCandidates : 1];
     __shared__ int count;
-    __shared__ float bound;
+    __shared__ uint32_t bound;  // in the order of whole numbers; 0: none
     const long row = blockIdx.x;
     const int part = blockIdx.y, first = part * p.part_len, end = min(p.C, first + p.part_len);
     const T *x = static_cast<const T *>(p.x) + row * p.pitch;
@@ -284,9 +324,7 @@ __global__ void __launch_bounds__(THREADS) token_logprobs_kernel(const LogpArgs 
         });
     }
     const float mine = st.m;
-    // (of nothing but -inf: the empty state; a NaN among them stays)
-    RowState all = mine == -INFINITY ? RowState{mine, st.all() == 0.f ? -1.f : st.all(), 0.f} : RowState{mine, st.all() - 1.f, st.u};
-    all = join_block<THREADS>(all, states);
+    RowState all = join_block<THREADS>(st, states);
     if (all.m > -INFINITY && all.s < 1.f) {
         // one class has m, and s may be all rounding of 1 + s: the sum around it without it
         float sum = st.all() * __expf(mine - all.m);  // (0 where nothing was seen)
@@ -295,14 +333,14 @@ __global__ void __launch_bounds__(THREADS) token_logprobs_kernel(const LogpArgs 
             share.round(st.at, [&](int, float v) { sum += v == all.m ? 0.f : __expf(v - all.m); });
         }
         block_sync<THREADS>();
-        all.s = sum_block<THREADS>(sum, reinterpret_cast<float *>(states));
+        all.s = sum_block<THREADS>(sum, &states[0][0]);
     }
     if (TOP) {
         float gt = mine;
 #pragma unroll
         for (int d = 1; d < kGroup; d <<= 1) gt = fmaxf(gt, __shfl_xor_sync(0xffffffffu, gt, d));
         if (threadIdx.x % kGroup == 0) group_top[threadIdx.x / kGroup] = gt;
-        if (threadIdx.x == 0) { count = 0; bound = -INFINITY; }
+        if (threadIdx.x == 0) count = 0, bound = 0;
     }
     if (threadIdx.x == 0) {
         if (p.parts == 1) {
@@ -316,29 +354,46 @@ __global__ void __launch_bounds__(THREADS) token_logprobs_kernel(const LogpArgs 
     const int top = min(p.top, end - first);
     block_sync<THREADS>();
     if ((int)threadIdx.x < kGroups) {
-        // the top-th largest of the groups' largest values, where there are as many groups
+        // the top-th largest of the groups' largest values, where there are as many groups: the largest that as many reach
         const float v = group_top[threadIdx.x];
-        int above = 0, equal = 0;
-        for (int i = 0; i < kGroups; ++i) {
-            above += group_top[i] > v;
-            equal += group_top[i] == v;
+        int reach = 0;
+#pragma unroll
+        for (int i = 0; i < kGroups; i += 4) {
+            const float4 g = *reinterpret_cast<const float4 *>(group_top + i);
+            reach += (g.x >= v) + (g.y >= v) + (g.z >= v) + (g.w >= v);
         }
-        if (above < top && above + equal >= top) bound = v;
+        if (reach >= top) atomicMax(&bound, order_of(v));
     }
     block_sync<THREADS>();
-    const float least = bound;
+    const float least = bound ? value_of((unsigned long long)bound << 32) : -INFINITY;
     const bool odd = isnan(all.s);  // NaN among the logits: the bound says nothing of them
     if (mine >= least || odd) {
         auto offer = [&](int j, float v) {
-            if (v >= least || v != v) {
+            if (!(v < least)) {
                 const int at = atomicAdd(&count, 1);
                 if (at < kCandidates) cand[at] = key_of(v, j);
             }
         };
-        if (odd || st.second >= least)
-            share.every(offer);
-        else
-            share.round(st.at, offer);
+        // (which values of a round reach it as bits: code for an offer in every place would not fit the instruction cache)
+        auto look = [&](int r) {
+            Wide<T> w[4];
+            constexpr int n = Wide<T>::n;
+            const int have = share.load(w, r);
+            uint32_t hits = 0;
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                if (k < have)
+#pragma unroll
+                    for (int i = 0; i < n; ++i) hits |= w[k].get(i) < least ? 0u : 1u << (k * n + i);
+            for (; hits; hits &= hits - 1) {
+                const int at = __ffs(hits) - 1, j = share.place(r, at / n) + at % n;
+                offer(j, to_f32<T>(x[j]));
+            }
+        };
+        const bool all_rounds = odd || st.second >= least;
+        if (all_rounds || st.at < 0) share.ends(offer);
+        for (int r = all_rounds ? 0 : st.at, end = all_rounds ? share.rounds() : r + 1; r < end; ++r)
+            if (r >= 0) look(r);
     }
     block_sync<THREADS>();
     const float m = all.m, L = p.parts == 1 ? p.stats[row * 3 + 1] : 0.f;
@@ -395,7 +450,7 @@ __global__ void __launch_bounds__(256) token_logprobs_join_kernel(const LogpArgs
         bound = 0;
     }
     const RowState mine = (int)threadIdx.x < p.parts ? p.part_state[row * p.parts + threadIdx.x] : RowState{-INFINITY, -1.f, 0.f};
-    const RowState all = join_block<256>(mine, states);
+    const RowState all = join_states<256>(mine, states);
     if (threadIdx.x == 0) finish_row(p, row, all, given);
     if (!p.top) return;
     __syncthreads();
@@ -519,9 +574,12 @@ void launch_forward(const LogpArgs &p, cudaStream_t stream) {
 
 template <typename T>
 int forward(LogpArgs &p, cudaStream_t stream) {
-    // a warp for short rows, four warps for rows that fit many to an SM, sixteen for the longest
-    if (p.part_len <= 512 && p.parts == 1)
+    // a warp for short rows, two warps for longer ones (20000 x 1000 fp32: 41 us with one, 59 with two, 86 with four; 8192 x 4097 bf16:
+    // 61 us with two, 65 with four), four for rows that fit many to an SM (8192 x 32001: 182 us, 195 with two), sixteen for the longest
+    if (p.part_len <= (p.N >= 2048 ? 1024 : 512))
         launch_forward<T, 32>(p, stream);
+    else if (p.part_len <= 6144)
+        launch_forward<T, 64>(p, stream);
     else if (p.part_len <= 65536)
         launch_forward<T, 128>(p, stream);
     else

@@ -14,7 +14,7 @@
 // (each thread reads what it asked for itself, so the ring needs no barrier) and the next angles in registers.  The blocks are
 // split between queries and keys, in proportion; weights then stay with a block, and so do the sums of their gradients: per lane
 // in registers, per block in shared memory, over the blocks by a second kernel in ascending order, so results do not depend on
-// timing.  4 x 8192 tokens of 32 + 8 bf16 heads of 128: 304 us for both passes (1.68 GB, 5.5 TB/s).
+// timing.  4 x 8192 tokens of 32 + 8 bf16 heads of 128: 113 us forward (0.67 GB, 5.9 TB/s), 179 us backward (1.01 GB, 5.6 TB/s).
 #include "lutgemm.h"
 #include "lutgemm_attention.cuh"
 #include "lutgemm_common.cuh"
