@@ -84,6 +84,8 @@ __global__ void __launch_bounds__(256) attention_delta_kernel(const AttnProblem 
 // out of fp16's subnormal range whatever the scale of the loss.
 // fp32: P and dS are split into planes as the operands were; there is one group, and each round's sums start from zero and are added up
 // in registers (in the accumulators, what additions cut off came to 2e-5 of the gradients of 4096 rows).
+// The workers' instructions per score bound both kernels.  2 x 4096, 16 / 4 heads of 128, bf16: 546 us with keys kept (256 blocks, not two
+// whole rounds of the GPU), 435 with rows kept; 719 TFLOP/s of the formula's five products, tensor pipe 58 and 49 %.
 template <typename T, int DP, bool BENT, bool KEYS>
 struct GradLayout {
     using Op = Operand<T, DP>;
