@@ -12,7 +12,7 @@
 // are loaded once for them and their loads are in flight together; a grid of few tokens takes one head per group instead, so that
 // it spreads over the GPU.  Where groups go round often, the loads of the next two rounds are under way in a ring in shared memory
 // (each thread reads what it asked for itself, so the ring needs no barrier) and the next angles in registers.  The blocks are
-// split between queries and keys, in proportion; weights then stay with a block, and so do the sums of their gradients: per lane
+// split between queries and keys, by their groups' turns; weights then stay with a block, and so do the sums of their gradients: per lane
 // in registers, per block in shared memory, over the blocks by a second kernel in ascending order, so results do not depend on
 // timing.  4 x 8192 tokens of 32 + 8 bf16 heads of 128: 113 us forward (0.67 GB, 5.9 TB/s), 179 us backward (1.01 GB, 5.6 TB/s).
 #include "lutgemm.h"
@@ -444,11 +444,14 @@ int launch(NormArgs &p, int sms, cudaStream_t stream) {
     // two blocks an SM with a ring, where each goes round at least eight times: 4 x 8192 tokens of 32 + 8 bf16 heads of 128 take 305 us
     // for both passes, 338 without it; 64 x 197 tokens of 6 + 6 fp32 heads of 64, which go round twice, 59 with it and 55 without
     const bool ring = sizeof(T) * V == 16 && rows >= 8L * 2 * sms * groups * kMany;
+    // blocks by turns of groups, which take as long for one head as for several (by heads, 4 x 8192 tokens of 16 + 1 bf16 heads of 128 took
+    // 120 us forward, by turns 58)
+    const auto share = [&](int i) { return (long)(p.side[i].heads + (many ? kMany - 1 : 0)) / (many ? kMany : 1); };
     long blocks[2];
     for (int i = 0; i < 2; ++i) {
         const int hc = many ? kMany : 1;
         const long units = (long)p.B * p.T * ((p.side[i].heads + hc - 1) / hc);
-        const long most = (ring ? 2L * sms : norm_rotate_blocks(sms)) * (long)p.side[i].heads / (p.side[0].heads + p.side[1].heads);
+        const long most = (ring ? 2L * sms : norm_rotate_blocks(sms)) * share(i) / (share(0) + share(1));
         blocks[i] = (units + groups - 1) / groups;
         if (blocks[i] > most) blocks[i] = most > 0 ? most : 1;
         p.side[i].blocks = (int)blocks[i];

@@ -256,7 +256,7 @@ def test_the_most_rows_of_a_batch(dtype, D):
 @pytest.mark.parametrize("B,T,H,G,D,rot,layout,place,dtype", [
     (2, 8195, 17, 5, 128, 64, "interleaved", False, torch.bfloat16), (3, 5003, 21, 3, 128, 128, "half", True, torch.float16),
     (1, 20011, 8, 8, 80, 40, "half", True, torch.float32), (2, 9001, 7, 3, 128, 0, "half", False, torch.float32),
-    (1, 40003, 13, 3, 48, 16, "interleaved", True, torch.bfloat16)])
+    (1, 40003, 13, 3, 48, 16, "interleaved", True, torch.bfloat16), (1, 16001, 40, 1, 64, 64, "half", False, torch.float16)])
 def test_norm_rotate_of_many_rows(B, T, H, G, D, rot, layout, place, dtype):
     import test_gpu_operators
     test_gpu_operators.test_norm_rotate(B, T, H, G, D, rot, layout, place, dtype)
