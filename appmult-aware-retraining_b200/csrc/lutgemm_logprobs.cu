@@ -39,11 +39,14 @@ __device__ __forceinline__ float exp2_approx(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+// sum of exp(-(d + d_j)) (d + d_j) from all = sum of exp(-d_j) and u = sum of exp(-d_j) d_j, with e = exp(-d).  Nothing where e is 0: d, from
+// logits masked with a type's lowest value, may be so large that its product with a sum is infinite.  (A NaN is in the sums themselves.)
+__device__ __forceinline__ float farther(float e, float d, float all, float u) { return e == 0.f ? 0.f : e * (u + d * all); }
 __device__ __forceinline__ RowState join(const RowState &a, const RowState &b) {
     const RowState &x = a.m >= b.m ? a : b, &y = a.m >= b.m ? b : a;
     if (y.m == -INFINITY) return {x.m, x.s + (y.s == -1.f ? 0.f : y.s), x.u};  // (a NaN in y.s stays)
     const float d = x.m - y.m, e = __expf(-d), n = 1.f + y.s;
-    return {x.m, x.s + e * n, x.u + e * (y.u + d * n)};
+    return {x.m, x.s + e * n, x.u + farther(e, d, n, y.u)};
 }
 // order of values by whole numbers: NaN above +inf, -0 as 0 (no key is all ones: that is where the search for ties begins)
 constexpr uint32_t kNanOrder = 0xfffffffeu;
@@ -156,7 +159,7 @@ struct ThreadState {
         }
         const float d = top - m, e = __expf(-d);  // (0 from -inf)
         rest += best;
-        u = m == -INFINITY ? u : e * (u + d * rest);
+        u = farther(e, d, rest, u);
         rest *= e;
         best = 0.f;
         second = m;
@@ -189,7 +192,7 @@ __device__ __forceinline__ RowState join_block(const ThreadState &st, float (*sh
     }
     // (nothing but -inf: no sums of its own; a NaN among them stays in s)
     const float e = st.m == m ? 1.f : __expf(st.m - m), all = st.all();
-    float s = all * e, u = st.m == -INFINITY ? 0.f : st.m == m ? st.u : e * (st.u + (m - st.m) * all);
+    float s = all * e, u = st.m == -INFINITY ? 0.f : st.m == m ? st.u : farther(e, m - st.m, all, st.u);
 #pragma unroll
     for (int d = 16; d; d >>= 1) {
         s += __shfl_xor_sync(0xffffffffu, s, d);

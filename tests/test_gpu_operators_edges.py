@@ -1,0 +1,73 @@
+"""Where head norms, attention and log probabilities meet the ends of their types' ranges, rows that are not there, and derivatives
+that they do not have; on a GPU."""
+import pytest
+import torch
+
+import operators_reference as R
+from test_gpu_operators import DTYPES, IDS, close, gen, randn, rounding
+
+pytestmark = pytest.mark.gpu
+
+
+def logprobs(*args, **kw):
+    import lutgemm_loss
+    return lutgemm_loss.token_logprobs(*args, **kw)
+
+
+def check_logprobs(x, targets, top, g_logp, g_entropy):
+    """Results and gradients against 64 bits.  Classes farther than 745 below a row's largest have no probability in 64 bits and none in
+    32; the others are `spread` apart at most.  Their distances to the largest are exact to f = 2^-24 of themselves, exponentials to
+    (spread + 4) f (of a rounded product), sums of positive terms, in runs and trees of at most 512, to 600 f, the logarithm to 4 f."""
+    x = x.detach().requires_grad_(True)
+    logp, entropy, top_logp, top_index = logprobs(x, targets, top)
+    both = torch.autograd.grad((logp, entropy), x, (g_logp, g_entropy), retain_graph=True)[0]
+    only = torch.autograd.grad(logp, x, g_logp)[0]
+    xd, f, u = x.detach().double(), 2.0 ** -24, rounding(x.dtype)
+    want = R.token_logprobs(xd, targets, top)
+    assert torch.equal(top_index, want[3])
+    m = xd.amax(1)
+    near = xd >= m[:, None] - 745
+    spread = m - xd.masked_fill(~near, torch.inf).amin(1)
+    rel = (2 * spread + 650) * f
+    others = (torch.logsumexp(xd, 1) - m).clamp(max=1.0)  # (L is off by at most rel * min(L, 1))
+    e_logp = 4 * f * (want[0].abs() + spread + 1) + rel * others
+    close(logp, want[0], e_logp, "logp")
+    close(entropy, want[1], (rel + 8 * f) * (want[1] + torch.logsumexp(xd, 1) - m) + 1e-30, "entropy")
+    close(top_logp, want[2], 4 * f * (want[2].abs() + spread[:, None] + 1) + (rel * others)[:, None], "top_logp")
+    logs, p = torch.log_softmax(xd, 1), torch.softmax(xd, 1)
+    hot = torch.zeros_like(p).scatter_(1, targets.clamp(min=0)[:, None], 1.0)
+    gl, ge = torch.where(targets == -100, 0.0, g_logp.double())[:, None], g_entropy.double()[:, None]
+    rest = torch.where(hot > 0, -torch.expm1(logs), -p)
+    tail = torch.where(p > 0, p * (logs.masked_fill(p == 0, 0.0) + want[1][:, None]), 0.0)
+    per = rel[:, None] + 8 * f  # of a probability
+    e = gl.abs() * (rest.abs() + hot * p) * per
+    # (below 2^-126 fp32 probabilities are nothing)
+    e_both = e + ge.abs() * (tail.abs() * per + p * 8 * f * (spread[:, None] + 1 + want[1][:, None])) + ge.abs() * 2.0 ** -126 * 100
+    tiny = (2.0 ** -25 if x.dtype is torch.float16 else 0.0) + 2.0 ** -126 * (1 + gl.abs())
+    close(only, gl * rest, u * (gl * rest).abs() + e + tiny, "gradient of logp alone")
+    close(both, gl * rest - ge * tail, u * (gl * rest - ge * tail).abs() + e_both + tiny, "gradient")
+
+
+# rows masked with the type's lowest value, which is not infinite: (rows, classes, which ones are left)
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("N,C,left", [(64, 64, "half"), (9, 40, "three"), (700, 1000, "half"), (5, 5000, "half"), (3, 32001, "three"),
+                                      (2500, 1024, "three"), (1, 128257, "start"), (2, 200003, "end"), (3, 100001, "three")])
+def test_logits_masked_with_the_lowest_value(N, C, left, dtype):
+    g = gen(N + C)
+    x = (2 * randn(g, N, C)).to(dtype)
+    if left == "half":
+        keep = torch.rand(N, C, generator=g, device="cuda") < 0.5
+    else:
+        keep = torch.zeros(N, C, dtype=torch.bool, device="cuda")
+        if left == "three":
+            keep.scatter_(1, torch.randint(0, C, (N, 3), generator=g, device="cuda"), True)
+        elif left == "start":  # whole parts of the row are masked
+            keep[:, :100] = True
+        else:
+            keep[:, -100:] = True
+    keep[:, C // 3] = keep[:, C // 3] | ~keep.any(1)
+    x = torch.where(keep, x, torch.finfo(dtype).min)
+    targets = x.float().argmax(1)
+    targets[1::2] = torch.randint(0, C, (N,), generator=g, device="cuda")[1::2]  # (masked ones among them)
+    targets[2::5] = -100
+    check_logprobs(x, targets, min(3, C), randn(g, N), randn(g, N))
