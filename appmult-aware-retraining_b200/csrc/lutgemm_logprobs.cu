@@ -532,8 +532,9 @@ __global__ void __launch_bounds__(256) token_logprobs_grad_kernel(const GradArgs
     const auto grads = [&](f32x2 x) {
         const f32x2 t = add2(x, from2);
         const float2 z = unpack2(fma2(t, log2e2, less2)), d = unpack2(t);
-        // (-inf: p is 0, and 0 * inf must not reach the product; a NaN reaches it through p)
-        return unpack2(mul2(pack2(exp2_approx(z.x), exp2_approx(z.y)), fma2(ge2, pack2(fmaxf(d.x, -1e30f), fmaxf(d.y, -1e30f)), gu2)));
+        // (p is 0 from a distance of 88 on, where the distance, infinite or times a large g_entropy, must not reach the product as an
+        // infinity; a NaN reaches it through p)
+        return unpack2(mul2(pack2(exp2_approx(z.x), exp2_approx(z.y)), fma2(ge2, pack2(fmaxf(d.x, -1e4f), fmaxf(d.y, -1e4f)), gu2)));
     };
     const auto grad = [&](int j, float x) {
         if (j != given) return grads(pack2(x, x)).x;

@@ -71,3 +71,20 @@ def test_logits_masked_with_the_lowest_value(N, C, left, dtype):
     targets[1::2] = torch.randint(0, C, (N,), generator=g, device="cuda")[1::2]  # (masked ones among them)
     targets[2::5] = -100
     check_logprobs(x, targets, min(3, C), randn(g, N), randn(g, N))
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("C", [33, 40000])
+def test_large_gradients_of_entropies_beside_classes_without_probability(C, dtype):
+    g = gen(C)
+    x = (2 * randn(g, 6, C)).to(dtype)
+    x[torch.rand(6, C, generator=g, device="cuda") < 0.3] = -torch.inf
+    x = x.requires_grad_(True)
+    entropy = logprobs(x, torch.zeros(6, dtype=torch.int64, device="cuda"))[1]
+    one = torch.autograd.grad(entropy, x, torch.ones(6, device="cuda"), retain_graph=True)[0]
+    # (a gradient is a product of g_entropy, so a power of two beyond it changes exponents alone; fp16 has no room for them)
+    many = torch.autograd.grad(entropy, x, torch.full((6,), 2.0 ** 40, device="cuda"))[0]
+    hidden = x.detach() == -torch.inf
+    assert not many[hidden].any()
+    if dtype is not torch.float16:
+        assert torch.equal(many, one * 2.0 ** 40)
