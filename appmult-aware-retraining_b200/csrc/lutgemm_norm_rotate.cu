@@ -358,7 +358,8 @@ __global__ void __launch_bounds__(kBlock, 2) norm_rotate_kernel(const NormArgs p
             }
             float sq = both(sq2);
             for (int d = p.lanes / 2; d; d >>= 1) sq += __shfl_xor_sync(0xffffffffu, sq, d);
-            const float r = rsqrtf(sq * inv_d + p.eps);
+            // (a head that is not there: zeros, also where eps is zero and the reciprocal infinite)
+            const float r = !BACKWARD || h < heads ? rsqrtf(sq * inv_d + p.eps) : 0.f;
             const f32x2 r2 = pack2(r, r);
             if constexpr (!BACKWARD) {
 #pragma unroll

@@ -4,7 +4,7 @@ import pytest
 import torch
 
 import operators_reference as R
-from test_gpu_operators import DTYPES, IDS, close, gen, randn, rounding
+from test_gpu_operators import DTYPES, IDS, close, gen, ops, randn, rounding
 
 pytestmark = pytest.mark.gpu
 
@@ -88,3 +88,33 @@ def test_large_gradients_of_entropies_beside_classes_without_probability(C, dtyp
     assert not many[hidden].any()
     if dtype is not torch.float16:
         assert torch.equal(many, one * 2.0 ** 40)
+
+
+# (B, T, H, G, D, rot, layout, type): groups of lanes without a head in the last turn, heads that do not fill a turn, loads that run ahead
+@pytest.mark.parametrize("B,T,H,G,D,rot,layout,dtype", [
+    (1, 197, 6, 6, 64, 64, "half", torch.float32), (1, 1, 1, 1, 8, 8, "half", torch.float32), (3, 33, 8, 2, 128, 64, "interleaved", torch.bfloat16),
+    (2, 1031, 5, 3, 64, 32, "half", torch.float16), (1, 13, 3, 1, 254, 254, "half", torch.float32), (2, 65, 4, 1, 80, 40, "half", torch.bfloat16),
+    (2, 8195, 17, 5, 128, 64, "interleaved", torch.bfloat16), (1, 20011, 7, 8, 80, 40, "half", torch.float32),
+    (3, 5003, 21, 3, 128, 128, "half", torch.float16)])
+def test_norms_without_eps(B, T, H, G, D, rot, layout, dtype):
+    g = gen(B + T + D)
+    q, k = (randn(g, B, T, n, D, dtype=dtype).requires_grad_(True) for n in (H, G))
+    qw, kw = ((1 + 0.2 * randn(g, D)).requires_grad_(True) for _ in range(2))
+    cos, sin = ops().rotary_tables(T, rot, device="cuda")
+    go = [randn(g, B, T, n, D, dtype=dtype) for n in (H, G)]
+    y = ops().norm_rotate(q, k, qw, kw, cos, sin, layout=layout, eps=0.0)
+    grads = torch.autograd.grad(y, (q, k, qw, kw), go)
+    u, f = rounding(dtype), 2.0 ** -24
+    for i, (x, w) in enumerate(((q, qw), (k, kw))):
+        xd, wd = x.detach().double().requires_grad_(True), w.detach().double().requires_grad_(True)
+        want = R.norm_rotate(xd, wd, cos, sin, None, layout, 0.0)
+        wx, ww = torch.autograd.grad(want, (xd, wd), go[i].double())
+        want, xd, god = want.detach(), xd.detach(), go[i].double()
+        # D/2 + 12 roundings of fp32 for a value, each of at most the largest of its head, and one of the type
+        close(y[i].detach(), want, u * want.abs() + (D + 24) * f * want.abs().amax(-1, keepdim=True), "y")
+        r = 1 / xd.square().mean(-1, keepdim=True).sqrt()
+        unit, most = xd * r, god.abs().amax(-1, keepdim=True) * 2 * wd.detach().abs().max()
+        close(grads[i], wx, u * wx.abs() + (D + 24) * f * r * most * (1 + unit.abs().amax(-1, keepdim=True) ** 2), "grad_x")
+        n = B * T * x.shape[2]
+        terms = (2 * god.abs().amax(-1, keepdim=True) * unit.abs()).sum((0, 1, 2))
+        close(grads[2 + i], ww, (min(n, 4096) + D + 24) * f * terms, "grad_w")
