@@ -64,8 +64,16 @@ Tensor scratch(size_t bytes, const Tensor &like) {
     return bytes ? at::empty({(int64_t)bytes}, like.options().dtype(at::kByte)) : Tensor();
 }
 void *stream_of(const Tensor &x) { return c10::cuda::getCurrentCUDAStream(x.get_device()).stream(); }
-void no_second_derivative(const char *what) {
+// a tangent that forward-mode differentiation has given a tensor would be lost: the result's derivative would be taken for zero
+void no_tangents(const char *what, std::initializer_list<const Tensor *> inputs) {
+    if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return;
+    for (const Tensor *x : inputs)
+        TORCH_CHECK(!x || !x->defined() || !x->_fw_grad(/*level=*/0).defined(), what, " has no forward-mode derivative");
+}
+const Tensor *given(const MaybeTensor &x) { return x.has_value() ? &*x : nullptr; }
+void no_second_derivative(const char *what, const variable_list &grads) {
     TORCH_CHECK(!at::GradMode::is_enabled(), what, " has no second derivative (create_graph=True)");
+    for (const Tensor &g : grads) no_tangents(what, {&g});
 }
 #define STRIDES(x) (long)(x).stride(0), (long)(x).stride(1), (long)(x).stride(2)
 
@@ -94,7 +102,7 @@ struct NormRotate : torch::autograd::Function<NormRotate> {
         return {out.first, out.second};
     }
     static variable_list backward(AutogradContext *ctx, variable_list grads) {
-        no_second_derivative("norm_rotate");
+        no_second_derivative("norm_rotate", grads);
         const variable_list saved = ctx->get_saved_variables();
         const Tensor &q = saved[0], &k = saved[1], &cos = saved[4], &sin = saved[5];
         const MaybeTensor qw = maybe(saved[2]), kw = maybe(saved[3]), positions = maybe(saved[6]);
@@ -126,6 +134,7 @@ std::pair<Tensor, Tensor> norm_rotate(const Tensor &q, const Tensor &k, const Ma
                                       const std::string &layout, double eps) {
     check_heads(q, "q");
     check_like(k, "k", q);
+    no_tangents("norm_rotate", {&q, &k, given(q_weight), given(k_weight), given(cos_table), given(sin_table)});
     const int64_t B = q.size(0), T = q.size(1), D = q.size(3);
     TORCH_CHECK(k.size(0) == B && k.size(1) == T && k.size(3) == D, "k has shape ", k.sizes(), ", expected [", B, ", ", T, ", heads, ", D, "]");
     TORCH_CHECK(q.size(2) > 0 && k.size(2) > 0 && D > 0 && D % 2 == 0 && D <= 256, "heads must be at least one of an even size up to 256, got ",
@@ -211,7 +220,7 @@ struct Attention : torch::autograd::Function<Attention> {
         return r.out;
     }
     static variable_list backward(AutogradContext *ctx, variable_list grads) {
-        no_second_derivative("attention");
+        no_second_derivative("attention", grads);
         const variable_list s = ctx->get_saved_variables();
         const Tensor &q = s[0], &k = s[1], &v = s[2], go = vectors(grads[0]);
         const Masks m{ctx->saved_data["scale"].toDouble(), ctx->saved_data["cap"].toDouble(), ctx->saved_data["causal"].toBool(), maybe(s[6]),
@@ -248,6 +257,7 @@ Tensor attention(const Tensor &q, const Tensor &k, const Tensor &v, c10::optiona
     check_heads(q, "q");
     check_like(k, "k", q);
     check_like(v, "v", q);
+    no_tangents("attention", {&q, &k, &v, given(slopes)});
     const int64_t B = q.size(0), Tq = q.size(1), H = q.size(2), D = q.size(3), Tk = k.size(1), G = k.size(2);
     TORCH_CHECK(k.size(0) == B && k.size(3) == D && k.sizes() == v.sizes(), "k and v must both be [", B, ", Tk, heads, ", D, "], got ", k.sizes(),
                 " and ", v.sizes());
@@ -318,7 +328,7 @@ struct TokenLogprobs : torch::autograd::Function<TokenLogprobs> {
         return out;
     }
     static variable_list backward(AutogradContext *ctx, variable_list grads) {
-        no_second_derivative("token_logprobs");
+        no_second_derivative("token_logprobs", grads);
         const variable_list s = ctx->get_saved_variables();
         const Tensor &logits = s[0];
         if (!grads[0].defined() && !grads[1].defined()) return {Tensor(), Tensor(), Tensor(), Tensor()};
@@ -339,6 +349,7 @@ struct TokenLogprobs : torch::autograd::Function<TokenLogprobs> {
 std::tuple<Tensor, Tensor, Tensor, Tensor> token_logprobs(const Tensor &logits, const Tensor &targets, int64_t top, int64_t ignore) {
     TORCH_CHECK(logits.is_cuda(), "logits must be a CUDAtensor");
     TORCH_CHECK(has_kernels(logits), "logits must be of type torch.float32, torch.bfloat16 or torch.float16");
+    no_tangents("token_logprobs", {&logits});
     TORCH_CHECK(logits.dim() >= 1 && logits.size(-1) > 0 && logits.size(-1) <= 0x7fffffffLL, "logits must be [..., classes], got ", logits.sizes());
     TORCH_CHECK(targets.scalar_type() == at::kLong && targets.device() == logits.device(), "targets must be of type torch.int64 on ",
                 logits.device());

@@ -4,8 +4,8 @@ on them with `attention="fused"`.
 
 Operands are CUDA tensors [B, T, heads, D] in fp32, bf16 or fp16, read by their strides (views of one projection's output need
 no copy; the last axis has to be contiguous), sums and statistics are fp32, results are contiguous and rounded once.  Calls run
-on the current stream of the operands' device and keep nothing; there are no second derivatives, and there is no fallback without
-the CUDA library."""
+on the current stream of the operands' device and keep nothing; second derivatives and forward-mode ones are refused, and there is no
+fallback without the CUDA library."""
 from __future__ import annotations
 
 import torch

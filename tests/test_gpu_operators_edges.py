@@ -118,3 +118,41 @@ def test_norms_without_eps(B, T, H, G, D, rot, layout, dtype):
         n = B * T * x.shape[2]
         terms = (2 * god.abs().amax(-1, keepdim=True) * unit.abs()).sum((0, 1, 2))
         close(grads[2 + i], ww, (min(n, 4096) + D + 24) * f * terms, "grad_w")
+
+
+def test_forward_mode_derivatives_are_refused():
+    """There are none, and a result without its tangent would be taken for one whose derivative is zero."""
+    import torch.autograd.forward_ad as forward_mode
+    g = gen(31)
+    q, k, v, w = randn(g, 1, 5, 2, 16), randn(g, 1, 5, 2, 16), randn(g, 1, 5, 2, 16), torch.ones(16, device="cuda")
+    cos, sin = ops().rotary_tables(5, 16, device="cuda")
+    x, t, slopes = randn(g, 5, 9), torch.arange(5, device="cuda"), torch.ones(2, device="cuda")
+    norm = dict(q=q, k=k, q_weight=w, k_weight=w, cos=cos, sin=sin)
+    attention = dict(q=q, k=k, v=v, slopes=slopes)
+    plain = [ops().norm_rotate(**norm)[0], ops().attention(**attention), logprobs(x, t)[0]]
+    learned = q.clone().requires_grad_(True)
+    with forward_mode.dual_level():
+        def dual(y):
+            return forward_mode.make_dual(y, torch.ones_like(y))
+        for grads in (torch.enable_grad, torch.no_grad):
+            with grads():
+                for name in norm:
+                    with pytest.raises(RuntimeError, match="forward-mode"):
+                        ops().norm_rotate(**{**norm, name: dual(norm[name])})
+                for name in attention:
+                    with pytest.raises(RuntimeError, match="forward-mode"):
+                        ops().attention(**{**attention, name: dual(attention[name])})
+                with pytest.raises(RuntimeError, match="forward-mode"):
+                    ops().attention(dual(q), k[:, :0], v[:, :0])  # nothing to see
+                with pytest.raises(RuntimeError, match="forward-mode"):
+                    logprobs(dual(x), t)
+                # tensors without a tangent, and a primal, are as they were
+                same = [ops().norm_rotate(**norm)[0], ops().attention(**attention), logprobs(forward_mode.unpack_dual(dual(x)).primal, t)[0]]
+                assert all(torch.equal(a, b) for a, b in zip(same, plain))
+        # a gradient that carries a tangent
+        go = dual(q.clone())
+        for y, leaf, grad in ((ops().norm_rotate(learned, k)[0], learned, go), (ops().attention(learned, k, v), learned, go),
+                              (logprobs(learned.view(10, 16), torch.zeros(10, dtype=torch.int64, device="cuda"))[0], learned,
+                               dual(torch.ones(10, device="cuda")))):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                torch.autograd.grad(y, leaf, grad)
