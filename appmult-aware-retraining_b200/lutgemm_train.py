@@ -52,10 +52,13 @@ def build(device, bits: int, conv_impl: str = "layer", use_ste: bool = False, lr
 def train_step(model, opt, reducer, images, labels, fused_loss: bool = False):
     """One step: forward, cross-entropy, backward with the bucketed gradient all-reduce launched from hooks
     while backward runs (`reducer`: an OverlappedGradReducer over the model's parameters), optimizer step.  `fused_loss`: the
-    cross-entropy by `lutgemm_loss.token_logprobs` instead of PyTorch."""
+    cross-entropy by `lutgemm_loss.token_logprobs` instead of PyTorch, the mean over the labels that are not -100 too."""
     reducer.zero_grad()
     logits = model(images)
-    loss = -token_logprobs(logits, labels)[0].mean() if fused_loss else F.cross_entropy(logits, labels)
+    if fused_loss:
+        loss = -token_logprobs(logits, labels)[0].sum() / (labels != -100).sum()
+    else:
+        loss = F.cross_entropy(logits, labels)
     loss.backward()
     reducer.finish()
     opt.step()
@@ -79,19 +82,20 @@ def evaluate(model, batches):
 @torch.no_grad()
 def evaluate_top(model, batches, top: int = 5):
     """Over (images, labels) batches: top-1 and top-`top` accuracy, mean negative log probability of the labels and mean entropy of
-    the answers, in one pass over the logits (`lutgemm_loss.token_logprobs`); one read by the host, at the end."""
+    the answers, in one pass over the logits (`lutgemm_loss.token_logprobs`); one read by the host, at the end.  Images whose label is
+    -100 do not count; without any that does, all four are zero."""
     was_training = model.training
     model.eval()
-    sums, total = None, 0
+    sums = None
     for images, labels in batches:
         logp, entropy, _, answers = token_logprobs(model(images), labels, top=top)
-        hits = answers == labels[:, None]
-        batch = torch.stack([hits[:, 0].sum(), hits.sum(), -logp.double().sum(), entropy.double().sum()])
+        hits, given = answers == labels[:, None], labels != -100
+        batch = torch.stack([hits[:, 0].sum(), hits.sum(), -logp.double().sum(), torch.where(given, entropy, 0.0).double().sum(),
+                             given.sum()])
         sums = batch if sums is None else sums + batch
-        total += labels.numel()
     model.train(was_training)
     names = ("top1", f"top{top}" if top > 1 else "top1", "nll", "entropy")
-    return dict(zip(names, (sums / total).tolist() if total else (0.0,) * 4))
+    return dict(zip(names, (sums[:4] / sums[4].clamp(min=1)).tolist() if sums is not None else (0.0,) * 4))
 
 
 def main():

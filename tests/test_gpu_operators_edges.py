@@ -156,3 +156,39 @@ def test_forward_mode_derivatives_are_refused():
                                dual(torch.ones(10, device="cuda")))):
             with pytest.raises(RuntimeError, match="forward-mode"):
                 torch.autograd.grad(y, leaf, grad)
+
+
+def test_losses_leave_out_ignored_labels():
+    """The fused loss is F.cross_entropy, whose mean is over the labels that are not -100; so are the figures of an evaluation."""
+    import copy
+    import torch.nn.functional as F
+    from lutgemm_dp import OverlappedGradReducer
+    from lutgemm_train import evaluate_top, train_step
+    torch.manual_seed(5)
+    model = torch.nn.Linear(20, 30).cuda()
+    other, exact = copy.deepcopy(model), copy.deepcopy(model).double()
+    g = gen(32)
+    x, y = randn(g, 64, 20), torch.randint(0, 30, (64,), generator=g, device="cuda")
+    f = 2.0 ** -24
+    for ignored in (0, 21, 63):
+        y[:ignored] = -100
+        want = F.cross_entropy(exact(x.double()), y)
+        wants = torch.autograd.grad(want, list(exact.parameters()))
+        for net, fused in ((model, True), (other, False)):
+            opt = torch.optim.SGD(net.parameters(), lr=0.0)
+            loss = train_step(net, opt, OverlappedGradReducer(net.parameters()), x, y, fused_loss=fused)
+            # logits: 21 roundings of at most 20 terms of up to 1; log probabilities of 30 classes of spread below 16 and a mean of
+            # 64: 1000 roundings are far more than any term of the loss or of a gradient (at most 64 times 5) has seen
+            assert abs(loss.item() - want.item()) <= 1000 * f * (1 + want.item())
+            for p, w in zip(net.parameters(), wants):
+                assert (p.grad - w).abs().max().item() <= 1000 * f * 5
+        found = evaluate_top(model, [(x, y), (x[:7], y[:7])], top=3)
+        xs, ys = torch.cat([x, x[:7]]), torch.cat([y, y[:7]])
+        logits, ys = exact(xs.double())[ys != -100], ys[ys != -100]
+        p = torch.softmax(logits, 1)
+        best = logits.topk(3, 1)[1] == ys[:, None]
+        for name, value in (("top1", best[:, 0].double().mean()), ("top3", best.sum(1).double().mean()), ("nll", F.cross_entropy(logits, ys)),
+                            ("entropy", -(p * p.log()).sum(1).mean())):
+            assert abs(found[name] - value.item()) <= 1000 * f * (1 + value.item()), name
+    y[:] = -100
+    assert evaluate_top(model, [(x, y)], top=3) == dict(top1=0.0, top3=0.0, nll=0.0, entropy=0.0)
