@@ -254,7 +254,7 @@ __global__ void __launch_bounds__(GradLayout<T, DP, BENT, KEYS>::kThreads, GradL
                         if (docs) row_doc[k] = in ? p.doc_q[b * p.doc_q_sb + i] : -1;
                         if (BENT && p.slopes) {
                             row_slope[k] = in ? p.slopes[g * p.R + m - i * p.R] * kLog2e : 0.f;
-                            row_place[k] = (float)(i + p.shift);
+                            row_place[k] = (float)(i + p.shift - o0);
                         }
                     }
                 }
@@ -556,7 +556,8 @@ __global__ void __launch_bounds__(GradLayout<T, DP, BENT, KEYS>::kThreads, GradL
                         float2 away, less;  // distances, and what they take from the scores
                         if (KEYS) {
                             const int c = 32 * h + j;
-                            away = make_float2(fabsf(cols[256 + c] - (float)key), fabsf(cols[257 + c] - (float)key));
+                            // (from the block's first key on: places are not whole numbers of fp32 for ever)
+                            away = make_float2(fabsf(cols[256 + c] - (float)r), fabsf(cols[257 + c] - (float)r));
                             less = make_float2(-cols[192 + c], -cols[193 + c]);
                         } else {
                             const float first = (float)(row.place - t0) - (float)(32 * h + j);

@@ -4,7 +4,7 @@ import pytest
 import torch
 
 import operators_reference as R
-from test_gpu_operators import DTYPES, IDS, close, gen, ops, randn, rounding
+from test_gpu_operators import DTYPES, IDS, attention_bounds, close, gen, ops, randn, rounding
 
 pytestmark = pytest.mark.gpu
 
@@ -192,3 +192,25 @@ def test_losses_leave_out_ignored_labels():
             assert abs(found[name] - value.item()) <= 1000 * f * (1 + value.item()), name
     y[:] = -100
     assert evaluate_top(model, [(x, y)], top=3) == dict(top1=0.0, top3=0.0, nll=0.0, entropy=0.0)
+
+
+@pytest.mark.parametrize("dtype", DTYPES[1:], ids=IDS[1:])
+def test_biases_by_distance_beyond_24_bits_of_place(dtype):
+    """Places of 2^24 and more are no longer whole numbers of fp32; distances of near keys have to be."""
+    g, T, n = gen(34), 2 ** 24 + 333, 2048
+    k, v = (torch.zeros(1, T, 1, 8, dtype=dtype, device="cuda") for _ in range(2))
+    for x in (k, v):
+        x[:, -n:] = randn(g, 1, n, 1, 8, dtype=dtype)
+    q, go = randn(g, 1, 5, 1, 8, dtype=dtype), randn(g, 1, 5, 1, 8, dtype=dtype)
+    leaves = [x.requires_grad_(True) for x in (q, k, v)]
+    slopes = torch.tensor([0.7], device="cuda")  # (2048 places away nothing is left: exp(-1400))
+    out = ops().attention(*leaves, slopes=slopes)
+    got = [out.detach(), *torch.autograd.grad(out, leaves, go)]
+    case = [q, k.detach()[:, -n:], v.detach()[:, -n:]]
+    want, tol = attention_bounds(*case, go, dict(slopes=slopes), dtype)
+    tiny = 0.0 if dtype is not torch.float16 else 2.0 ** -24 * 40  # (as in test_attention: subnormal results and probabilities)
+    for name, x, w, t in zip(("out", "grad_q", "grad_k", "grad_v"), got, want, tol):
+        if x.shape[1] == T:
+            assert not x[:, :-n].any(), name
+            x = x[:, -n:]
+        close(x, w, t + tiny, name)
