@@ -41,8 +41,8 @@ __global__ void __launch_bounds__(256) attention_split_kernel(const AttnProblem 
         }
     }
     uint32_t w[3][16];
-    plane_words<float>(w, 0, x[0], x[1]);
-    plane_words<float>(w, 1, x[2], x[3]);
+    plane_words<float, true>(w, 0, x[0], x[1]);
+    plane_words<float, true>(w, 1, x[2], x[3]);
 #pragma unroll
     for (int e = 0; e < 3; ++e) *reinterpret_cast<uint2 *>(o.to + at * kPlaneWidth + 64 * e + d) = make_uint2(w[e][0], w[e][1]);
     if (k == 3) {

@@ -66,11 +66,17 @@ __device__ __forceinline__ float2 unpack_pair(uint32_t v) {
     return __half22float2(*reinterpret_cast<const __half2 *>(&v));
 }
 
-// two values as words of the planes of their type (one of 16-bit types), for half a word row each
-template <typename T, int N>
+// Two values as words of the planes of their type (one of 16-bit types), for half a word row each.  OPERAND: any finite fp32 values; those
+// that would round to an infinity of bf16 take its largest value, and the other planes what is left.
+template <typename T, bool OPERAND = false, int N>
 __device__ __forceinline__ void plane_words(uint32_t (&w)[N][16], int at, float a, float b) {
     using O = typename Operand<T, 64>::Type;
-    w[0][at] = pack_pair<O>(a, b);
+    if constexpr (OPERAND) {
+        const float most = __uint_as_float(0x7f7f0000u);
+        w[0][at] = pack_pair<O>(fminf(fmaxf(a, -most), most), fminf(fmaxf(b, -most), most));  // (a NaN is in the other planes)
+    } else {
+        w[0][at] = pack_pair<O>(a, b);
+    }
     if constexpr (N == 3) {
         float2 h = unpack_pair<O>(w[0][at]);
         a -= h.x;

@@ -214,3 +214,38 @@ def test_biases_by_distance_beyond_24_bits_of_place(dtype):
             assert not x[:, :-n].any(), name
             x = x[:, -n:]
         close(x, w, t + tiny, name)
+
+
+@pytest.mark.parametrize("dtype", DTYPES[:2], ids=IDS[:2])
+@pytest.mark.parametrize("D", [64, 72])
+def test_attention_beside_the_largest_values_of_a_type(D, dtype):
+    """Another document's values of +-finfo.max in the same tile are finite, and a probability of zero hides them."""
+    g = gen(35 + D)
+    ids = torch.zeros(1, 70, dtype=torch.int32, device="cuda")
+    ids[:, 31:50] = 1
+    other, kw = ids[0] == 1, dict(documents=ids, cap=20.0)
+    near = [randn(g, 1, 70, 2, D, dtype=dtype) for _ in range(4)]
+    for x in near[1:]:
+        x[:, other] = 0.0
+    want, tol = attention_bounds(*near, kw, dtype)
+    for filler in (torch.finfo(dtype).max, torch.finfo(dtype).min):
+        xs = [x.clone() for x in near]
+        for x in xs[1:]:
+            x[:, other] = filler
+        leaves = [x.requires_grad_(True) for x in xs[:3]]
+        out = ops().attention(*leaves, **kw)
+        got = [out.detach(), *torch.autograd.grad(out, leaves, xs[3])]
+        for name, x, w, t in zip(("out", "grad_q", "grad_k", "grad_v"), got, want, tol):
+            close(x[:, ~other], w[:, ~other], t[:, ~other], name)
+
+
+def test_attention_of_the_largest_fp32_values():
+    """Beyond the largest bf16 value, where a first plane of 16 bits would round to infinity."""
+    g = gen(36)
+    q, k = randn(g, 1, 5, 1, 64), randn(g, 1, 1, 1, 64)
+    v = torch.full((1, 1, 1, 64), torch.finfo(torch.float32).max, device="cuda")
+    v[..., ::2] *= -1 + 2.0 ** -9
+    # one key: its probability is one, whose products with three planes and sum are off by a rounding each, 2^-22 in all
+    out = ops().attention(q, k, v).double()
+    want = v.double().expand(1, 5, 1, 64)
+    assert ((out - want).abs() <= 2.0 ** -22 * want.abs()).all()
