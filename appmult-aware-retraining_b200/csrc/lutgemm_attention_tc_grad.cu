@@ -17,18 +17,49 @@ namespace {
 // ---- delta ------------------------------------------------------------------------------------------------------------
 constexpr int kDeltaRows = 64;  // rows of a block of the first kernel
 
-// delta of every packed row; for fp16 also the largest |grad_o| of every 64 rows.  8 lanes to a row, 16 bytes to a lane and step.
+// fp16: what the score gradients of a batch row and key head are at most.  P (gP - delta) is no more than |grad_o| |v| + |delta|, the lengths as
+// vectors, whichever query and key it belongs to.
+struct GradBounds {
+    float *length;     // of grad_o of every packed row
+    float *row_most;   // of every kDeltaRows rows: the largest length, the largest |delta|
+    float *key_most;   // of every kDeltaRows keys: the largest length of v
+    int row_parts, key_parts;
+};
+// the power of two that a bound is from 2^14 to 2^15 of, so that no score gradient comes near fp16's largest value and those down to
+// 2^-28 of the bound are normal; an infinite or NaN bound, or none at all: one
+__device__ __forceinline__ float unit_of(float bound) {
+    const int e = (int)(__float_as_uint(bound) >> 23);
+    return e > 14 && e < 255 ? __uint_as_float((uint32_t)(e - 14) << 23) : 1.f;
+}
+
+// delta of every packed row; for fp16 also the bounds, the keys' by further blocks.  8 lanes to a row, 16 bytes to a lane and step.
 template <typename T>
 __global__ void __launch_bounds__(256) attention_delta_kernel(const AttnProblem p, const AttnTensor go, const T *out, const T *rest,
-                                                              float *delta, float *most) {
-    __shared__ float top[8];
+                                                              float *delta, const GradBounds bounds) {
+    constexpr bool kBounds = !IsBf16<T>::value;
+    __shared__ float tops[2][8];
     const int b = blockIdx.z, g = blockIdx.y, lane = threadIdx.x & 7;
-    float big = 0.f;
+    const bool keys = kBounds && (int)blockIdx.x >= bounds.row_parts;
+    const int part = blockIdx.x - (keys ? bounds.row_parts : 0);
+    float longest = 0.f, most = 0.f;
 #pragma unroll
     for (int k = 0; k < kDeltaRows / 32; ++k) {
-        const int m = blockIdx.x * kDeltaRows + 32 * k + (threadIdx.x >> 3);
-        float s = 0.f;
-        if (m < p.M) {
+        const int m = part * kDeltaRows + 32 * k + (threadIdx.x >> 3);
+        float s = 0.f, sq = 0.f;
+        if (keys) {
+            if (m < p.Tk && (!p.doc_k || p.doc_k[b * p.doc_k_sb + m] >= 0)) {
+                const T *x = static_cast<const T *>(p.v.p) + b * p.v.sb + m * p.v.st + g * p.v.sh;
+                for (int d = lane * 8; d < p.D; d += 64) {
+                    const uint4 a = *reinterpret_cast<const uint4 *>(x + d);
+                    const uint32_t av[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float2 u = unpack_pair<T>(av[e]);
+                        sq += u.x * u.x + u.y * u.y;
+                    }
+                }
+            }
+        } else if (m < p.M) {
             const int i = m / p.R, h = g * p.R + m - i * p.R;
             if (!p.doc_q || p.doc_q[b * p.doc_q_sb + i] >= 0) {
                 const T *x = static_cast<const T *>(go.p) + b * go.sb + i * go.st + h * go.sh;
@@ -41,24 +72,47 @@ __global__ void __launch_bounds__(256) attention_delta_kernel(const AttnProblem 
                     for (int e = 0; e < 4; ++e) {
                         const float2 u = unpack_pair<T>(av[e]), v = unpack_pair<T>(ov[e]), w = unpack_pair<T>(rv[e]);
                         s += u.x * (v.x + w.x) + u.y * (v.y + w.y);
-                        big = fmaxf(big, fmaxf(fabsf(u.x), fabsf(u.y)));
+                        if (kBounds) sq += u.x * u.x + u.y * u.y;
                     }
                 }
             }
         }
 #pragma unroll
-        for (int d = 4; d; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
-        if (m < p.M && lane == 0) delta[((long)b * p.G + g) * p.M + m] = s;
+        for (int d = 4; d; d >>= 1) {
+            s += __shfl_xor_sync(0xffffffffu, s, d);
+            if (kBounds) sq += __shfl_xor_sync(0xffffffffu, sq, d);
+        }
+        if (!keys && m < p.M && lane == 0) {
+            delta[((long)b * p.G + g) * p.M + m] = s;
+            if (kBounds) bounds.length[((long)b * p.G + g) * p.M + m] = sqrtf(sq);
+        }
+        longest = fmaxf(longest, sq);
+        most = fmaxf(most, fabsf(s));
     }
-    if (!most) return;
+    if (!kBounds) return;
 #pragma unroll
-    for (int d = 16; d; d >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, d));
-    if ((threadIdx.x & 31) == 0) top[threadIdx.x >> 5] = big;
+    for (int d = 16; d; d >>= 1) {
+        longest = fmaxf(longest, __shfl_xor_sync(0xffffffffu, longest, d));
+        most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, d));
+    }
+    if ((threadIdx.x & 31) == 0) {
+        tops[0][threadIdx.x >> 5] = longest;
+        tops[1][threadIdx.x >> 5] = most;
+    }
     __syncthreads();
     if (threadIdx.x == 0) {
 #pragma unroll
-        for (int w = 1; w < 8; ++w) big = fmaxf(big, top[w]);
-        most[((long)b * p.G + g) * gridDim.x + blockIdx.x] = big;
+        for (int w = 1; w < 8; ++w) {
+            longest = fmaxf(longest, tops[0][w]);
+            most = fmaxf(most, tops[1][w]);
+        }
+        const long at = (long)b * p.G + g;
+        if (keys) {
+            bounds.key_most[at * bounds.key_parts + part] = sqrtf(longest);
+        } else {
+            bounds.row_most[2 * (at * bounds.row_parts + part)] = sqrtf(longest);
+            bounds.row_most[2 * (at * bounds.row_parts + part) + 1] = most;
+        }
     }
 }
 
@@ -80,8 +134,9 @@ __global__ void __launch_bounds__(256) attention_delta_kernel(const AttnProblem 
 //                                   950 us for both kernels (as above 1100), without one 600 us (as above 530)
 // Results go through shared memory, which the ring has left, so that whole rows are written (a row to a thread took 6000 clocks of
 // a block of 16000 where there are 197 keys).
-// fp16: P is kept 2^10 larger, and grad_o is taken in units of its largest value in this key head (a power of two), so that dS stays
-// out of fp16's subnormal range whatever the scale of the loss.
+// fp16: P is kept 2^10 larger, out of its subnormal range down to 2^-24.  dS is in units (powers of two) of what it is at most: with rows kept, for
+// every row by itself; with keys kept, for all rows that the block goes over, whose sums it shares.  So dS keeps its bits whatever the
+// scale of the loss and of the values down to 2^-28 of the most: P of 2^-12 in a row whose gradients are 2^-12 of the largest, say.
 // fp32: P and dS are split into planes as the operands were; there is one group, and each round's sums start from zero and are added up
 // in registers (in the accumulators, what additions cut off came to 2e-5 of the gradients of 4096 rows).
 // The workers' instructions per score bound both kernels.  2 x 4096, 16 / 4 heads of 128, bf16: 546 us with keys kept (256 blocks, not two
@@ -110,7 +165,7 @@ template <typename T, int DP, bool BENT, bool KEYS>
 __global__ void __launch_bounds__(GradLayout<T, DP, BENT, KEYS>::kThreads, GradLayout<T, DP, BENT, KEYS>::kPerSm)
     attention_tc_grad_kernel(const AttnProblem p, const AttnTensor go, const __grid_constant__ CUtensorMap map_x,
                              const __grid_constant__ CUtensorMap map_y, const DocRange *key_ranges, const DocRange *row_ranges,
-                             const float *lse, const float *delta, const float *most, int most_parts, T *g1, T *g2, int *error_word) {
+                             const float *lse, const float *delta, const GradBounds bounds, T *g1, T *g2, int *error_word) {
     using L = GradLayout<T, DP, BENT, KEYS>;
     constexpr int G = L::kGroups;
     using Op = typename L::Op;
@@ -126,7 +181,7 @@ __global__ void __launch_bounds__(GradLayout<T, DP, BENT, KEYS>::kThreads, GradL
     volatile int *tiles = reinterpret_cast<int *>(smem + L::kBars + 176);    // of the last eight rounds begun; then how many there were
     volatile int *brought = reinterpret_cast<int *>(smem + L::kBars + 212);  // of the stages
     volatile int *rounds_seen = reinterpret_cast<int *>(smem + L::kBars + 236);  // how many there are, once that is known
-    float *tops = reinterpret_cast<float *>(smem + L::kBars + 240);          // of the workers' warps
+    float *tops = reinterpret_cast<float *>(smem + L::kBars + 240);          // of the workers' warps, twice 16
     const int tid = threadIdx.x, warp = warp_index();
     int bid = blockIdx.x;
     const int g = bid % p.G;
@@ -161,16 +216,32 @@ __global__ void __launch_bounds__(GradLayout<T, DP, BENT, KEYS>::kThreads, GradL
     }
     __syncthreads();
     // (the warp that brings tiles begins at once; the others meet again when X and Y have come)
-    float unit = 1.f;  // fp16: the unit of grad_o, a power of two above its largest value
+    float unit = 1.f;  // fp16: of dS, of this thread's row (with KEYS of the block)
     uint32_t tmem = 0;
     if (warp != L::kWorkers / 32 + 1) {
         if (warp == L::kWorkers / 32) tmem_alloc(smem_u32(slot), L::kColumns);
         if (!kBf16 && warp < L::kWorkers / 32) {
-            float top = 0.f;
-            for (int i = tid; i < most_parts; i += L::kWorkers) top = fmaxf(top, most[((long)b * p.G + g) * most_parts + i]);
+            // with KEYS the largest length of grad_o and |delta| of the rows that may see the block, else the largest length of v
+            float top = 0.f, top_delta = 0.f;
+            const long at = (long)b * p.G + g;
+            if (KEYS) {
+                const int first = p.causal && o0 >= pre ? (int)min((long)max(0, o0 - p.shift) * p.R, (long)p.M) / kDeltaRows : 0;
+                for (int i = first + tid; i < bounds.row_parts; i += L::kWorkers) {
+                    top = fmaxf(top, bounds.row_most[2 * (at * bounds.row_parts + i)]);
+                    top_delta = fmaxf(top_delta, bounds.row_most[2 * (at * bounds.row_parts + i) + 1]);
+                }
+            } else {
+                for (int i = tid; i < bounds.key_parts; i += L::kWorkers) top = fmaxf(top, bounds.key_most[at * bounds.key_parts + i]);
+            }
 #pragma unroll
-            for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-            if ((tid & 31) == 0) tops[warp] = top;
+            for (int d = 16; d; d >>= 1) {
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+                top_delta = fmaxf(top_delta, __shfl_xor_sync(0xffffffffu, top_delta, d));
+            }
+            if ((tid & 31) == 0) {
+                tops[warp] = top;
+                tops[16 + warp] = top_delta;
+            }
         }
         if (warp < 8) {  // X by four warps, Y by four
             const bool y = warp >= 4;
@@ -195,12 +266,20 @@ __global__ void __launch_bounds__(GradLayout<T, DP, BENT, KEYS>::kThreads, GradL
         tmem_after_sync();
         tmem = *slot;
         if (!kBf16) {
-            float top = 0.f;
+            float top = 0.f, top_delta = 0.f;
 #pragma unroll
-            for (int w = 0; w < L::kWorkers / 32; ++w) top = fmaxf(top, tops[w]);
-            // (an infinite or NaN gradient, or none at all: as it is)
-            const int e = (int)(__float_as_uint(top) >> 23);
-            if (e > 0 && e < 254) unit = __uint_as_float((uint32_t)(e + 1) << 23);
+            for (int w = 0; w < L::kWorkers / 32; ++w) {
+                top = fmaxf(top, tops[w]);
+                top_delta = fmaxf(top_delta, tops[16 + w]);
+            }
+            if (KEYS) {
+                const float *own = bounds.key_most + ((long)b * p.G + g) * bounds.key_parts;
+                const int part = o0 / kDeltaRows;
+                unit = unit_of(top * fmaxf(own[part], own[min(part + 1, bounds.key_parts - 1)]) + top_delta);
+            } else {
+                const int m = o0 + (tid & 127);
+                if (m < p.M) unit = unit_of(bounds.length[stat0 + m] * top + fabsf(delta[stat0 + m]));
+            }
         }
     }
 
@@ -665,20 +744,20 @@ __global__ void __launch_bounds__(GradLayout<T, DP, BENT, KEYS>::kThreads, GradL
 
 template <typename T, int DP, bool BENT, bool KEYS>
 int launch(const AttnProblem &p, const AttnTensor &go, const CUtensorMap &map_x, const CUtensorMap &map_y, const DocRange *kr, const DocRange *rr,
-           const float *lse, const float *delta, const float *most, int most_parts, void *g1, void *g2, int *error_word, cudaStream_t stream) {
+           const float *lse, const float *delta, const GradBounds &bounds, void *g1, void *g2, int *error_word, cudaStream_t stream) {
     using L = GradLayout<T, DP, BENT, KEYS>;
     if (!cuda_ok(cudaFuncSetAttribute(attention_tc_grad_kernel<T, DP, BENT, KEYS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)L::kBytes)))
         return LUTGEMM_E_CUDA;
     const long blocks = (long)(((KEYS ? p.Tk : p.M) + 127) / 128) * p.B * p.G;
     if (blocks > 0x7fffffffL) return LUTGEMM_E_TOOLARGE;
     attention_tc_grad_kernel<T, DP, BENT, KEYS><<<(unsigned)blocks, L::kThreads, L::kBytes, stream>>>(
-        p, go, map_x, map_y, kr, rr, lse, delta, most, most_parts, static_cast<T *>(g1), static_cast<T *>(g2), error_word);
+        p, go, map_x, map_y, kr, rr, lse, delta, bounds, static_cast<T *>(g1), static_cast<T *>(g2), error_word);
     return launch_status();
 }
 
-// the two kernels; delta and, for fp16, the largest gradients stand in scratch
+// the two kernels; delta and, for fp16, the bounds stand in scratch
 template <typename T, int DP>
-int gradients(const AttnProblem &p, const AttnTensor &go, const float *lse, const float *delta, const float *most, int parts, const DocRange *kr,
+int gradients(const AttnProblem &p, const AttnTensor &go, const float *lse, const float *delta, const GradBounds &bounds, const DocRange *kr,
               const DocRange *rr, void *gq, void *gk, void *gv, int *error_word, cudaStream_t stream) {
     using Op = Operand<T, DP>;
     const int width = Op::kPlanes ? kPlaneWidth : p.D;
@@ -687,32 +766,36 @@ int gradients(const AttnProblem &p, const AttnTensor &go, const float *lse, cons
         !attention_map(&map_k, Op::kBf16, p.k, p.B, p.Tk, p.G, 1, width) || !attention_map(&map_v, Op::kBf16, p.v, p.B, p.Tk, p.G, 1, width))
         return LUTGEMM_E_CUDA;  // (no tensor maps on this driver)
     const bool bent = p.cap > 0.f || p.slopes;
-    const int rc = bent ? launch<T, DP, true, true>(p, go, map_q, map_go, kr, rr, lse, delta, most, parts, gk, gv, error_word, stream)
-                        : launch<T, DP, false, true>(p, go, map_q, map_go, kr, rr, lse, delta, most, parts, gk, gv, error_word, stream);
+    const int rc = bent ? launch<T, DP, true, true>(p, go, map_q, map_go, kr, rr, lse, delta, bounds, gk, gv, error_word, stream)
+                        : launch<T, DP, false, true>(p, go, map_q, map_go, kr, rr, lse, delta, bounds, gk, gv, error_word, stream);
     if (rc != LUTGEMM_OK) return rc;
-    return bent ? launch<T, DP, true, false>(p, go, map_k, map_v, kr, rr, lse, delta, most, parts, gq, nullptr, error_word, stream)
-                : launch<T, DP, false, false>(p, go, map_k, map_v, kr, rr, lse, delta, most, parts, gq, nullptr, error_word, stream);
+    return bent ? launch<T, DP, true, false>(p, go, map_k, map_v, kr, rr, lse, delta, bounds, gq, nullptr, error_word, stream)
+                : launch<T, DP, false, false>(p, go, map_k, map_v, kr, rr, lse, delta, bounds, gq, nullptr, error_word, stream);
 }
 
 template <typename T>
-int backward(const AttnProblem &p, const AttnTensor &go, const void *out, const void *rest, const float *lse, float *delta, float *most,
-             const DocRange *kr, const DocRange *rr, void *gq, void *gk, void *gv, int *error_word, cudaStream_t stream) {
-    const int parts = (p.M + kDeltaRows - 1) / kDeltaRows;
-    attention_delta_kernel<T><<<dim3(parts, p.G, p.B), 256, 0, stream>>>(p, go, static_cast<const T *>(out), static_cast<const T *>(rest), delta,
-                                                                        IsBf16<T>::value ? nullptr : most);
+int backward(const AttnProblem &p, const AttnTensor &go, const void *out, const void *rest, const float *lse, float *delta, const DocRange *kr,
+             const DocRange *rr, void *gq, void *gk, void *gv, int *error_word, cudaStream_t stream) {
+    const int row_parts = (p.M + kDeltaRows - 1) / kDeltaRows, key_parts = (p.Tk + kDeltaRows - 1) / kDeltaRows;
+    const long heads = (long)p.B * p.G;
+    GradBounds bounds{};
+    if (!IsBf16<T>::value)
+        bounds = {delta + heads * p.M, delta + 2 * heads * p.M, delta + 2 * heads * (p.M + row_parts), row_parts, key_parts};
+    attention_delta_kernel<T><<<dim3(row_parts + bounds.key_parts, p.G, p.B), 256, 0, stream>>>(p, go, static_cast<const T *>(out),
+                                                                                               static_cast<const T *>(rest), delta, bounds);
     const int rc = launch_status();
     if (rc != LUTGEMM_OK) return rc;
-    return p.D <= 64 ? gradients<T, 64>(p, go, lse, delta, most, parts, kr, rr, gq, gk, gv, error_word, stream)
-                     : gradients<T, 128>(p, go, lse, delta, most, parts, kr, rr, gq, gk, gv, error_word, stream);
+    return p.D <= 64 ? gradients<T, 64>(p, go, lse, delta, bounds, kr, rr, gq, gk, gv, error_word, stream)
+                     : gradients<T, 128>(p, go, lse, delta, bounds, kr, rr, gq, gk, gv, error_word, stream);
 }
 
 }  // namespace
 
-// fp32: the planes of q, grad_o, k and v; ranges of documents, delta, fp16's largest gradients
+// fp32: the planes of q, grad_o, k and v; ranges of documents, delta, fp16's bounds
 size_t attention_tc_backward_scratch_bytes(const AttnProblem &p, int dtype) {
-    const size_t parts = (p.M + kDeltaRows - 1) / kDeltaRows;
+    const size_t row_parts = (p.M + kDeltaRows - 1) / kDeltaRows, key_parts = (p.Tk + kDeltaRows - 1) / kDeltaRows;
     return (dtype == LUTGEMM_F32 ? 2 * plane_bytes(p.B, p.Tq, p.H) + 2 * plane_bytes(p.B, p.Tk, p.G) : 0) + doc_range_bytes(p) +
-           sizeof(float) * p.B * p.G * (p.M + parts);
+           sizeof(float) * p.B * p.G * (p.M + (dtype == LUTGEMM_F16 ? p.M + 2 * row_parts + key_parts : 0));
 }
 
 int attention_tc_backward(const AttnProblem &problem, int dtype, const AttnTensor &grad, const void *out, const void *rest, const float *lse,
@@ -726,9 +809,9 @@ int attention_tc_backward(const AttnProblem &problem, int dtype, const AttnTenso
     const DocRange *kr, *rr;
     int rc = doc_ranges(p, at, &kr, &rr, stream);
     if (rc != LUTGEMM_OK) return rc;
-    float *delta = reinterpret_cast<float *>(at + doc_range_bytes(p)), *most = delta + (size_t)p.B * p.G * p.M;
-    if (dtype == LUTGEMM_BF16) return backward<__nv_bfloat16>(p, grad, out, rest, lse, delta, most, kr, rr, gq, gk, gv, error_word, stream);
-    if (dtype == LUTGEMM_F16) return backward<__half>(p, grad, out, rest, lse, delta, most, kr, rr, gq, gk, gv, error_word, stream);
+    float *delta = reinterpret_cast<float *>(at + doc_range_bytes(p));
+    if (dtype == LUTGEMM_BF16) return backward<__nv_bfloat16>(p, grad, out, rest, lse, delta, kr, rr, gq, gk, gv, error_word, stream);
+    if (dtype == LUTGEMM_F16) return backward<__half>(p, grad, out, rest, lse, delta, kr, rr, gq, gk, gv, error_word, stream);
     __nv_bfloat16 *planes = static_cast<__nv_bfloat16 *>(scratch);
     const SplitOperand ops[4] = {{p.q, planes, p.doc_q, p.doc_q_sb, p.Tq, p.H},
                                  {p.k, planes + nq / 2, p.doc_k, p.doc_k_sb, p.Tk, p.G},
@@ -739,7 +822,7 @@ int attention_tc_backward(const AttnProblem &problem, int dtype, const AttnTenso
     p.q = plane_tensor(ops[0].to, p.Tq, p.H);
     p.k = plane_tensor(ops[1].to, p.Tk, p.G);
     p.v = plane_tensor(ops[2].to, p.Tk, p.G);
-    return gradients<float, 64>(p, plane_tensor(ops[3].to, p.Tq, p.H), lse, delta, most, 0, kr, rr, gq, gk, gv, error_word, stream);
+    return gradients<float, 64>(p, plane_tensor(ops[3].to, p.Tq, p.H), lse, delta, GradBounds{}, kr, rr, gq, gk, gv, error_word, stream);
 }
 
 }  // namespace lutgemm

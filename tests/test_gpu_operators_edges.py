@@ -249,3 +249,67 @@ def test_attention_of_the_largest_fp32_values():
     out = ops().attention(q, k, v).double()
     want = v.double().expand(1, 5, 1, 64)
     assert ((out - want).abs() <= 2.0 ** -22 * want.abs()).all()
+
+
+def score_gradients(q, k, v, go, **kw):
+    """p, p (gp - delta) and gp in 64 bits, [B, H, Tq, Tk]; heads of their own, no cap, no bias."""
+    qd, kd, vd, god = (x.detach().double() for x in (q, k, v, go))
+    seen = R.visible(q.shape[0], q.shape[1], k.shape[1], kw.get("causal", False), None, kw.get("documents"), None, q.device)[:, None]
+    s = torch.einsum("bihd,bjhd->bhij", qd, kd) * q.shape[3] ** -0.5
+    p = torch.softmax(s.masked_fill(~seen, -torch.inf), -1)
+    gp = torch.einsum("bihd,bjhd->bhij", god, vd)
+    return p, p * (gp - (p * gp).sum(-1, keepdim=True)), gp
+
+
+# gradients of very different sizes, or values that are large: one row's beside the others', one document's, all of them tiny
+@pytest.mark.parametrize("form", ["one row", "causal", "tiny", "large values", "document"])
+@pytest.mark.parametrize("D", [64, 128])
+def test_fp16_score_gradients_of_uneven_rows(form, D):
+    """dS = p (gp - delta) is rounded to fp16, in units that keep it normal: by row for grad_q, by block of keys for grad_k."""
+    g, T, H = gen(33 + D), 4096 if form != "large values" else 50, 1
+    q, k, v = (randn(g, 1, T, H, D, dtype=torch.float16).requires_grad_(True) for _ in range(3))
+    go = randn(g, 1, T, H, D)
+    kw = {}
+    big = slice(T // 2, T // 2 + 1)
+    if form in ("one row", "causal"):
+        go[:, big] *= 2.0 ** 13
+        kw = dict(causal=form == "causal")
+    elif form == "document":  # (the last tile of the first document holds rows of the second)
+        ids = torch.zeros(1, T, dtype=torch.int32, device="cuda")
+        ids[:, 1000:] = 1
+        go[:, 1000:] *= 2.0 ** 12
+        kw = dict(documents=ids)
+        big = slice(1000, T)
+    elif form == "tiny":
+        go[:, :T // 2] *= 2.0 ** -9
+        big = slice(T // 2, T)
+    else:
+        sign = 1.0 - 2.0 * (torch.arange(T, device="cuda") % 2)
+        with torch.no_grad():
+            q.mul_(2.0)  # (rows have a few probable keys)
+            v[..., :16] = 60000.0 * sign[:, None, None]  # gp is beyond fp16, in units of the largest gradient too
+        go[..., :16] = 2.0
+        go *= 2.0 ** -11
+    go = go.half()
+    got = torch.autograd.grad(ops().attention(q, k, v, **kw), (q, k, v), go)
+    qd, kd, vd = (x.detach().double().requires_grad_(True) for x in (q, k, v))
+    wants = torch.autograd.grad(R.attention(qd, kd, vd, **kw), (qd, kd, vd), go.double())
+    p, gs, gp = score_gradients(q, k, v, go, **kw)
+    u, f, scale = 2.0 ** -11, 2.0 ** -24, D ** -0.5
+    # a term: its rounding u, the relative error of p (scores of up to 2^6 by exp2 and sums of T terms), gp and delta by D products of
+    # fp32; delta besides by the errors of out, whose probabilities were rounded, and sums of T products, each of 2 f or less
+    most = torch.einsum("bihd,bjhd->bhij", go.double().abs(), vd.detach().abs())
+    off = (u + (2 * D + T + 64) * 2 * f)
+    e = gs.abs() * off + p * ((D + 8) * f * most + (p * most).sum(-1, keepdim=True) * off)
+    # what lies below fp16's normal range is off by 2^-25 units; a row's unit is at most 2^-14 of a bound of its terms, sqrt of the two
+    # sums of squares and delta, and a block of keys' the largest of its rows'
+    length = go.double().square().sum(-1).sqrt().transpose(1, 2)  # [B, H, T]
+    longest = vd.detach().square().sum(-1).sqrt().amax(1)[..., None]
+    bound = (length * longest + (p * gp).sum(-1).abs()) * 2.0 ** -39
+
+    def check(name, got, want, terms, least, with_, spec, rows):
+        tol = torch.einsum(spec, terms + least, with_.detach().abs()) * scale + u * want.abs() + 2.0 ** -25
+        close(got[:, rows], want[:, rows], tol[:, rows], name)
+    everything = slice(0, T)
+    check("grad_q", got[0], wants[0], e, bound[..., None] * p.gt(0), kd, "bhij,bjhd->bihd", everything)
+    check("grad_k", got[1], wants[1], e, bound.amax(-1)[..., None, None] * p.gt(0), qd, "bhij,bihd->bjhd", everything)
