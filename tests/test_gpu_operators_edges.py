@@ -313,3 +313,55 @@ def test_fp16_score_gradients_of_uneven_rows(form, D):
     everything = slice(0, T)
     check("grad_q", got[0], wants[0], e, bound[..., None] * p.gt(0), kd, "bhij,bjhd->bihd", everything)
     check("grad_k", got[1], wants[1], e, bound.amax(-1)[..., None, None] * p.gt(0), qd, "bhij,bihd->bjhd", everything)
+
+
+# (B, Tq, Tk, H): keys in one part, keys split over blocks and joined
+@pytest.mark.parametrize("dtype", DTYPES[1:], ids=IDS[1:])
+@pytest.mark.parametrize("B,Tq,Tk,H", [(2, 100, 100, 4), (32, 1, 1024, 4)])
+def test_gradients_use_the_unrounded_result(B, Tq, Tk, H, dtype):
+    """Two equal keys share a query's probability, and their values are neighbours in the operands' type: the result lies between them.
+    A score's gradient p (gp - delta) is then the difference of near values, and delta from the rounded result would be off by as much."""
+    D, g = 64, gen(37 + Tk)
+    k, v = (randn(g, B, Tk // 2, H, D) for _ in range(2))
+    k = (8 * k / k.norm(dim=-1, keepdim=True)).to(dtype).repeat_interleave(2, dim=1)
+    v = torch.where(v.abs() < 2.0 ** -6, 1.0, v).to(dtype).repeat_interleave(2, dim=1)
+    v[:, 1::2] = (v[:, 1::2].contiguous().view(torch.int16) + 1).view(dtype)
+    at = 2 * torch.randint(0, Tk // 2, (B, Tq, H), generator=g, device="cuda")
+    q = (3 * k.gather(1, at[..., None].expand(B, Tq, H, D))).requires_grad_(True)
+    go = randn(g, B, Tq, H, D, dtype=dtype)
+    got = torch.autograd.grad(ops().attention(q, k, v), q, go)[0]
+    qd, kd, vd, god = (x.detach().double() for x in (q, k, v, go))
+    qd.requires_grad_(True)
+    want = R.attention(qd, kd, vd)
+    grad = torch.autograd.grad(want, qd, god)[0]
+    want, u, f, scale = want.detach(), rounding(dtype), 2.0 ** -24, D ** -0.5
+    s = torch.einsum("bihd,bjhd->bhij", qd.detach(), kd) * scale
+    p = torch.softmax(s, -1)
+    peak = p > 0.25
+    rest = p.masked_fill(peak, 0.0)
+    # both keys are more than 8 above everything else in log 2, so their P are relative to themselves: one up to f |s| log2 e, which is
+    # rounded away; the sum of unrounded P keeps it
+    assert (peak.sum(-1) == 2).all() and (rest.amax(-1) < p.amax(-1) * 2.0 ** -8).all()
+    most = torch.einsum("bihd,bjhd->bhij", qd.detach().abs(), kd.abs()) * scale
+    off = (D + 8) * f * most + 16 * f * s.abs() + 60 * f
+    # out: errors of the other probabilities, relative to themselves, by any two values; of the sum; of a part's sums of products (256
+    # keys at most, cut off or rounded) and the joining of parts; the rest of the rounding is itself rounded, by u^2
+    both = rest * (off + off.amax(-1, keepdim=True) + u)
+    assert vd.abs().max() <= 8
+    e_out = 16 * both.sum(-1)[..., None].transpose(1, 2) + want.abs() * u * u + want.abs() * f * (
+        2 * (min(Tk, 256) + 64) + 16 + 2 * s.abs().amax(-1)[..., None].transpose(1, 2)) + (2.0 ** -25 if dtype is torch.float16 else 0.0)
+    gp = torch.einsum("bihd,bjhd->bhij", god, vd)
+    gp_most = torch.einsum("bihd,bjhd->bhij", god.abs(), vd.abs())
+    delta = (p * gp).sum(-1, keepdim=True)
+    e_delta = torch.einsum("bihd,bihd->bhi", god.abs(), e_out + D * f * want.abs())[..., None]
+    gs = p * (gp - delta)
+    e_gs = gs.abs() * (off + off.amax(-1, keepdim=True) + u + 8 * f + 2 * (Tk + 64) * f) + p * ((D + 8) * f * gp_most + e_delta)
+    if dtype is torch.float16:  # dS below fp16's normal range: 2^-25 of a unit, which is at most 2^-14 of |grad_o| |v| + |delta|
+        bound = god.norm(dim=-1).transpose(1, 2) * vd.norm(dim=-1).amax(1)[..., None] + delta[..., 0].abs()
+        e_gs = e_gs + 2.0 ** -39 * bound[..., None]
+    tol = torch.einsum("bhij,bjhd->bihd", e_gs, kd.abs()) * scale + u * grad.abs() + (2.0 ** -25 if dtype is torch.float16 else 0.0)
+    # delta from the rounded result would not pass
+    rounded = torch.einsum("bihd,bihd->bhi", god, want.to(dtype).double())[..., None]
+    planted = grad - torch.einsum("bhij,bjhd->bihd", p * (rounded - delta), kd) * scale
+    assert ((planted - grad).abs() > 2 * tol).any()
+    close(got, grad, tol, "grad_q")
