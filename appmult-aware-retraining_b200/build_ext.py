@@ -1,12 +1,15 @@
 """In-tree build of liblutgemm_b200.so (sm_100a only) and of lutgemm_torch.so, the PyTorch operators over it.
 
-    python appmult-aware-retraining_b200/build_ext.py [--force] [--verbose]
+    python appmult-aware-retraining_b200/build_ext.py [--force] [--verbose] [--library-only]
 
 Each .cu under csrc/ is compiled with nvcc for compute_100a/sm_100a and linked into one shared
-library next to this file; lutgemm_torch.cpp is compiled against the installed PyTorch and linked to that library.  nvcc cross-compiles without a GPU, so this also runs on a CPU-only box.
+library next to this file; lutgemm_torch.cpp is compiled against the installed PyTorch and linked to that library, and again when
+another PyTorch or Python is installed.  C callers need the library alone: --library-only, and where PyTorch is not installed, leaves
+the module out.  nvcc cross-compiles without a GPU, so this also runs on a CPU-only box.
 """
 from __future__ import annotations
 
+import importlib.metadata
 import os
 import subprocess
 import sys
@@ -20,6 +23,7 @@ OBJ_DIR = os.path.join(HERE, "build")
 LIB = os.path.join(HERE, "liblutgemm_b200.so")
 TORCH_SRC = os.path.join(CSRC, "lutgemm_torch.cpp")
 TORCH_LIB = os.path.join(HERE, "lutgemm_torch.so")
+TORCH_STAMP = os.path.join(OBJ_DIR, "torch_module.version")  # what the module was compiled against
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
@@ -53,6 +57,22 @@ def _compile(src: str, verbose: bool) -> str:
     return obj
 
 
+def _torch_version():
+    """The PyTorch and Python that the extension module has to fit; None without PyTorch."""
+    try:
+        return f"torch {importlib.metadata.version('torch')} {sys.implementation.cache_tag}"
+    except importlib.metadata.PackageNotFoundError:
+        return None
+
+
+def _built_for() -> str:
+    try:
+        with open(TORCH_STAMP) as f:
+            return f.read()
+    except OSError:
+        return ""
+
+
 def _compile_torch(lib_ready) -> None:
     """The extension module: compiled while the library's sources are, linked when it is there (`lib_ready`: waits for that)."""
     import sysconfig
@@ -77,24 +97,39 @@ def _compile_torch(lib_ready) -> None:
     os.replace(TORCH_LIB + ".tmp", TORCH_LIB)
 
 
-def build(force: bool = False, verbose: bool = False) -> str:
+def build(force: bool = False, verbose: bool = False, module: bool = True) -> str:
+    """Builds what is older than its sources (`force`: all) and returns the library's path; `module`: lutgemm_torch.so too, if PyTorch is
+    installed."""
     os.makedirs(OBJ_DIR, exist_ok=True)
     newest = _deps_mtime()
-    if not force and all(os.path.exists(x) and os.path.getmtime(x) >= newest for x in (LIB, TORCH_LIB)):
-        return LIB
+
+    def fresh(path):
+        return not force and os.path.exists(path) and os.path.getmtime(path) >= newest
+
+    version = _torch_version() if module else None
+    make_library, make_module = not fresh(LIB), version is not None and not (fresh(TORCH_LIB) and _built_for() == version)
     srcs = _sources()
     linked = threading.Event()
     with ThreadPoolExecutor(max_workers=min(8, len(srcs)) + 1) as ex:
-        module = ex.submit(_compile_torch, linked.wait)
+        compiled = ex.submit(_compile_torch, linked.wait) if make_module else None
         try:
-            objs = list(ex.map(lambda s: _compile(s, verbose), srcs))
-            subprocess.run(["nvcc", "-shared", "-o", LIB + ".tmp", *objs, "-lcudart"], check=True)
-            os.replace(LIB + ".tmp", LIB)
+            if make_library:
+                objs = list(ex.map(lambda s: _compile(s, verbose), srcs))
+                subprocess.run(["nvcc", "-shared", "-o", LIB + ".tmp", *objs, "-lcudart"], check=True)
+                os.replace(LIB + ".tmp", LIB)
         finally:
             linked.set()
-        module.result()
+        if compiled is not None:
+            try:
+                compiled.result()
+            except Exception as e:
+                raise RuntimeError(f"{LIB} is built, but not its PyTorch module; --library-only leaves that out") from e
+            with open(TORCH_STAMP, "w") as f:
+                f.write(version)
     return LIB
 
 
 if __name__ == "__main__":
-    print(build(force="--force" in sys.argv, verbose="--verbose" in sys.argv))
+    print(build(force="--force" in sys.argv, verbose="--verbose" in sys.argv, module="--library-only" not in sys.argv))
+    if "--library-only" not in sys.argv and _torch_version() is None:
+        print("PyTorch is not installed: lutgemm_torch.so was left out")
