@@ -21,8 +21,8 @@ constexpr int kThreads = 160;  // four warps with a row to a thread, one that br
 // fp32: P is split into planes as the operands were, and each tile's products with V start from zero and are added up in registers: the
 // tensor cores cut off what an addition loses, which over a long row would add up.
 //
-// Heads of 64 values are bound by exponentials (4 x 4096 x 6 x 64 bf16: 185 us, 556 TFLOP/s, 60 % of the exponential unit), 128 by the
-// turns of products and probabilities (tensor pipe and exponential unit 50 % each): 2 x 4096, 16 / 4 heads, bf16 288 us (955 TFLOP/s);
+// The turns of products and probabilities bound it; no unit is full.  Heads of 64 values: exponential unit 60 %, tensor pipe 30 %, 4 x 4096 x 6
+// x 64 bf16 185 us (556 TFLOP/s).  Heads of 128: 50 % each, 2 x 4096, 16 / 4 heads, bf16 288 us (955 TFLOP/s);
 // 1 x 8192, 16 heads, fp16, causal 264 us (1040; 8 TB/s of tiles from L2, a third of its rate), 306 in a loop under the power cap.
 // fp32, 64 x 197 x 6 x 64: 73 us.  One query, 16 x 16385 keys, 16 / 4 heads of 64 bf16: 60 us with its join (4.5 TB/s).
 template <typename T, int DP>

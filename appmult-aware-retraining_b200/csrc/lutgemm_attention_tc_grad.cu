@@ -4,9 +4,9 @@
 //     dS = P (gP - delta) cap',   grad_v = P^T grad_o,   grad_k = scale dS^T q,   grad_q = scale dS k
 // Two kernels of one form give grad_q and grad_k with grad_v: each block keeps 128 rows of one side and goes over the other in tiles of 64,
 // so that every sum has one owner and one order and no result depends on timing.  That costs seven products per pair of tiles
-// where sums by atomics would need five, which here is the smaller part of the time: the exponentials and conversions bound both.
-// delta uses out before its rounding (out + out_rest): where few keys have all of the probability, the rounding of out would be
-// the largest error of grad_q and grad_k.
+// where sums by atomics would need five.
+// delta uses out before its rounding (out + out_rest): where a few keys with near values share the probability, gP - delta is no larger than
+// that rounding's product with grad_o.
 #include "lutgemm_attention_tc.cuh"
 #include "lutgemm_kernels.h"
 
@@ -139,8 +139,9 @@ __global__ void __launch_bounds__(256) attention_delta_kernel(const AttnProblem 
 // scale of the loss and of the values down to 2^-28 of the most: P of 2^-12 in a row whose gradients are 2^-12 of the largest, say.
 // fp32: P and dS are split into planes as the operands were; there is one group, and each round's sums start from zero and are added up
 // in registers (in the accumulators, what additions cut off came to 2e-5 of the gradients of 4096 rows).
-// The workers' instructions per score bound both kernels.  2 x 4096, 16 / 4 heads of 128, bf16: 546 us with keys kept (256 blocks, not two
-// whole rounds of the GPU), 435 with rows kept; 719 TFLOP/s of the formula's five products, tensor pipe 58 and 49 %.
+// No unit is full (tensor pipe 58 % with keys kept and 49 % with rows kept, exponential unit 30 and 34 %, issue 38 and 33 %): what a round
+// waits for, scores, workers and sums handing over to each other, bounds both kernels.  2 x 4096, 16 / 4 heads of 128, bf16: 546 us with keys kept (256 blocks, not two
+// whole rounds of the GPU), 435 with rows kept; 719 TFLOP/s of the formula's five products.
 template <typename T, int DP, bool BENT, bool KEYS>
 struct GradLayout {
     using Op = Operand<T, DP>;

@@ -62,7 +62,8 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: float = 
     documents  int32 [B, Tk]: tokens see tokens of their own id; ids below zero are padding, whose q, k and v may hold anything.
                Queries have the ids of their places, or `query_documents` [B, Tq]
 
-    A query that sees nothing gives zeros and no gradient.  Values that some query of the same row of the batch sees have to be
-    finite (a probability of zero does not hide an infinity from its neighbours); padding need not be.  Gradients for q, k and v;
-    they do not depend on the order in which the GPU runs."""
+    A query that sees nothing gives zeros and no gradient.  All values but padding have to be finite, those that no query sees among
+    them (a probability of zero does not hide an infinity from its neighbours).  Gradients for q, k and v; they do not depend on the
+    order in which the GPU runs.  Of fp16 operands, the gradients of scores lose bits below 2^-28 of the largest that |grad_o| |v|
+    allows: in their row for q, in all rows that see the same block of 128 keys for k."""
     return approx_ops.torch_operators().attention(q, k, v, scale, cap, slopes, causal, prefix, documents, query_documents)
